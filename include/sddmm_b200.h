@@ -181,6 +181,100 @@ SDDMM_API int sddmm_spmm_execute(sddmm_plan_t p, const float *Pval, const float 
 SDDMM_API int sddmm_fused_execute(sddmm_plan_t p, const float *W, const float *H, const float *Sval,
                                   float *P_out, float *Y, uint32_t flags);
 
+/*
+ * Attention under a mask that is described, not listed (no counterpart in the reference, which stops at SDDMM: the sampled
+ * score product of sparse attention, with the softmax and the product with V that follow it, and their gradient).
+ * For query i and key j of one sequence with n_q queries and n_k keys, head h:
+ *
+ *   pos_i = n_k - n_q + i                                         (the last query stands at the last key)
+ *   s_ij  = cap tanh(scale q_i.k_j / cap) - slope_h |pos_i - j|   (softcap 0: no cap; slopes NULL: no bias)
+ *   seen  : j < prefix, or pos_i - window_left <= j <= pos_i + window_right   (-1: no limit; causal: -1 and 0)
+ *   lse_i = log sum_j exp s_ij  (natural),  O_i = sum_j exp(s_ij - lse_i) V_j
+ *
+ * A query that sees nothing gets O = 0 and lse = -inf, and no gradient.  A key that a query does not see takes no part in that query's
+ * results, whatever it holds (NaN and infinities included).
+ *
+ * Sequences lie one behind the other: sequence b has rows q_offsets[b] .. q_offsets[b+1] of Q and O, and of K and V rows k_offsets[b] ..
+ * k_offsets[b+1], or where k_len is given the first k_len[b] of these (slots of a cache, filled so far); k_offsets NULL: those of Q.
+ * n_seqs + 1 offsets, ascending; sequences of no queries or no keys are fine.  All of these are read on the device by every call, so a captured
+ * call follows them.  A sequence whose numbers leave the arrays (q_rows, k_rows) or the limits (max_q, max_k) is left out
+ * and reported as SDDMM_INDEX_OUT_OF_RANGE by the call, or behind SDDMM_FLAG_ASYNC by sddmm_sync().  Rows that belong to no
+ * sequence are neither read nor written (rows of K and V behind k_len: their gradients are not written).
+ *
+ * Query head h reads KV head h / (q_heads / kv_heads).  Operands are fp32, fp16 or bfloat16, all of one type; products, softmax and sums
+ * are fp32; weights are rounded to the operands' type before the product with V where the kernel is a tensor-core one
+ * (fp16, bfloat16).  head_dim: a multiple of 8 up to 128.
+ */
+enum { SDDMM_F32 = 0, SDDMM_F16 = 1, SDDMM_BF16 = 2 };
+typedef struct sddmm_attention_s *sddmm_attention_t;
+/* Rows x heads x head_dim in device memory, the last dimension contiguous; strides in elements, not negative (0 repeats, for what is
+ * only read).  What is written must not overlap itself or what the call reads. */
+typedef struct {
+    void *data;
+    int64_t row_stride, head_stride;
+} sddmm_head_array;
+typedef struct {
+    int32_t dtype, head_dim, q_heads, kv_heads;
+    int32_t n_seqs, max_q, max_k;  /* limits of the sequences' lengths: they size the launch */
+    int64_t q_rows, k_rows;        /* of the arrays, up to 2^29 */
+    float scale, softcap;
+    int32_t window_left, window_right;
+    const int32_t *q_offsets, *k_offsets, *k_len, *prefix; /* device; all but q_offsets may be NULL; prefix: n_seqs */
+    const float *slopes;                                   /* device, q_heads; or NULL */
+} sddmm_attention_desc;
+/* The plan borrows the device arrays of the description, keeps no scratch and reads nothing before a call.  The calls of one plan may
+ * overlap on different streams and in captured graphs if each has a workspace of its own. */
+SDDMM_API int sddmm_attention_plan(sddmm_handle_t h, const sddmm_attention_desc *desc, sddmm_attention_t *out);
+SDDMM_API int sddmm_attention_destroy(sddmm_attention_t a);
+/* Bytes of device memory, 16-byte aligned, that a forward (backward = 0) or backward call needs beside its arrays; may be 0. */
+SDDMM_API int sddmm_attention_workspace(sddmm_attention_t a, int backward, int64_t *bytes);
+/* lse: q_heads x q_rows fp32, or NULL.  flags: 0 or SDDMM_FLAG_ASYNC (which a captured call has to have). */
+SDDMM_API int sddmm_attention_forward(sddmm_attention_t a, const sddmm_head_array *Q, const sddmm_head_array *K, const sddmm_head_array *V,
+                                      const sddmm_head_array *O, float *lse, void *workspace, int64_t workspace_bytes, uint32_t flags);
+/* Gradients of sum(O * dO): O and lse as the forward call left them.  dK and dV of a KV head are summed over its query heads.  No
+ * atomics: the same inputs give the same bits. */
+SDDMM_API int sddmm_attention_backward(sddmm_attention_t a, const sddmm_head_array *Q, const sddmm_head_array *K, const sddmm_head_array *V,
+                                       const sddmm_head_array *O, const float *lse, const sddmm_head_array *dO, const sddmm_head_array *dQ,
+                                       const sddmm_head_array *dK, const sddmm_head_array *dV, void *workspace, int64_t workspace_bytes,
+                                       uint32_t flags);
+/* The kernel that the plan's last call launched (static storage); "none" before the first. */
+SDDMM_API const char *sddmm_attention_last_kernel(sddmm_attention_t a);
+
+/*
+ * Rotary positions (no counterpart in the reference): the first rot_dim elements of every head are rot_dim / 2 pairs, (i, i + rot_dim / 2)
+ * or interleaved (2i, 2i + 1); pair i of a row at position t is turned by the angle t * frequencies[i] (radians) and multiplied by magnitude;
+ * the rest of the head is copied.  inverse: turned back, and multiplied by the same magnitude: the gradient of the rotation.  Angles are
+ * exact to 2^-25 of half a turn for every 64-bit position.
+ *
+ * One launch turns up to four arrays of the same rows (Q and K; V with rotate = 0 is only copied), each to dst, which may be src itself
+ * with the same strides, or to listed rows of dst (a cache): row i goes to row dst_rows[i]; negative: it is not stored; n_dst_rows or more: it is
+ * left out and reported as SDDMM_INDEX_OUT_OF_RANGE, as above.  Listed rows must differ from one another.
+ */
+enum { SDDMM_ROTARY_HALF = 0, SDDMM_ROTARY_INTERLEAVED = 1 };
+typedef struct {
+    int32_t dtype, head_dim, rot_dim, layout;
+    int64_t n_rows;
+    const int64_t *positions;  /* device, n_rows; NULL: row i stands at position0 + i */
+    int64_t position0;
+    const double *frequencies; /* HOST, rot_dim / 2; read during the call */
+    float magnitude;
+    int32_t inverse;
+} sddmm_rotary_desc;
+typedef struct {
+    const void *src;
+    void *dst;
+    int64_t src_row_stride, src_head_stride, dst_row_stride, dst_head_stride; /* elements */
+    int32_t heads, rotate;
+    const int64_t *dst_rows;   /* device, n_rows; or NULL */
+    int64_t n_dst_rows;
+} sddmm_rotary_part;
+SDDMM_API int sddmm_rotary(sddmm_handle_t h, const sddmm_rotary_desc *desc, const sddmm_rotary_part *parts, int n_parts, uint32_t flags);
+/* frequencies[i] = f (kept + (1 - kept) / factor), f = base^(-2i / rot_dim): kept = 0 for original_len 0 (all frequencies scaled alike),
+ * else the pairs that turn less than low_turns times in original_len positions are scaled, those over high_turns kept, and linear
+ * between.  Host only. */
+SDDMM_API int sddmm_rotary_frequencies(int rot_dim, double base, double factor, double original_len, double low_turns,
+                                       double high_turns, double *frequencies);
+
 /* Milliseconds of the kernels of the last synchronous sddmm_execute(), sddmm_spmm_execute() or
  * sddmm_fused_execute() -- the region the reference times and prints as "Time for SDDMM with K = ..."
  * (sddmm.cu:93,109-114); -1 behind an asynchronous call.  A call that is one launch of the gather or SpMM

@@ -27,6 +27,8 @@ FLAG_KERNEL_GATHER = 0x10
 FLAG_KERNEL_PANEL = 0x20
 FLAG_KERNEL_RING = 0x40
 FLAG_OPERANDS_BF16 = 0x100
+F32, F16, BF16 = range(3)
+ROTARY_HALF, ROTARY_INTERLEAVED = range(2)
 PLAN_SKIP_VALIDATION = 0x1
 PLAN_DEVICE_INDICES = 0x2
 PLAN_FORCE_H_CHUNKS = 0x4
@@ -43,6 +45,8 @@ EXPORTED_SYMBOLS = [
     "sddmm_multi_plan_coo", "sddmm_multi_plan_destroy", "sddmm_multi_plan_get_cuts", "sddmm_multi_execute",
     "sddmm_multi_last_kernel_ms",
     "sddmm_mtx_close", "sddmm_mtx_open_ex", "sddmm_coo_save_binary", "sddmm_coo_sort_rows_gpu", "sddmm_gen_open", "sddmm_coo_is_row_sorted", "sddmm_mtx_write", "sddmm_coo_sort_rows",
+    "sddmm_attention_plan", "sddmm_attention_destroy", "sddmm_attention_workspace", "sddmm_attention_forward", "sddmm_attention_backward",
+    "sddmm_attention_last_kernel", "sddmm_rotary", "sddmm_rotary_frequencies",
 ]
 
 
@@ -60,6 +64,28 @@ class PlanInfo(C.Structure):
                 ("n_nonempty_cols", C.c_int64), ("device_bytes", C.c_int64), ("plan_ms", C.c_float),
                 ("reserved0", C.c_int32), ("n_dense_cells", C.c_int64), ("n_dense_nnz", C.c_int64),
                 ("n_hub_cols", C.c_int64)]
+
+
+class HeadArray(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class AttentionDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "head_dim", "q_heads", "kv_heads", "n_seqs", "max_q", "max_k")] + [
+        ("q_rows", C.c_int64), ("k_rows", C.c_int64), ("scale", C.c_float), ("softcap", C.c_float), ("window_left", C.c_int32),
+        ("window_right", C.c_int32)] + [(n, C.c_void_p) for n in ("q_offsets", "k_offsets", "k_len", "prefix", "slopes")]
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("head_dim", C.c_int32), ("rot_dim", C.c_int32), ("layout", C.c_int32), ("n_rows", C.c_int64),
+                ("positions", C.c_void_p), ("position0", C.c_int64), ("frequencies", C.c_void_p), ("magnitude", C.c_float),
+                ("inverse", C.c_int32)]
+
+
+class _RotaryPart(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_row_stride", C.c_int64), ("src_head_stride", C.c_int64),
+                ("dst_row_stride", C.c_int64), ("dst_head_stride", C.c_int64), ("heads", C.c_int32), ("rotate", C.c_int32),
+                ("dst_rows", C.c_void_p), ("n_dst_rows", C.c_int64)]
 
 
 _lib = None
@@ -93,6 +119,16 @@ def lib():
     L.sddmm_spmm_execute.argtypes = [vp, vp, vp, vp, u32]
     L.sddmm_fused_execute.argtypes = [vp, vp, vp, vp, vp, vp, u32]
     L.sddmm_sync.argtypes = [vp]
+    L.sddmm_attention_plan.argtypes = [vp, C.POINTER(AttentionDesc), C.POINTER(vp)]
+    L.sddmm_attention_destroy.argtypes = [vp]
+    L.sddmm_attention_workspace.argtypes = [vp, C.c_int, C.POINTER(i64)]
+    heads = C.POINTER(HeadArray)
+    L.sddmm_attention_forward.argtypes = [vp, heads, heads, heads, heads, vp, vp, i64, u32]
+    L.sddmm_attention_backward.argtypes = [vp, heads, heads, heads, heads, vp, heads, heads, heads, heads, vp, i64, u32]
+    L.sddmm_attention_last_kernel.restype = C.c_char_p
+    L.sddmm_attention_last_kernel.argtypes = [vp]
+    L.sddmm_rotary.argtypes = [vp, C.POINTER(RotaryDesc), C.POINTER(_RotaryPart), C.c_int, u32]
+    L.sddmm_rotary_frequencies.argtypes = [C.c_int] + [C.c_double] * 5 + [vp]
     L.sddmm_kernel_launches.argtypes = [vp, C.POINTER(i64)]
     L.sddmm_check_result.argtypes = [vp, vp, vp, vp, vp, i64, C.c_double, C.POINTER(C.c_double), C.POINTER(i64),
                                      C.POINTER(i64)]
@@ -305,12 +341,184 @@ class Handle:
         keep = (rows, cols) if is_dev else None  # device indices are borrowed, keep them alive
         return Plan(self, p, nnz, keep)
 
+    def attention_plan(self, dtype, head_dim, q_heads, kv_heads, q_offsets, max_q, max_k, k_offsets=None, k_len=None, prefix=None,
+                       slopes=None, scale=None, softcap=0.0, window=(-1, -1), q_rows=None, k_rows=None):
+        """Attention over sequences that lie one behind the other (sddmm_attention_plan); scale None: 1 / sqrt(head_dim).
+
+        q_offsets, k_offsets, k_len, prefix: int32 CUDA tensors, slopes: float32.  q_rows, k_rows: rows of the arrays, by default
+        the last offset (which is then read back once, here); without k_offsets K and V have the rows of Q."""
+        import torch
+        n = q_offsets.shape[0] - 1
+        if q_rows is None:
+            q_rows = int(q_offsets[-1])
+        if k_rows is None:
+            k_rows = q_rows if k_offsets is None else int(k_offsets[-1])
+        at = [_cuda_vector(a, name, t, m, self.device) for a, name, t, m in (
+            (q_offsets, "q_offsets", torch.int32, n + 1), (k_offsets, "k_offsets", torch.int32, n + 1), (k_len, "k_len", torch.int32, n),
+            (prefix, "prefix", torch.int32, n), (slopes, "slopes", torch.float32, q_heads))]
+        d = AttentionDesc(_dtype(dtype), head_dim, q_heads, kv_heads, n, max_q, max_k, q_rows, k_rows,
+                          max(head_dim, 1) ** -0.5 if scale is None else scale, softcap, window[0], window[1], *at)
+        return Attention(self, d, dtype, (q_offsets, k_offsets, k_len, prefix, slopes))
+
+    def rotary(self, parts, positions, frequencies, layout="half", inverse=False, magnitude=1.0, flags=0):
+        """Turn the pairs of up to four arrays of the same rows (RotaryPart) by position * frequency (sddmm_rotary).
+
+        positions: int64 CUDA tensor, one for each row, or the int position of the first row; frequencies: float64 numpy
+        array, radians a position of every pair; layout: "half" or "interleaved"; inverse: the gradient of the rotation."""
+        import torch
+        if not 1 <= len(parts) <= 4:
+            raise ValueError("one to four parts")
+        x = parts[0].src
+        n, d, dtype = x.shape[0], x.shape[2], x.dtype
+        array = (_RotaryPart * len(parts))()
+        for i, p in enumerate(parts):
+            for t in (p.src, p.dst):
+                if t.dim() != 3 or t.shape[2] != d or t.shape[1] != p.src.shape[1] or t.dtype != dtype or t.stride(2) != 1 and d > 1 or \
+                        t.get_device() != self.device:
+                    raise ValueError(f"part {i} must be tensors (rows, heads, {d}) of {dtype} on cuda:{self.device} with contiguous heads")
+            if p.src.shape[0] != n or p.rows is None and p.dst.shape[0] != n:
+                raise ValueError(f"part {i} has other rows than the first")
+            rows = _cuda_vector(p.rows, "rows", torch.int64, n, self.device)
+            array[i] = _RotaryPart(p.src.data_ptr(), p.dst.data_ptr(), p.src.stride(0), p.src.stride(1), p.dst.stride(0), p.dst.stride(1),
+                                   p.src.shape[1], p.rotate, rows, p.dst.shape[0])
+        f = np.ascontiguousarray(frequencies, np.float64)
+        at = None if isinstance(positions, int) else _cuda_vector(positions, "positions", torch.int64, n, self.device)
+        desc = RotaryDesc(_dtype(dtype), d, 2 * f.shape[0], ("half", "interleaved").index(layout), n, at,
+                          positions if at is None else 0, f.ctypes.data, magnitude, inverse)
+        self._follow_torch_stream(x)
+        st = _lib.sddmm_rotary(self._h, desc, array, len(parts), flags)
+        if st:
+            self._check(st)
+
     def sddmm_coo(self, M, N, rows, cols, W, H, K, P, Sval=None, nnz=None):
         if nnz is None:
             nnz = int(rows.shape[0])
         self._follow_torch_stream(rows, cols, W, H, P, Sval)
         self._check(lib().sddmm_coo(self._h, M, N, nnz, _ptr(rows), _ptr(cols), _ptr(Sval), _ptr(W), _ptr(H), K,
                                     _ptr(P)))
+
+
+class RotaryPart:
+    """One array of a Handle.rotary() call: rows x heads x head_dim, turned (rotate) or only copied to dst, or to the listed
+    rows of dst (int64 CUDA tensor; negative: not stored)."""
+    __slots__ = ("src", "dst", "rows", "rotate")
+
+    def __init__(self, src, dst=None, rows=None, rotate=True):
+        self.src, self.dst, self.rows, self.rotate = src, src if dst is None else dst, rows, rotate
+
+
+_TYPES = {}
+
+
+def _dtype(t):
+    """F32, F16 or BF16 of a torch dtype."""
+    if not _TYPES:
+        import torch
+        _TYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    if t not in _TYPES:
+        raise TypeError(f"dtype {t}: torch.float32, float16 or bfloat16 is wanted")
+    return _TYPES[t]
+
+
+def _cuda_vector(a, name, dtype, n, device):
+    """Address of a contiguous CUDA tensor of this type with n values; None stays None."""
+    if a is None:
+        return None
+    if not _is_cuda_tensor(a) or a.dim() != 1 or a.shape[0] != n or a.dtype != dtype or not a.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous CUDA tensor of {n} values of {dtype}")
+    if a.device.index != device:
+        raise ValueError(f"{name} is on {a.device}, the engine on cuda:{device}")
+    return a.data_ptr()
+
+
+class Attention:
+    """Attention under a described mask, forward and backward (sddmm_attention_plan; Handle.attention_plan()).
+
+    Arrays are CUDA tensors of shape (rows, heads, head_dim), the last dimension contiguous, any other strides.  Lengths, offsets and
+    masks are read on the GPU at every call: they may change in place between calls and between replays of a captured
+    call.  Workspace comes from torch's allocator in every call, in a captured call from its graph's pool."""
+
+    def __init__(self, handle, desc, dtype, keep):
+        self.handle = handle
+        self.desc = desc
+        self._dtype = dtype
+        self._keep = keep  # the plan borrows these
+        self._a = C.c_void_p()
+        handle._check(lib().sddmm_attention_plan(handle._h, C.byref(desc), C.byref(self._a)))
+        n = C.c_int64()
+        self._bytes = []
+        for backward in (0, 1):
+            handle._check(lib().sddmm_attention_workspace(self._a, backward, C.byref(n)))
+            self._bytes.append(n.value)
+        d = desc
+        self._shape_q, self._shape_k = (d.q_rows, d.q_heads, d.head_dim), (d.k_rows, d.kv_heads, d.head_dim)
+
+    def close(self):
+        if self._a:
+            lib().sddmm_attention_destroy(self._a)
+            self._a = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _heads(self, t, shape, name):
+        if t.shape != shape or t.dtype != self._dtype or t.stride(2) != 1 and t.shape[2] > 1 or t.get_device() != self.handle.device:
+            raise ValueError(f"{name} must be a tensor {tuple(shape)} of {self._dtype} on cuda:{self.handle.device} with contiguous heads, "
+                             f"got {tuple(t.shape)} of {t.dtype} on {t.device}, strides {t.stride()}")
+        return HeadArray(t.data_ptr(), t.stride(0), t.stride(1))
+
+    def _lse(self, lse):
+        if lse.shape != (self.desc.q_heads, self.desc.q_rows) or str(lse.dtype) != "torch.float32" or not lse.is_contiguous() or \
+                lse.get_device() != self.handle.device:
+            raise ValueError(f"lse must be a contiguous float32 tensor {(self.desc.q_heads, self.desc.q_rows)} on cuda:{self.handle.device}")
+        return lse.data_ptr()
+
+    def _workspace(self, backward, like):
+        import torch
+        n = self._bytes[backward]
+        return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None
+
+    def forward(self, Q, K, V, O, lse=None, flags=0):
+        """O (and lse, heads x rows, natural log) of the whole batch; returns O."""
+        h = self.handle
+        q, k, v, o = (self._heads(Q, self._shape_q, "Q"), self._heads(K, self._shape_k, "K"), self._heads(V, self._shape_k, "V"),
+                      self._heads(O, self._shape_q, "O"))
+        l = None if lse is None else self._lse(lse)
+        h._follow_torch_stream(Q)
+        w = self._workspace(0, Q)
+        st = _lib.sddmm_attention_forward(self._a, q, k, v, o, l, w.data_ptr() if w is not None else None, self._bytes[0], flags)
+        if st:
+            h._check(st)
+        return O
+
+    def backward(self, Q, K, V, O, lse, dO, dQ, dK, dV, flags=0):
+        """Gradients of sum(O * dO) into dQ, dK, dV; O and lse from forward()."""
+        h = self.handle
+        arrays = [self._heads(t, s, n) for t, s, n in (
+            (Q, self._shape_q, "Q"), (K, self._shape_k, "K"), (V, self._shape_k, "V"), (O, self._shape_q, "O"), (dO, self._shape_q, "dO"),
+            (dQ, self._shape_q, "dQ"), (dK, self._shape_k, "dK"), (dV, self._shape_k, "dV"))]
+        l = self._lse(lse)
+        h._follow_torch_stream(Q)
+        w = self._workspace(1, Q)
+        st = _lib.sddmm_attention_backward(self._a, *arrays[:4], l, *arrays[4:], w.data_ptr() if w is not None else None, self._bytes[1], flags)
+        if st:
+            h._check(st)
+        return dQ, dK, dV
+
+    def last_kernel_name(self):
+        return lib().sddmm_attention_last_kernel(self._a).decode()
+
+
+def rotary_frequencies(rot_dim, base=10000.0, factor=1.0, original_len=0.0, low_turns=1.0, high_turns=32.0):
+    """Radians a position of the rot_dim / 2 pairs (float64), scaled for a longer context (sddmm_rotary_frequencies)."""
+    out = np.empty(max(rot_dim, 0) // 2, np.float64)
+    st = lib().sddmm_rotary_frequencies(rot_dim, base, factor, original_len, low_turns, high_turns, out.ctypes.data)
+    if st != OK:
+        raise SddmmError(st)
+    return out
 
 
 class Plan:

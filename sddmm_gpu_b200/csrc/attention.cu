@@ -1,0 +1,203 @@
+// C entries of attention under a described mask: plan, checks of arguments, choice of the kernel.
+#include <cuda_runtime.h>
+
+#include <climits>
+#include <cmath>
+#include <new>
+#include <string>
+
+#include "attention.cuh"
+#include "device_guard.hpp"
+#include "engine_internal.hpp"
+#include "sddmm_b200.h"
+
+struct sddmm_attention_s {
+    sddmm_handle_s *h = nullptr;
+    AttentionParams p{};
+    const char *last_kernel = "none";
+};
+
+namespace {
+
+constexpr int64_t MAX_ROWS = 1 << 29;
+constexpr int MAX_WINDOW = (1 << 30) - 1;  // more than any distance
+constexpr int MAX_HEAD_DIM = 128;
+
+int bad(sddmm_handle_s *h, const char *why)
+{
+    h->last_error = why;
+    return SDDMM_INVALID_ARG;
+}
+
+// An array of the call: in memory of the handle's GPU, aligned to its elements.  rows 0: it may be anything.
+int check_array(sddmm_handle_s *h, const sddmm_head_array *a, const char *name, int dtype, int head_dim, int heads, int64_t rows, bool written,
+                HeadArray *out)
+{
+    const size_t size = dtype == SDDMM_F32 ? 4 : 2;
+    if (!a) {
+        h->last_error = std::string(name) + " is missing";
+        return SDDMM_INVALID_ARG;
+    }
+    *out = HeadArray{a->data, a->row_stride, a->head_stride};
+    if (rows == 0) return SDDMM_OK;
+    if (!on_device(a->data, h->device) || (uintptr_t)a->data % size != 0) {
+        h->last_error = std::string(name) + " must be device memory of the handle's GPU, aligned to its elements";
+        return SDDMM_INVALID_ARG;
+    }
+    if (a->row_stride < 0 || a->head_stride < 0) {
+        h->last_error = std::string(name) + " has a negative stride";
+        return SDDMM_INVALID_ARG;
+    }
+    if (written && !(strides_apart(a->head_stride, heads, a->row_stride, rows, head_dim))) {
+        h->last_error = std::string(name) + " is written, and its strides let entries overlap";
+        return SDDMM_INVALID_ARG;
+    }
+    return SDDMM_OK;
+}
+
+bool capturing(cudaStream_t s)
+{
+    cudaStreamCaptureStatus c = cudaStreamCaptureStatusNone;
+    return cudaStreamIsCapturing(s, &c) == cudaSuccess && c != cudaStreamCaptureStatusNone;
+}
+
+int finish(sddmm_attention_s *a, cudaError_t e, const char *name, int launches, uint32_t flags)
+{
+    sddmm_handle_s *h = a->h;
+    if (e == cudaSuccess) {
+        a->last_kernel = name;
+        h->n_launches += launches;
+        if (flags & SDDMM_FLAG_ASYNC) return SDDMM_OK;
+        e = cudaStreamSynchronize(h->stream);
+        if (e == cudaSuccess) return device_status(h);
+    }
+    h->last_error = std::string(name) + ": " + cudaGetErrorString(e);
+    (void)cudaGetLastError();
+    return SDDMM_CUDA_ERROR;
+}
+
+}  // namespace
+
+int sddmm_attention_plan(sddmm_handle_t h, const sddmm_attention_desc *d, sddmm_attention_t *out)
+{
+    if (!h || !out) return SDDMM_INVALID_ARG;
+    *out = nullptr;
+    if (!d) return bad(h, "no description");
+    if (d->dtype != SDDMM_F32 && d->dtype != SDDMM_F16 && d->dtype != SDDMM_BF16) return bad(h, "unknown dtype");
+    if (d->head_dim < 8 || d->head_dim > MAX_HEAD_DIM || d->head_dim % 8) {
+        h->last_error = "head_dim must be a multiple of 8 from 8 to 128";
+        return SDDMM_K_UNSUPPORTED;
+    }
+    if (d->q_heads < 1 || d->kv_heads < 1 || d->q_heads % d->kv_heads) return bad(h, "q_heads must be a multiple of kv_heads");
+    if (d->n_seqs < 0 || d->max_q < 0 || d->max_k < 0) return bad(h, "negative size");
+    if (d->q_rows < 0 || d->q_rows > MAX_ROWS || d->k_rows < 0 || d->k_rows > MAX_ROWS) return bad(h, "q_rows and k_rows go from 0 to 2^29");
+    if (!(d->scale > 0.f) || !std::isfinite(d->scale)) return bad(h, "scale must be positive and finite");
+    if (!(d->softcap >= 0.f) || !std::isfinite(d->softcap)) return bad(h, "softcap must be 0 (none) or positive and finite");
+    if (d->window_left < -1 || d->window_right < -1) return bad(h, "a window's side is -1 (no limit), 0 or positive");
+    DeviceGuard guard(h->device);
+    if (d->n_seqs > 0 && !on_device(d->q_offsets, h->device)) return bad(h, "q_offsets must be device memory of the handle's GPU");
+    if (d->k_len && !d->k_offsets) return bad(h, "k_len goes with k_offsets");
+    const void *more[] = {d->k_offsets, d->k_len, d->prefix, d->slopes};
+    for (const void *x : more)
+        if (x && d->n_seqs > 0 && !on_device(x, h->device)) return bad(h, "k_offsets, k_len, prefix and slopes must be device memory of the handle's GPU");
+    AttentionParams p{};
+    p.dtype = d->dtype;
+    p.head_dim = d->head_dim;
+    p.q_heads = d->q_heads;
+    p.kv_heads = d->kv_heads;
+    p.group = d->q_heads / d->kv_heads;
+    p.n_seqs = d->n_seqs;
+    p.q_rows = d->q_rows;
+    p.k_rows = d->k_offsets ? d->k_rows : d->q_rows;
+    if (!d->k_offsets && d->k_rows != d->q_rows) return bad(h, "without k_offsets K has the rows of Q");
+    p.max_q = (int)(d->max_q < d->q_rows ? d->max_q : d->q_rows);
+    p.max_k = (int)(d->max_k < p.k_rows ? d->max_k : p.k_rows);
+    p.scale = d->scale;
+    p.cap = d->softcap;
+    p.window.left = d->window_left < MAX_WINDOW ? d->window_left : MAX_WINDOW;
+    p.window.right = d->window_right < MAX_WINDOW ? d->window_right : MAX_WINDOW;
+    p.q_offsets = d->q_offsets;
+    p.k_offsets = d->k_offsets;
+    p.k_len = d->k_len;
+    p.prefix = d->prefix;
+    p.slopes = d->slopes;
+    p.status = h->d_status;
+    if ((most_blocks(p.q_rows, p.n_seqs, p.max_q, 16) + 1) * p.q_heads > INT_MAX || (most_blocks(p.k_rows, p.n_seqs, p.max_k, 64) + 1) * p.q_heads > INT_MAX)
+        return bad(h, "too many heads and rows for one launch");
+    sddmm_attention_s *a = new (std::nothrow) sddmm_attention_s;
+    if (!a) return SDDMM_OUT_OF_MEMORY;
+    a->h = h;
+    a->p = p;
+    *out = a;
+    return SDDMM_OK;
+}
+
+int sddmm_attention_destroy(sddmm_attention_t a)
+{
+    delete a;
+    return SDDMM_OK;
+}
+
+int sddmm_attention_workspace(sddmm_attention_t a, int backward, int64_t *bytes)
+{
+    if (!a || !bytes) return SDDMM_INVALID_ARG;
+    *bytes = backward ? (int64_t)sizeof(float) * a->p.q_heads * a->p.q_rows : 0;
+    return SDDMM_OK;
+}
+
+int sddmm_attention_forward(sddmm_attention_t a, const sddmm_head_array *Q, const sddmm_head_array *K, const sddmm_head_array *V,
+                            const sddmm_head_array *O, float *lse, void *workspace, int64_t workspace_bytes, uint32_t flags)
+{
+    if (!a) return SDDMM_INVALID_ARG;
+    sddmm_handle_s *h = a->h;
+    if (flags & ~(uint32_t)SDDMM_FLAG_ASYNC) return bad(h, "unknown flag");
+    AttentionParams p = a->p;
+    DeviceGuard guard(h->device);
+    int st;
+    if ((st = check_array(h, Q, "Q", p.dtype, p.head_dim, p.q_heads, p.q_rows, false, &p.q))) return st;
+    if ((st = check_array(h, K, "K", p.dtype, p.head_dim, p.kv_heads, p.k_rows, false, &p.k))) return st;
+    if ((st = check_array(h, V, "V", p.dtype, p.head_dim, p.kv_heads, p.k_rows, false, &p.v))) return st;
+    if ((st = check_array(h, O, "O", p.dtype, p.head_dim, p.q_heads, p.q_rows, true, &p.o))) return st;
+    if (lse && p.q_rows > 0 && !on_device(lse, h->device)) return bad(h, "lse must be device memory of the handle's GPU");
+    p.lse = lse;
+    int64_t need = 0;
+    sddmm_attention_workspace(a, 0, &need);
+    if (need > 0 && (workspace_bytes < need || !on_device(workspace, h->device) || (uintptr_t)workspace % 16))
+        return bad(h, "workspace: sddmm_attention_workspace() bytes of device memory, 16-byte aligned");
+    if (!(flags & SDDMM_FLAG_ASYNC) && capturing(h->stream)) return bad(h, "a captured call must be asynchronous");
+    if (p.n_seqs == 0 || p.max_q == 0) return SDDMM_OK;
+    return finish(a, launch_attention_forward_general(p, h->stream), "attention_general", 1, flags);
+}
+
+int sddmm_attention_backward(sddmm_attention_t a, const sddmm_head_array *Q, const sddmm_head_array *K, const sddmm_head_array *V,
+                             const sddmm_head_array *O, const float *lse, const sddmm_head_array *dO, const sddmm_head_array *dQ,
+                             const sddmm_head_array *dK, const sddmm_head_array *dV, void *workspace, int64_t workspace_bytes,
+                             uint32_t flags)
+{
+    if (!a) return SDDMM_INVALID_ARG;
+    sddmm_handle_s *h = a->h;
+    if (flags & ~(uint32_t)SDDMM_FLAG_ASYNC) return bad(h, "unknown flag");
+    AttentionParams p = a->p;
+    DeviceGuard guard(h->device);
+    int st;
+    if ((st = check_array(h, Q, "Q", p.dtype, p.head_dim, p.q_heads, p.q_rows, false, &p.q))) return st;
+    if ((st = check_array(h, K, "K", p.dtype, p.head_dim, p.kv_heads, p.k_rows, false, &p.k))) return st;
+    if ((st = check_array(h, V, "V", p.dtype, p.head_dim, p.kv_heads, p.k_rows, false, &p.v))) return st;
+    if ((st = check_array(h, O, "O", p.dtype, p.head_dim, p.q_heads, p.q_rows, false, &p.o))) return st;
+    if ((st = check_array(h, dO, "dO", p.dtype, p.head_dim, p.q_heads, p.q_rows, false, &p.d_o))) return st;
+    if ((st = check_array(h, dQ, "dQ", p.dtype, p.head_dim, p.q_heads, p.q_rows, true, &p.dq))) return st;
+    if ((st = check_array(h, dK, "dK", p.dtype, p.head_dim, p.kv_heads, p.k_rows, true, &p.dk))) return st;
+    if ((st = check_array(h, dV, "dV", p.dtype, p.head_dim, p.kv_heads, p.k_rows, true, &p.dv))) return st;
+    if (p.q_rows > 0 && !on_device(lse, h->device)) return bad(h, "lse must be device memory of the handle's GPU");
+    p.lse = const_cast<float *>(lse);
+    int64_t need = 0;
+    sddmm_attention_workspace(a, 1, &need);
+    if (need > 0 && (workspace_bytes < need || !on_device(workspace, h->device) || (uintptr_t)workspace % 16))
+        return bad(h, "workspace: sddmm_attention_workspace() bytes of device memory, 16-byte aligned");
+    p.delta = static_cast<float *>(workspace);
+    if (!(flags & SDDMM_FLAG_ASYNC) && capturing(h->stream)) return bad(h, "a captured call must be asynchronous");
+    if (p.n_seqs == 0 || (p.max_q == 0 && p.max_k == 0)) return SDDMM_OK;
+    return finish(a, launch_attention_backward_general(p, h->stream), "attention_backward_general", 2, flags);
+}
+
+const char *sddmm_attention_last_kernel(sddmm_attention_t a) { return a ? a->last_kernel : "none"; }

@@ -1,0 +1,106 @@
+// Attention over a mask that is described, not listed: what its kernels share.
+//
+//   s_ij   = cap tanh(scale q_i.k_j / cap) - slope_h |pos_i - j|,   pos_i = n_k - n_q + i
+//   seen   : j < prefix, or pos_i - left <= j <= pos_i + right
+//   lse_i  = log sum_j exp s_ij,   O_i = sum_j exp(s_ij - lse_i) V_j;   nothing seen: O_i = 0, lse_i = -inf
+//
+// for the queries i and keys j of one sequence of a batch.  Sequences lie one behind the other in Q, and packed or in slots in K and
+// V; offsets and lengths are read on the device, and a sequence whose numbers leave the arrays or the plan's limits is
+// left out and reported.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "attention_mask.hpp"
+#include "common.cuh"
+
+namespace sddmm {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+struct HeadArray {  // rows x heads x head_dim, the last dimension contiguous
+    void *data;
+    int64_t row, head;  // strides in elements
+};
+
+struct AttentionParams {
+    int n_seqs, q_heads, kv_heads, group, head_dim, dtype;
+    int max_q, max_k;
+    int64_t q_rows, k_rows;
+    float scale, cap;  // cap 0: none
+    Window window;
+    const int32_t *q_offsets, *k_offsets, *k_len, *prefix;
+    const float *slopes;
+    HeadArray q, k, v, o, d_o, dq, dk, dv;
+    float *lse;    // q_heads x q_rows
+    float *delta;  // q_heads x q_rows, workspace of the backward pass
+    float *part_o, *part_lse;  // parts of a split long axis (workspace)
+    int n_splits;
+    int *status;
+};
+
+__device__ __forceinline__ void report_bad_index(int *dev_status)
+{
+    *reinterpret_cast<volatile int *>(dev_status) = (int)DEV_BAD_INDEX;
+    __threadfence_system();
+}
+
+// Sequence b; one whose numbers are not good (negative, outside the arrays, above the plan's limits) counts as empty.
+__device__ __forceinline__ Sequence sequence_of(const AttentionParams &p, int b)
+{
+    Sequence s;
+    s.q0 = __ldg(p.q_offsets + b);
+    s.nq = __ldg(p.q_offsets + b + 1) - s.q0;
+    const int32_t *ko = p.k_offsets ? p.k_offsets : p.q_offsets;
+    s.k0 = __ldg(ko + b);
+    const int room = __ldg(ko + b + 1) - s.k0;
+    s.nk = p.k_len ? __ldg(p.k_len + b) : room;
+    s.prefix = p.prefix ? max(0, min(__ldg(p.prefix + b), s.nk)) : 0;
+    const bool good = s.q0 >= 0 && s.nq >= 0 && s.nq <= p.max_q && (int64_t)s.q0 + s.nq <= p.q_rows && s.k0 >= 0 && s.nk >= 0 &&
+                      s.nk <= room && s.nk <= p.max_k && (int64_t)s.k0 + s.nk <= p.k_rows;
+    if (!good) {
+        report_bad_index(p.status);
+        s.q0 = s.nq = s.k0 = s.nk = s.prefix = 0;
+    }
+    return s;
+}
+
+// Block `index` of ceil(n / T) blocks per sequence, over all sequences: its sequence and its number there.  Returns false behind
+// the last one.  keys: blocks of keys, else of queries.  All threads of a warp call it together.
+template <int T>
+__device__ __forceinline__ bool find_block(const AttentionParams &p, int index, bool keys, Sequence &s, int &seq, int &number)
+{
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    for (int b0 = 0; b0 < p.n_seqs; b0 += 32) {
+        const int b = b0 + lane;
+        Sequence mine = {};
+        if (b < p.n_seqs) mine = sequence_of(p, b);
+        const int blocks = ((keys ? mine.nk : mine.nq) + T - 1) / T;
+        int sum = blocks;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, index < before + sum);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            number = index - before - __shfl_sync(0xffffffffu, sum - blocks, l);
+            seq = b0 + l;
+            s.q0 = __shfl_sync(0xffffffffu, mine.q0, l);
+            s.nq = __shfl_sync(0xffffffffu, mine.nq, l);
+            s.k0 = __shfl_sync(0xffffffffu, mine.k0, l);
+            s.nk = __shfl_sync(0xffffffffu, mine.nk, l);
+            s.prefix = __shfl_sync(0xffffffffu, mine.prefix, l);
+            return true;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return false;
+}
+cudaError_t launch_attention_forward_general(const AttentionParams &p, cudaStream_t s);
+cudaError_t launch_attention_backward_general(const AttentionParams &p, cudaStream_t s);
+
+}  // namespace sddmm

@@ -78,8 +78,8 @@ inline cudaError_t optin_dynamic_smem(Kern kern, size_t bytes, SmemOptinCache &c
     return e;
 }
 
-// Device status word written by kernels whose bounded waits give up.
-enum DeviceStatus : int { DEV_OK = 0, DEV_MBARRIER_TIMEOUT = 1 };
+// Device status word: written by kernels whose bounded waits give up, or that met an index outside its array and left it out.
+enum DeviceStatus : int { DEV_OK = 0, DEV_MBARRIER_TIMEOUT = 1, DEV_BAD_INDEX = 2 };
 
 struct PanelConfig {
     int panel_rows;      // rows of W per staged panel

@@ -18,6 +18,7 @@
 
 #include "binning.cuh"
 #include "common.cuh"
+#include "device_guard.hpp"
 #include "gather_index.hpp"
 #include "sddmm_b200.h"
 
@@ -225,10 +226,12 @@ struct CallTimer {
 int check_device_status(sddmm_handle_s *h)
 {
     volatile int *status = h->h_status;
-    if (*status != DEV_OK) {
-        h->last_error = "a bounded device-side wait (mbarrier) gave up";
+    const int found = *status;
+    if (found != DEV_OK) {
         *status = DEV_OK;
-        return SDDMM_DEVICE_TIMEOUT;
+        h->last_error = found == DEV_BAD_INDEX ? "an offset, length or row index on the device leaves its array or the plan's limits; what it names was left out"
+                                               : "a bounded device-side wait (mbarrier) gave up";
+        return found == DEV_BAD_INDEX ? SDDMM_INDEX_OUT_OF_RANGE : SDDMM_DEVICE_TIMEOUT;
     }
     return SDDMM_OK;
 }
@@ -426,6 +429,8 @@ cudaError_t launch_rows(sddmm_plan_s *p, const int32_t *rows, const int32_t *col
 }
 
 }  // namespace sddmm
+
+int sddmm::device_status(sddmm_handle_s *h) { return check_device_status(h); }
 
 extern "C" {
 
