@@ -166,6 +166,9 @@ int sddmm_attention_forward(sddmm_attention_t a, const sddmm_head_array *Q, cons
         return bad(h, "workspace: sddmm_attention_workspace() bytes of device memory, 16-byte aligned");
     if (!(flags & SDDMM_FLAG_ASYNC) && capturing(h->stream)) return bad(h, "a captured call must be asynchronous");
     if (p.n_seqs == 0 || p.max_q == 0) return SDDMM_OK;
+    bool taken = false;
+    const cudaError_t e = launch_attention_forward_tc(p, &taken, h->stream);
+    if (taken) return finish(a, e, "attention_tc", 1, flags);
     return finish(a, launch_attention_forward_general(p, h->stream), "attention_general", 1, flags);
 }
 

@@ -82,7 +82,7 @@ __device__ __forceinline__ bool no_number_left(const float (&x)[PER_LANE], int D
 
 // One warp: O of query i from its lse.
 template <class T>
-__device__ __noinline__ void output_row(const AttentionParams &p, const Sequence &s, int head, int i, float lse)
+__device__ __forceinline__ void output_row(const AttentionParams &p, const Sequence &s, int head, int i, float lse)
 {
     if (isnan(lse)) return;
     const int kv = head / p.group, pos = s.nk - s.nq + i;
@@ -102,7 +102,7 @@ __device__ __noinline__ void output_row(const AttentionParams &p, const Sequence
 
 // One warp: dQ of query i.
 template <class T>
-__device__ __noinline__ void dq_row(const AttentionParams &p, const Sequence &s, int head, int i, float lse, float delta)
+__device__ __forceinline__ void dq_row(const AttentionParams &p, const Sequence &s, int head, int i, float lse, float delta)
 {
     if (isnan(lse) || isnan(delta)) return;
     const int kv = head / p.group, pos = s.nk - s.nq + i;
@@ -124,7 +124,7 @@ __device__ __noinline__ void dq_row(const AttentionParams &p, const Sequence &s,
 
 // One warp: dK and dV of key j.
 template <class T>
-__device__ __noinline__ void dkv_row(const AttentionParams &p, const Sequence &s, int kv, int j)
+__device__ __forceinline__ void dkv_row(const AttentionParams &p, const Sequence &s, int kv, int j)
 {
     float k[PER_LANE], v[PER_LANE], q[PER_LANE], d_o[PER_LANE], dk[PER_LANE] = {}, dv[PER_LANE] = {}, dcap;
     load<T>(k, p.k, (int64_t)s.k0 + j, kv, p.head_dim);

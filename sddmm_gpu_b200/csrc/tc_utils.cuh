@@ -1,0 +1,164 @@
+// Tensor-core building blocks of the attention kernels: tile copies (TMA), shared-memory and instruction descriptors of tcgen05.mma with
+// 16-bit operands, tensor memory, bounded waits.
+//
+// Operand tiles lie in shared memory as boxes of 64 elements (128 bytes) by some rows, with the 128-byte swizzle: the 16-byte piece c of
+// row r sits at piece c ^ (r % 8) of the row's line; eight rows are 1,024 bytes.  Two ways to read such a box:
+//   K-major  (the 64 elements are the product's K): 16 of them, a K step, are 32 bytes further in every line;
+//   MN-major (the rows are the product's K): a K step is 16 rows, 2,048 bytes; boxes beside one another continue M or N.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "attention.cuh"
+#include "device_utils.cuh"
+
+namespace sddmm {
+namespace tc {
+
+using dev::mbar_arrive;
+using dev::mbar_fence_init;
+using dev::mbar_init;
+using dev::mbar_try_wait;
+using dev::smem_u32;
+
+// Shared-memory matrix descriptor: start address, leading / stride byte offsets (all >> 4), version 1, 128-byte swizzle.
+// K-major: stride = 1,024 (from eight rows to the next), leading unused.  MN-major: stride = 1,024 (from eight K rows to the
+// next), leading = bytes from a box of 64 to the one that continues M or N.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo_bytes)
+{
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)((lbo_bytes >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024u >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// Instruction descriptor of kind::f16: D fp32, A and B both fp16 or both bfloat16, K-major or MN-major each.
+__host__ __device__ constexpr uint32_t instr_desc(bool bf16, int M, int N, bool a_mn, bool b_mn)
+{
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
+           ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// D (tensor memory) = or += A B^T, one K step of 16; A from shared memory or (ts) from tensor memory, two elements a column.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+                 "l"(b), "r"(idesc), "r"((uint32_t)add)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+                 "l"(b), "r"(idesc), "r"((uint32_t)add)
+                 : "memory");
+}
+// Arrives on the barrier when all MMAs that this thread has issued are complete.
+__device__ __forceinline__ void commit(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tmem_alloc(uint32_t *holder, uint32_t columns)
+{
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(holder)), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t tmem, uint32_t columns)
+{
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+}
+
+// 32 columns of this warp's 32 lanes, a lane's row in a thread; loads are complete behind wait_ld().
+#define TC_R8(m, v, i) m(v[i]), m(v[i + 1]), m(v[i + 2]), m(v[i + 3]), m(v[i + 4]), m(v[i + 5]), m(v[i + 6]), m(v[i + 7])
+#define TC_OUT(x) "=r"(x)
+#define TC_IN(x) "r"(x)
+__device__ __forceinline__ void tmem_ld32(uint32_t *v, uint32_t taddr)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+        "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : TC_R8(TC_OUT, v, 0), TC_R8(TC_OUT, v, 8), TC_R8(TC_OUT, v, 16), TC_R8(TC_OUT, v, 24)
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *v)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+        "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::TC_R8(TC_IN, v, 0), TC_R8(TC_IN, v, 8), TC_R8(TC_IN, v, 16),
+        TC_R8(TC_IN, v, 24), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::TC_R8(TC_IN, v, 0),
+        TC_R8(TC_IN, v, 8), "r"(taddr)
+        : "memory");
+}
+
+__device__ __forceinline__ void expect_bytes(uint64_t *bar, uint32_t bytes)
+{
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+// Box of a rows x heads x head_dim array: elements from `x` on (a multiple of 64), one head, rows from `row` on.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, int x, int head, int row, uint64_t *bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
+        "r"(x), "r"(head), "r"(row), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Bounded wait of a thread.  try_wait suspends the thread by itself, so there is no sleep between polls; the limit is wall-clock time, with
+// a count behind it.
+static __device__ __forceinline__ bool wait_long(uint64_t *bar, unsigned parity)
+{
+    dev::WaitClock clock;
+#pragma unroll 1
+    for (int it = 0; it < dev::MBAR_SPIN_LIMIT; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (clock.expired(it)) return false;
+    }
+    return false;
+}
+__device__ __forceinline__ bool wait(uint64_t *bar, unsigned parity) { return mbar_try_wait(bar, parity) || wait_long(bar, parity); }
+
+// The same for a whole warp: one answer for all of its threads.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, unsigned parity) { return __all_sync(0xffffffffu, wait(bar, parity)); }
+
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Two values in a word, the first in its lower half.
+template <class T> __device__ __forceinline__ uint32_t pack(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b)
+{
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+
+}  // namespace tc
+
+// Tensor map of one array for boxes of 64 elements x `box_rows` rows; false where the array cannot have one (strides, alignment).
+bool make_tensor_map(CUtensorMap *map, const HeadArray &a, int dtype, int head_dim, int heads, int64_t rows, int box_rows);
+
+}  // namespace sddmm
