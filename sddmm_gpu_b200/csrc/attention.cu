@@ -200,6 +200,9 @@ int sddmm_attention_backward(sddmm_attention_t a, const sddmm_head_array *Q, con
     p.delta = static_cast<float *>(workspace);
     if (!(flags & SDDMM_FLAG_ASYNC) && capturing(h->stream)) return bad(h, "a captured call must be asynchronous");
     if (p.n_seqs == 0 || (p.max_q == 0 && p.max_k == 0)) return SDDMM_OK;
+    bool taken = false;
+    const cudaError_t e = launch_attention_backward_tc(p, &taken, h->stream);
+    if (taken) return finish(a, e, "attention_backward_tc", 2, flags);
     return finish(a, launch_attention_backward_general(p, h->stream), "attention_backward_general", 2, flags);
 }
 

@@ -102,6 +102,7 @@ __device__ __forceinline__ bool find_block(const AttentionParams &p, int index, 
 }
 // On the tensor cores; *taken false, and nothing launched, where the call's type, strides or alignment do not allow it.
 cudaError_t launch_attention_forward_tc(const AttentionParams &p, bool *taken, cudaStream_t s);
+cudaError_t launch_attention_backward_tc(const AttentionParams &p, bool *taken, cudaStream_t s);
 cudaError_t launch_attention_forward_general(const AttentionParams &p, cudaStream_t s);
 cudaError_t launch_attention_backward_general(const AttentionParams &p, cudaStream_t s);
 

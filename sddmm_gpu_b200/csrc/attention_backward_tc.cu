@@ -1,0 +1,472 @@
+// Attention, backward, on the tensor cores (tcgen05), for fp16 and bfloat16: two kernels of one shape, without atomics.
+//
+//   dQ      a block has 128 queries of a head, Q and dO in shared memory, and goes over the keys in tiles of 128:
+//             S = Q K^T, dP = dO V^T, dS = P (dP - delta), dQ += dS K
+//   dK, dV  a block has 128 keys of a KV head, K and V in shared memory, and goes over the queries of all heads of the group:
+//             S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
+//
+// with P = exp(S - lse) and delta_i = dO_i.O_i, which the first kernel leaves for the second.  Scores are computed in both (7 products
+// where one kernel would do with 5): a single kernel would have to add up dQ over blocks, by atomics in no fixed order, in a
+// fp32 array of its own.  P and dS are rounded to the operands' type, as every operand of the tensor cores is; fp16 thus
+// limits |P (dP - delta)| to 65,504.
+//
+//   warps 0-7  a row of the block in every thread, a half of the tile's columns in each group of four warps: scores from tensor
+//              memory, weights and score gradients back to it;
+//   warp 8     one thread issues the products; the second operand of the last ones is the streamed tile as it lies, MN-major;
+//   warp 9     one thread brings the tiles by tile copies.
+//
+// dQ: score gradients have a place of their own in tensor memory (two, in turn), so the next tile's scores are computed as soon as the
+// last ones have been read.  dK, dV: tensor memory is full (S, dP, dV, dK); P and dS take the place of S and dP, and the
+// products take turns: dV, S of the next tile, dK, dP of the next tile.
+#include <type_traits>
+
+#include "attention_strict.cuh"
+#include "tc_utils.cuh"
+
+namespace sddmm {
+
+namespace {
+
+using tc::mbar_arrive;
+using tc::mbar_fence_init;
+using tc::mbar_init;
+
+constexpr int T = 128;
+constexpr int ROW_WARPS = 8, MMA_WARP = 8, LOAD_WARP = 9, THREADS = 384;
+constexpr uint32_t TMEM_COLUMNS = 512, S_AT = 0, DP_AT = 128;
+// dQ: accumulator, then two places of 64 columns for score gradients.  dK, dV: the two accumulators.
+constexpr uint32_t DQ_AT = 256, DS_AT = 384, DV_AT = 256, DK_AT = 384;
+#define ROW_REGISTERS "216"
+#define OTHER_REGISTERS "72"
+
+struct alignas(64) Maps {
+    CUtensorMap q, k, v, d_o;
+};
+
+template <int DP, bool KV> struct Shape {
+    static constexpr int BOXES = DP / 64, TILE_BYTES = T * DP * 2, BOX_BYTES = T * 128;
+    static constexpr int SLOTS = DP == 64 ? 8 : KV ? 4 : 5;                        // of one streamed tile
+    static constexpr int STATS = KV ? ROW_WARPS * 2 * 64 * 4 : 0;                  // lse and delta of a warp's 64 columns
+    static constexpr int SMEM = (2 + SLOTS) * TILE_BYTES + STATS;
+};
+
+template <class E, int DP, bool CAP, bool BIAS, bool KV>
+__global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const AttentionParams p, const __grid_constant__ Maps maps)
+{
+    using Sh = Shape<DP, KV>;
+    constexpr int BOXES = Sh::BOXES, TILE_BYTES = Sh::TILE_BYTES, BOX_BYTES = Sh::BOX_BYTES, SLOTS = Sh::SLOTS;
+    constexpr bool BF16 = !std::is_same<E, __half>::value;
+    extern __shared__ __align__(1024) unsigned char smem[];  // the block's two tiles, the ring, lse and delta
+    // dQ: s_full = scores and dP there, p_ready = they have been read
+    __shared__ uint64_t own_full, full[SLOTS], empty[SLOTS], s_full, dp_full, p_ready, ds_ready, acc_full, tail;
+    __shared__ uint32_t tmem_holder, bad[4];
+    __shared__ float row_lse[T], row_delta[2][T];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int heads = KV ? p.kv_heads : p.q_heads, head = blockIdx.x % heads, kv = KV ? head : head / p.group;
+    Sequence s;
+    int seq, block;
+    // causal sequences: the last queries see the most keys, the first keys are seen by the most queries
+    if (!find_block<T>(p, KV ? blockIdx.x / heads : (gridDim.x - 1 - blockIdx.x) / heads, KV, s, seq, block)) return;
+    const int r0 = block * T, n_rows = min(T, (KV ? s.nk : s.nq) - r0);
+    // the tiles of the other side
+    Reach reach = {};
+    KeyTiles keys = {};
+    int from = 0, per_head = 0, count;
+    if (KV) {
+        int to;
+        queries_of(p.window, s, r0, r0 + n_rows, from, to);
+        from /= T;
+        per_head = to > from * T ? (to + T - 1) / T - from : 0;
+        count = per_head * p.group;
+    } else {
+        reach = reach_of(p.window, s, r0, r0 + n_rows);
+        keys = key_tiles<T>(reach);
+        count = keys.n;
+    }
+    auto tile_at = [&](int j) { return (KV ? from + j % per_head : keys.tile(j)) * T; };
+    auto head_at = [&](int j) { return KV ? kv * p.group + j / per_head : head; };
+
+    if (threadIdx.x == 0) {
+        mbar_init(&own_full, 1);
+        mbar_init(&tail, 1);
+        for (int i = 0; i < SLOTS; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+        mbar_init(&s_full, 1);
+        mbar_init(&dp_full, 1);
+        mbar_init(&p_ready, ROW_WARPS);
+        mbar_init(&ds_ready, ROW_WARPS);
+        mbar_init(&acc_full, 1);
+        mbar_fence_init();
+    }
+    if (threadIdx.x < 4) bad[threadIdx.x] = 0;
+    if (warp == MMA_WARP) tc::tmem_alloc(&tmem_holder, TMEM_COLUMNS);
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;  // of warps 0-7
+    if (!KV && warp < ROW_WARPS) {
+        // half of a row's delta in each thread
+        float d = 0.f;
+        if (row < n_rows) {
+            const int64_t at = (int64_t)s.q0 + r0 + row;
+            const E *o = static_cast<const E *>(p.o.data) + at * p.o.row + head * p.o.head;
+            const E *d_o = static_cast<const E *>(p.d_o.data) + at * p.d_o.row + head * p.d_o.head;
+            for (int c = half * (DP / 2); c < min(p.head_dim, (half + 1) * (DP / 2)); c += 8) {
+                uint4 x = *reinterpret_cast<const uint4 *>(o + c), y = *reinterpret_cast<const uint4 *>(d_o + c);
+                const E *xe = reinterpret_cast<const E *>(&x), *ye = reinterpret_cast<const E *>(&y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d = fmaf(to_f(xe[e]), to_f(ye[e]), d);
+            }
+            if (half == 0) row_lse[row] = __ldg(p.lse + (int64_t)head * p.q_rows + at);
+        }
+        row_delta[half][row] = d;
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = tmem_holder, base = tc::smem_u32(smem), ring = base + 2 * TILE_BYTES;
+    bool ok = true;
+
+    if (warp >= ROW_WARPS) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 " OTHER_REGISTERS ";");
+        if (warp == LOAD_WARP && count > 0) {
+            const CUtensorMap *own0 = KV ? &maps.k : &maps.q, *own1 = KV ? &maps.v : &maps.d_o;
+            const CUtensorMap *other0 = KV ? &maps.q : &maps.k, *other1 = KV ? &maps.d_o : &maps.v;
+            const int own_row = (KV ? s.k0 : s.q0) + r0, other_row = KV ? s.q0 : s.k0, there = KV ? s.nq : s.nk;
+            if (lane == 0) {
+                tc::expect_bytes(&own_full, 2 * TILE_BYTES);
+                for (int b = 0; b < BOXES; ++b) tc::load_box(base + b * BOX_BYTES, own0, 64 * b, head, own_row, &own_full);
+                for (int b = 0; b < BOXES; ++b) tc::load_box(base + TILE_BYTES + b * BOX_BYTES, own1, 64 * b, head, own_row, &own_full);
+            }
+            int issued = 0;
+            unsigned tails = 0;
+            for (int n = 0; n < 2 * count && ok; ++n) {
+                const int slot = n % SLOTS, t0 = tile_at(n / 2), of = KV ? head_at(n / 2) : kv;
+                if (n >= SLOTS) ok = tc::warp_wait(&empty[slot], (n / SLOTS - 1) & 1);
+                if (!ok) break;
+                // rows behind the sequence's end, where they meet zero weights in a product: zeros (0 x NaN is NaN)
+                const bool second = n & 1, cut = (KV || !second) && t0 + T > there;
+                const uint32_t at = ring + slot * TILE_BYTES;
+                uint64_t *bar = cut ? &tail : &full[slot];
+                if (lane == 0) {
+                    tc::expect_bytes(bar, TILE_BYTES);
+                    for (int b = 0; b < BOXES; ++b) tc::load_box(at + b * BOX_BYTES, second ? other1 : other0, 64 * b, of, other_row + t0, bar);
+                }
+                ++issued;
+                if (cut) {
+                    ok = tc::warp_wait(&tail, tails++ & 1);
+                    if (!ok) break;
+                    const int first = there - t0;
+                    for (int i = lane; i < (T - first) * BOXES * 8; i += 32) {
+                        const int b = i / ((T - first) * 8), r = first + i / 8 % (T - first);
+                        *reinterpret_cast<uint4 *>(smem + (2 + slot) * TILE_BYTES + b * BOX_BYTES + r * 128 + i % 8 * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    tc::fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full[slot]);
+                }
+            }
+            // copies of a role that gave up still land in this block's shared memory: wait for them
+            if (!ok)
+                for (int n = issued > SLOTS ? issued - SLOTS : 0; n < issued; ++n) (void)tc::wait(&full[n % SLOTS], (n / SLOTS) & 1);
+        } else if (warp == MMA_WARP) {
+            constexpr uint32_t ID_S = tc::instr_desc(BF16, T, T, false, false), ID_ACC = tc::instr_desc(BF16, T, DP, false, true);
+            // own tile x (0 or 1) times the streamed tile of a slot, rows by rows
+            auto rows_by_rows = [&](uint32_t to, int x, int slot) {
+                if (lane == 0) {
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        const uint32_t o = k / 4 * BOX_BYTES + k % 4 * 32;
+                        tc::mma_ss(tmem + to, tc::smem_desc(base + x * TILE_BYTES + o, 16), tc::smem_desc(ring + slot * TILE_BYTES + o, 16), ID_S, k > 0);
+                    }
+                }
+                __syncwarp();
+            };
+            // accumulator += weights (two runs of 32 columns, `apart` columns from one to the next) times the streamed tile
+            auto weights_by_tile = [&](uint32_t to, uint32_t weights, uint32_t apart, int slot, bool add) {
+                if (lane == 0) {
+#pragma unroll
+                    for (int k = 0; k < T / 16; ++k)
+                        tc::mma_ts(tmem + to, tmem + weights + k / 4 * apart + k % 4 * 8, tc::smem_desc(ring + slot * TILE_BYTES + k * 2048, BOX_BYTES), ID_ACC,
+                                   add || k > 0);
+                }
+                __syncwarp();
+            };
+            auto done = [&](uint64_t *bar) {
+                if (lane == 0) tc::commit(bar);
+            };
+            auto slot_of = [](int n) { return n % SLOTS; };
+            auto wait_tile = [&](int n) {
+                ok = ok && tc::warp_wait(&full[n % SLOTS], (n / SLOTS) & 1);
+                tc::fence_after();
+                return ok;
+            };
+            if (count > 0) {
+                ok = tc::warp_wait(&own_full, 0);
+                if (ok && wait_tile(0)) {
+                    rows_by_rows(S_AT, 0, 0);
+                    if (KV) done(&s_full);
+                    if (wait_tile(1)) {
+                        rows_by_rows(DP_AT, 1, slot_of(1));
+                        done(KV ? &dp_full : &s_full);
+                        if (!KV) done(&empty[slot_of(1)]);
+                    }
+                }
+            }
+            for (int j = 0; j < count && ok; ++j) {
+                const int n = 2 * j;
+                const bool more = j + 1 < count;
+                if (KV) {
+                    ok = tc::warp_wait(&p_ready, j & 1);
+                    if (!ok) break;
+                    tc::fence_after();
+                    weights_by_tile(DV_AT, S_AT, 64, slot_of(n + 1), j > 0);
+                    done(&empty[slot_of(n + 1)]);
+                    if (more) {
+                        if (!wait_tile(n + 2)) break;
+                        rows_by_rows(S_AT, 0, slot_of(n + 2));
+                        done(&s_full);
+                    }
+                    ok = tc::warp_wait(&ds_ready, j & 1);
+                    if (!ok) break;
+                    tc::fence_after();
+                    weights_by_tile(DK_AT, DP_AT, 64, slot_of(n), j > 0);
+                    done(&empty[slot_of(n)]);
+                    if (more) {
+                        if (!wait_tile(n + 3)) break;
+                        rows_by_rows(DP_AT, 1, slot_of(n + 3));
+                        done(&dp_full);
+                    }
+                } else {
+                    if (more) {
+                        if (!wait_tile(n + 2) || !wait_tile(n + 3)) break;
+                        ok = tc::warp_wait(&p_ready, j & 1);
+                        if (!ok) break;
+                        tc::fence_after();
+                        rows_by_rows(S_AT, 0, slot_of(n + 2));
+                        rows_by_rows(DP_AT, 1, slot_of(n + 3));
+                        done(&s_full);
+                        done(&empty[slot_of(n + 3)]);
+                    }
+                    ok = tc::warp_wait(&ds_ready, j & 1);
+                    if (!ok) break;
+                    tc::fence_after();
+                    weights_by_tile(DQ_AT, DS_AT + 64 * (j & 1), 32, slot_of(n), j > 0);
+                    done(&empty[slot_of(n)]);
+                }
+            }
+            // nothing of this block is in flight when it ends, also where a role has given up
+            done(&acc_full);
+            __syncwarp();
+            ok = tc::warp_wait(&acc_full, 0) && ok;
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 " ROW_REGISTERS ";");
+        const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const float c = CAP ? 2.f * LOG2E * p.scale / p.cap : p.scale * LOG2E, top_of = p.cap * LOG2E;
+        float slope = BIAS && !KV ? __ldg(p.slopes + head) * LOG2E : 0.f;
+        const int off = s.nk - s.nq;
+        // what a row sees: columns [lo, hi] of the other side, and the first `pre`
+        int lo, hi, pre;
+        float lse2 = 0.f, delta = 0.f;
+        if (KV) {
+            const int j = r0 + row;
+            pre = j < s.prefix ? s.nq : 0;
+            lo = p.window.right < 0 ? 0 : max(0, j - p.window.right - off);
+            hi = p.window.left < 0 ? s.nq - 1 : min(s.nq - 1, j + p.window.left - off);
+            if (row >= n_rows) pre = 0, lo = 0, hi = -1;
+        } else {
+            const int pos = off + r0 + row;
+            pre = s.prefix;
+            lo = p.window.left < 0 ? 0 : max(0, pos - p.window.left);
+            hi = p.window.right < 0 ? s.nk - 1 : min(s.nk - 1, pos + p.window.right);
+            const float lse = row < n_rows ? row_lse[row] : -INFINITY;
+            delta = row_delta[0][row] + row_delta[1][row];
+            lse2 = lse == -INFINITY ? INFINITY : lse * LOG2E;  // a row that has seen nothing: weights of zero
+            if (half == 0 && row < n_rows) p.delta[(int64_t)head * p.q_rows + s.q0 + r0 + row] = delta;
+        }
+        float *const my_lse = reinterpret_cast<float *>(smem + (2 + SLOTS) * TILE_BYTES) + warp * 128, *const my_delta = my_lse + 64;
+        float ahead[4] = {};
+        auto fetch = [&](int j) {  // lse and delta of this warp's 64 columns of tile j
+            const int i = tile_at(j) + 64 * half + lane;
+            const int64_t at = (int64_t)head_at(j) * p.q_rows + s.q0 + i;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const bool in = i + 32 * x < s.nq;
+                const float l = in ? __ldg(p.lse + at + 32 * x) : -INFINITY;
+                ahead[x] = l == -INFINITY ? INFINITY : l * LOG2E;
+                ahead[2 + x] = in ? __ldg(p.delta + at + 32 * x) : 0.f;
+            }
+        };
+        if (KV && count > 0) fetch(0);
+        for (int j = 0; j < count && ok; ++j) {
+            const int t0 = tile_at(j), c0 = t0 + 64 * half;
+            if (KV) {
+                __syncwarp();
+                my_lse[lane] = ahead[0], my_lse[lane + 32] = ahead[1], my_delta[lane] = ahead[2], my_delta[lane + 32] = ahead[3];
+                __syncwarp();
+                if (BIAS) slope = __ldg(p.slopes + head_at(j)) * LOG2E;
+                if (j + 1 < count) fetch(j + 1);
+            }
+            bool open;
+            if (KV) open = n_rows == T && t0 + T <= s.nq && tile_is_open<T>(p.window, s, reach_of(p.window, s, t0, t0 + T), r0);
+            else open = tile_is_open<T>(p.window, s, reach, t0);
+            ok = tc::warp_wait(&s_full, j & 1);
+            if (!ok) break;
+            tc::fence_after();
+            float x[64], y[64];
+            tc::tmem_ld32(reinterpret_cast<uint32_t *>(x), mine + S_AT + 64 * half);
+            tc::tmem_ld32(reinterpret_cast<uint32_t *>(x) + 32, mine + S_AT + 64 * half + 32);
+            if (!KV) {
+                tc::tmem_ld32(reinterpret_cast<uint32_t *>(y), mine + DP_AT + 64 * half);
+                tc::tmem_ld32(reinterpret_cast<uint32_t *>(y) + 32, mine + DP_AT + 64 * half + 32);
+            }
+            tc::wait_ld();
+            if (!KV) {
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_ready);  // the next tile's scores may come
+            }
+            // weights; with a cap, x leaves as weight times (1 - tanh^2), and w holds the weights
+            const int a = lo - c0, n = hi - lo, pr = pre - c0;
+            const float away = KV ? (float)(off + c0 - (r0 + row)) : (float)(c0 - (off + r0 + row));
+            uint32_t w[32];
+#pragma unroll
+            for (int u = 0; u < 64; u += 2) {
+                float l2[2] = {lse2, lse2}, e[2];
+                if (KV) {
+                    const float2 l = *reinterpret_cast<const float2 *>(my_lse + u);
+                    l2[0] = l.x, l2[1] = l.y;
+                }
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    float z = x[u + v], slope_of_cap = 1.f;
+                    if (CAP) {
+                        const float g = tc::rcp(1.f + tc::ex2(z * c));  // tanh = 1 - 2 g
+                        z = fmaf(-2.f * top_of, g, top_of);
+                        slope_of_cap = 4.f * g * (1.f - g);
+                    }
+                    if (BIAS) z = fmaf(-slope, fabsf(away + (float)(u + v)), CAP ? z : z * c);
+                    e[v] = tc::ex2(CAP || BIAS ? z - l2[v] : fmaf(z, c, -l2[v]));
+                    x[u + v] = CAP ? e[v] * slope_of_cap : e[v];
+                    if (!open && !(u + v < pr || (n >= 0 && (unsigned)(u + v - a) <= (unsigned)n))) e[v] = x[u + v] = 0.f;
+                }
+                if (KV) w[u / 2] = tc::pack<E>(e[0], e[1]);
+            }
+            if (KV) {
+                tc::tmem_st32(mine + S_AT + 64 * half, w);
+                tc::wait_st();
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_ready);
+                ok = tc::warp_wait(&dp_full, j & 1);
+                if (!ok) break;
+                tc::fence_after();
+                tc::tmem_ld32(reinterpret_cast<uint32_t *>(y), mine + DP_AT + 64 * half);
+                tc::tmem_ld32(reinterpret_cast<uint32_t *>(y) + 32, mine + DP_AT + 64 * half + 32);
+                tc::wait_ld();
+            }
+#pragma unroll
+            for (int u = 0; u < 64; u += 2) {
+                float2 d = make_float2(delta, delta);
+                if (KV) d = *reinterpret_cast<const float2 *>(my_delta + u);
+                float g0 = x[u] * (y[u] - d.x), g1 = x[u + 1] * (y[u + 1] - d.y);
+                if (!open) {  // hidden: zero whatever dP holds
+                    if (x[u] == 0.f) g0 = 0.f;
+                    if (x[u + 1] == 0.f) g1 = 0.f;
+                }
+                w[u / 2] = tc::pack<E>(g0, g1);
+            }
+            tc::tmem_st32(mine + (KV ? DP_AT + 64 * half : DS_AT + 64 * (j & 1) + 32 * half), w);
+            tc::wait_st();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ds_ready);
+        }
+        if (ok) ok = tc::warp_wait(&acc_full, 0);
+        if (ok) {
+            tc::fence_after();
+            // dQ: half of the columns in each group of warps; dK, dV: an array in each
+            constexpr int COLUMNS = KV ? DP : DP / 2;
+            const HeadArray &to = KV ? (half ? p.dk : p.dv) : p.dq;
+            const uint32_t from_column = KV ? (half ? DK_AT : DV_AT) : DQ_AT + half * COLUMNS;
+            const int first = KV ? 0 : half * COLUMNS;
+            const float by = KV && !half ? 1.f : p.scale;
+            E *dst = static_cast<E *>(to.data) + ((int64_t)(KV ? s.k0 : s.q0) + r0 + row) * to.row + head * to.head;
+            bool wrong = false;
+#pragma unroll
+            for (int b = 0; b < COLUMNS / 32; ++b) {
+                float o[32];
+                if (count > 0) {
+                    tc::tmem_ld32(reinterpret_cast<uint32_t *>(o), mine + from_column + 32 * b);
+                    tc::wait_ld();
+                }
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    o[i] = count > 0 ? o[i] * by : 0.f;
+                    wrong = wrong || (!isfinite(o[i]) && first + 32 * b + i < p.head_dim);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = tc::pack<E>(o[2 * i], o[2 * i + 1]);
+                if (row < n_rows) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (first + 32 * b + 8 * i < p.head_dim)
+                            *reinterpret_cast<uint4 *>(dst + first + 32 * b + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                }
+            }
+            const unsigned rows = __ballot_sync(0xffffffffu, wrong && row < n_rows);
+            if (lane == 0 && rows) atomicOr(&bad[warp & 3], rows);
+        }
+    }
+    if (!ok && lane == 0) dev::report_timeout(p.status);
+    tc::fence_before();
+    __syncthreads();
+    if (warp == MMA_WARP) tc::tmem_dealloc(tmem, TMEM_COLUMNS);
+    if (warp < ROW_WARPS)
+        for (int q = 0; q < 4; ++q)
+            for (unsigned left = bad[q], turn = 0; left; left &= left - 1, ++turn)
+                if (turn % ROW_WARPS == (unsigned)warp) {
+                    const int r = 32 * q + __ffs(left) - 1;
+                    if (KV) strict::dkv_row<E>(p, s, kv, r0 + r);
+                    else strict::dq_row<E>(p, s, head, r0 + r, row_lse[r], row_delta[0][r] + row_delta[1][r]);
+                }
+}
+
+template <class E, int DP, bool CAP, bool BIAS>
+cudaError_t launch(const AttentionParams &p, const Maps &maps, cudaStream_t s)
+{
+    static SmemOptinCache optin_q, optin_kv;
+    constexpr size_t smem_q = Shape<DP, false>::SMEM, smem_kv = Shape<DP, true>::SMEM;
+    cudaError_t e = optin_dynamic_smem(attention_backward_tc_kernel<E, DP, CAP, BIAS, false>, smem_q, optin_q);
+    if (e == cudaSuccess) e = optin_dynamic_smem(attention_backward_tc_kernel<E, DP, CAP, BIAS, true>, smem_kv, optin_kv);
+    if (e != cudaSuccess) return e;
+    const unsigned grid_q = (unsigned)(p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, T));
+    const unsigned grid_kv = (unsigned)(p.kv_heads * most_blocks(p.k_rows, p.n_seqs, p.max_k, T));
+    if (grid_q) attention_backward_tc_kernel<E, DP, CAP, BIAS, false><<<grid_q, THREADS, smem_q, s>>>(p, maps);
+    if (grid_kv) attention_backward_tc_kernel<E, DP, CAP, BIAS, true><<<grid_kv, THREADS, smem_kv, s>>>(p, maps);
+    return cudaGetLastError();
+}
+template <class E, int DP>
+cudaError_t by_score(const AttentionParams &p, const Maps &maps, cudaStream_t s)
+{
+    if (p.cap > 0.f) return p.slopes ? launch<E, DP, true, true>(p, maps, s) : launch<E, DP, true, false>(p, maps, s);
+    return p.slopes ? launch<E, DP, false, true>(p, maps, s) : launch<E, DP, false, false>(p, maps, s);
+}
+
+// 16-byte accesses to the rows of an array
+bool wide(const HeadArray &a) { return (uintptr_t)a.data % 16 == 0 && a.row % 8 == 0 && a.head % 8 == 0; }
+
+}  // namespace
+
+cudaError_t launch_attention_backward_tc(const AttentionParams &p, bool *taken, cudaStream_t s)
+{
+    Maps maps;
+    *taken = p.dtype != 0 && wide(p.o) && wide(p.d_o) && wide(p.dq) && wide(p.dk) && wide(p.dv) &&
+             make_tensor_map(&maps.q, p.q, p.dtype, p.head_dim, p.q_heads, p.q_rows, T) &&
+             make_tensor_map(&maps.k, p.k, p.dtype, p.head_dim, p.kv_heads, p.k_rows, T) &&
+             make_tensor_map(&maps.v, p.v, p.dtype, p.head_dim, p.kv_heads, p.k_rows, T) &&
+             make_tensor_map(&maps.d_o, p.d_o, p.dtype, p.head_dim, p.q_heads, p.q_rows, T);
+    if (!*taken) return cudaSuccess;
+    if (p.dtype == 1) return p.head_dim <= 64 ? by_score<__half, 64>(p, maps, s) : by_score<__half, 128>(p, maps, s);
+    return p.head_dim <= 64 ? by_score<__nv_bfloat16, 64>(p, maps, s) : by_score<__nv_bfloat16, 128>(p, maps, s);
+}
+
+}  // namespace sddmm

@@ -96,10 +96,11 @@ class Problem:
                 p = torch.where(seen, torch.exp(x - torch.where(l == -math.inf, 0.0, l)[:, None]), 0.0)
                 v = V[keys, h // (self.hq // self.hkv)].double()
                 o = p @ v
+                tiny = 2.0 ** -25 if self.dtype == torch.float16 else 0.0  # half a step of a subnormal weight
                 # a weight: its score's error, exp (2^-22, and its argument of up to 2^5 rounded: 2^-19), its rounding; sums of n terms
                 rel = 2 * wobble + 2.0 ** -19 + (n + 16) * 2.0 ** -24 + (u if u > 2.0 ** -24 else 0.0)
                 O[rows, h], lse[h, rows] = o, l
-                tol_o[rows, h] = rel[:, None] * (p @ v.abs()) * 2 + u * o.abs() + 1e-30 + (2.0 ** -24 if self.dtype == torch.float16 else 0.0)
+                tol_o[rows, h] = rel[:, None] * (p @ v.abs()) * 2 + tiny * (seen.double() @ v.abs()) + u * o.abs() + 1e-30 + (2.0 ** -24 if self.dtype == torch.float16 else 0.0)
                 tol_l[h, rows] = wobble + 2.0 ** -20 + (n + 16) * 2.0 ** -24 + 2.0 ** -22 * torch.where(l == -math.inf, 0.0, l).abs()
         return O, lse, tol_o, tol_l
 
@@ -127,13 +128,15 @@ class Problem:
                 e_p = (3 * wobble + 2.0 ** -19 + (nk + 16) * 2.0 ** -24)[:, None]
                 most = p * (dp - delta).abs() * self.scale
                 e_ds = most * slope * e_p + p * self.scale * ((self.d + 8) * 2.0 ** -24 * (size + dsize) + (2 * w + u) * dsize)
-                e_ds = e_ds + most * (2.0 ** -20 + (4 * wobble[:, None] / self.cap if self.cap else 0.0)) + w * ds.abs()
+                # weights and score gradients below 2^-14 are subnormal in fp16: half a step is 2^-25
+                tiny = 2.0 ** -25 if self.dtype == torch.float16 else 0.0
+                e_ds = e_ds + seen * tiny * self.scale + most * (2.0 ** -20 + (4 * wobble[:, None] / self.cap if self.cap else 0.0)) + w * ds.abs()
                 dQ[rows, h] = ds @ k
                 tQ[rows, h] = e_ds @ k.abs() + (nk + 16) * 2.0 ** -24 * (ds.abs() @ k.abs())
                 dK[keys, g] += ds.T @ q
                 tK[keys, g] += e_ds.T @ q.abs() + (nq * self.hq + 16) * 2.0 ** -24 * (ds.abs().T @ q.abs())
                 dV[keys, g] += p.T @ do
-                tV[keys, g] += (p * (e_p + w)).T @ do.abs() + (nq * self.hq + 16) * 2.0 ** -24 * (p.T @ do.abs())
+                tV[keys, g] += (p * (e_p + w) + seen * tiny).T @ do.abs() + (nq * self.hq + 16) * 2.0 ** -24 * (p.T @ do.abs())
         floor = 1e-30 + (2.0 ** -24 if self.dtype == torch.float16 else 0.0)
         return (dQ, dK, dV), tuple(t + u * x.abs() + floor for t, x in ((tQ, dQ), (tK, dK), (tV, dV)))
 
