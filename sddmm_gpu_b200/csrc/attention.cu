@@ -14,6 +14,7 @@
 struct sddmm_attention_s {
     sddmm_handle_s *h = nullptr;
     AttentionParams p{};
+    FewPlan few{};
     const char *last_kernel = "none";
 };
 
@@ -128,6 +129,7 @@ int sddmm_attention_plan(sddmm_handle_t h, const sddmm_attention_desc *d, sddmm_
     if (!a) return SDDMM_OUT_OF_MEMORY;
     a->h = h;
     a->p = p;
+    a->few = plan_attention_few(p, h->sm_count);
     *out = a;
     return SDDMM_OK;
 }
@@ -141,7 +143,7 @@ int sddmm_attention_destroy(sddmm_attention_t a)
 int sddmm_attention_workspace(sddmm_attention_t a, int backward, int64_t *bytes)
 {
     if (!a || !bytes) return SDDMM_INVALID_ARG;
-    *bytes = backward ? (int64_t)sizeof(float) * a->p.q_heads * a->p.q_rows : 0;
+    *bytes = backward ? (int64_t)sizeof(float) * a->p.q_heads * a->p.q_rows : a->few.bytes;
     return SDDMM_OK;
 }
 
@@ -167,7 +169,9 @@ int sddmm_attention_forward(sddmm_attention_t a, const sddmm_head_array *Q, cons
     if (!(flags & SDDMM_FLAG_ASYNC) && capturing(h->stream)) return bad(h, "a captured call must be asynchronous");
     if (p.n_seqs == 0 || p.max_q == 0) return SDDMM_OK;
     bool taken = false;
-    const cudaError_t e = launch_attention_forward_tc(p, &taken, h->stream);
+    cudaError_t e = launch_attention_few_tc(p, a->few, workspace, &taken, h->stream);
+    if (taken) return finish(a, e, "attention_few_tc", a->few.n_splits > 1 ? 2 : 1, flags);
+    e = launch_attention_forward_tc(p, &taken, h->stream);
     if (taken) return finish(a, e, "attention_tc", 1, flags);
     return finish(a, launch_attention_forward_general(p, h->stream), "attention_general", 1, flags);
 }

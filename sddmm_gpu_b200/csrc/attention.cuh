@@ -36,7 +36,7 @@ struct AttentionParams {
     float *lse;    // q_heads x q_rows
     float *delta;  // q_heads x q_rows, workspace of the backward pass
     float *part_o, *part_lse;  // parts of a split long axis (workspace)
-    int n_splits;
+    int n_splits, chunk_tiles;  // chunks of the keys, at most; key tiles of one
     int *status;
 };
 
@@ -100,6 +100,14 @@ __device__ __forceinline__ bool find_block(const AttentionParams &p, int index, 
     }
     return false;
 }
+// Few queries of many keys: how the keys are cut, 0 splits where another kernel is to be taken; workspace bytes.
+constexpr int MOST_FEW_ROWS = 64;
+struct FewPlan {
+    int n_splits, chunk_tiles;
+    int64_t bytes;
+};
+FewPlan plan_attention_few(const AttentionParams &p, int sm_count);
+cudaError_t launch_attention_few_tc(const AttentionParams &p, const FewPlan &f, void *workspace, bool *taken, cudaStream_t s);
 // On the tensor cores; *taken false, and nothing launched, where the call's type, strides or alignment do not allow it.
 cudaError_t launch_attention_forward_tc(const AttentionParams &p, bool *taken, cudaStream_t s);
 cudaError_t launch_attention_backward_tc(const AttentionParams &p, bool *taken, cudaStream_t s);
