@@ -8,6 +8,7 @@ built library (or without a GPU, for the compute calls) everything here raises.
 """
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -76,17 +77,9 @@ class AttentionDesc(C.Structure):
         ("window_right", C.c_int32)] + [(n, C.c_void_p) for n in ("q_offsets", "k_offsets", "k_len", "prefix", "slopes")]
 
 
-class RotaryDesc(C.Structure):
-    _fields_ = [("dtype", C.c_int32), ("head_dim", C.c_int32), ("rot_dim", C.c_int32), ("layout", C.c_int32), ("n_rows", C.c_int64),
-                ("positions", C.c_void_p), ("position0", C.c_int64), ("frequencies", C.c_void_p), ("magnitude", C.c_float),
-                ("inverse", C.c_int32)]
-
-
-class _RotaryPart(C.Structure):
-    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_row_stride", C.c_int64), ("src_head_stride", C.c_int64),
-                ("dst_row_stride", C.c_int64), ("dst_head_stride", C.c_int64), ("heads", C.c_int32), ("rotate", C.c_int32),
-                ("dst_rows", C.c_void_p), ("n_dst_rows", C.c_int64)]
-
+# sddmm_rotary_desc and sddmm_rotary_part, written with one call each (field by field costs microseconds a call)
+_ROTARY_DESC = struct.Struct("@iiiiqPqPfi")
+_ROTARY_PART = struct.Struct("@PPqqqqiiPq")
 
 _lib = None
 
@@ -127,7 +120,7 @@ def lib():
     L.sddmm_attention_backward.argtypes = [vp, heads, heads, heads, heads, vp, heads, heads, heads, heads, vp, i64, u32]
     L.sddmm_attention_last_kernel.restype = C.c_char_p
     L.sddmm_attention_last_kernel.argtypes = [vp]
-    L.sddmm_rotary.argtypes = [vp, C.POINTER(RotaryDesc), C.POINTER(_RotaryPart), C.c_int, u32]
+    L.sddmm_rotary.argtypes = [vp, vp, vp, C.c_int, u32]
     L.sddmm_rotary_frequencies.argtypes = [C.c_int] + [C.c_double] * 5 + [vp]
     L.sddmm_kernel_launches.argtypes = [vp, C.POINTER(i64)]
     L.sddmm_check_result.argtypes = [vp, vp, vp, vp, vp, i64, C.c_double, C.POINTER(C.c_double), C.POINTER(i64),
@@ -251,6 +244,8 @@ class Handle:
         self.device = device
         self._explicit_stream = False
         self._stream = None  # what sddmm_set_stream was last given (None: the handle's own stream)
+        self._rotary_desc = C.create_string_buffer(_ROTARY_DESC.size)   # argument blocks of rotary(): a handle is one thread's at a time
+        self._rotary_parts = C.create_string_buffer(4 * _ROTARY_PART.size)
 
     def _follow_torch_stream(self, *args):
         """Launch on torch's current stream when a CUDA tensor is among the arguments
@@ -365,30 +360,40 @@ class Handle:
 
         positions: int64 CUDA tensor, one for each row, or the int position of the first row; frequencies: float64 numpy
         array, radians a position of every pair; layout: "half" or "interleaved"; inverse: the gradient of the rotation."""
-        import torch
-        if not 1 <= len(parts) <= 4:
+        count = len(parts)
+        if not 1 <= count <= 4:
             raise ValueError("one to four parts")
         x = parts[0].src
-        n, d, dtype = x.shape[0], x.shape[2], x.dtype
-        array = (_RotaryPart * len(parts))()
+        (n, _, d), dtype, device = x.shape, x.dtype, self.device
         for i, p in enumerate(parts):
-            for t in (p.src, p.dst):
-                if t.dim() != 3 or t.shape[2] != d or t.shape[1] != p.src.shape[1] or t.dtype != dtype or t.stride(2) != 1 and d > 1 or \
-                        t.get_device() != self.device:
-                    raise ValueError(f"part {i} must be tensors (rows, heads, {d}) of {dtype} on cuda:{self.device} with contiguous heads")
-            if p.src.shape[0] != n or p.rows is None and p.dst.shape[0] != n:
+            src, dst, rows = p.src, p.dst, p.rows
+            shape, to = src.shape, dst.shape
+            a, b = src.stride(), dst.stride()
+            if len(shape) != 3 or len(to) != 3 or shape[2] != d or shape[1:] != to[1:] or src.dtype != dtype or dst.dtype != dtype or \
+                    d > 1 and (a[2] != 1 or b[2] != 1) or src.get_device() != device or dst.get_device() != device:
+                raise ValueError(f"part {i} must be tensors (rows, heads, {d}) of {dtype} on cuda:{device} with contiguous heads")
+            if shape[0] != n or rows is None and to[0] != n:
                 raise ValueError(f"part {i} has other rows than the first")
-            rows = _cuda_vector(p.rows, "rows", torch.int64, n, self.device)
-            array[i] = _RotaryPart(p.src.data_ptr(), p.dst.data_ptr(), p.src.stride(0), p.src.stride(1), p.dst.stride(0), p.dst.stride(1),
-                                   p.src.shape[1], p.rotate, rows, p.dst.shape[0])
-        f = np.ascontiguousarray(frequencies, np.float64)
-        at = None if isinstance(positions, int) else _cuda_vector(positions, "positions", torch.int64, n, self.device)
-        desc = RotaryDesc(_dtype(dtype), d, 2 * f.shape[0], ("half", "interleaved").index(layout), n, at,
-                          positions if at is None else 0, f.ctypes.data, magnitude, inverse)
+            if rows is not None:
+                rows = self._int64_vector(rows, "rows", n)
+            _ROTARY_PART.pack_into(self._rotary_parts, i * _ROTARY_PART.size, src.data_ptr(), dst.data_ptr(), a[0], a[1], b[0], b[1],
+                                   shape[1], p.rotate, rows or 0, to[0])
+        f = frequencies
+        if type(f) is not np.ndarray or f.dtype != np.float64 or not f.flags.c_contiguous:
+            f = np.ascontiguousarray(f, np.float64)
+        first, at = (positions, 0) if isinstance(positions, int) else (0, self._int64_vector(positions, "positions", n))
+        _ROTARY_DESC.pack_into(self._rotary_desc, 0, _dtype(dtype), d, 2 * f.shape[0], ("half", "interleaved").index(layout), n, at,
+                               first, f.__array_interface__["data"][0], magnitude, inverse)
         self._follow_torch_stream(x)
-        st = _lib.sddmm_rotary(self._h, desc, array, len(parts), flags)
+        st = lib().sddmm_rotary(self._h, self._rotary_desc, self._rotary_parts, count, flags)
         if st:
             self._check(st)
+
+    def _int64_vector(self, a, name, n):
+        import torch
+        if getattr(a, "dtype", None) is not torch.int64 or a.shape != (n,) or not a.is_contiguous() or a.get_device() != self.device:
+            raise ValueError(f"{name} must be a contiguous int64 tensor of {n} values on cuda:{self.device}")
+        return a.data_ptr()
 
     def sddmm_coo(self, M, N, rows, cols, W, H, K, P, Sval=None, nnz=None):
         if nnz is None:

@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             constexpr uint32_t ID_S = tc::instr_desc(BF16, T, T, false, false), ID_ACC = tc::instr_desc(BF16, T, DP, false, true);
             // own tile x (0 or 1) times the streamed tile of a slot, rows by rows
             auto rows_by_rows = [&](uint32_t to, int x, int slot) {
-                if (lane == 0) {
+                if (tc::elected()) {
 #pragma unroll
                     for (int k = 0; k < DP / 16; ++k) {
                         const uint32_t o = k / 4 * BOX_BYTES + k % 4 * 32;
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             };
             // accumulator += weights (two runs of 32 columns, `apart` columns from one to the next) times the streamed tile
             auto weights_by_tile = [&](uint32_t to, uint32_t weights, uint32_t apart, int slot, bool add) {
-                if (lane == 0) {
+                if (tc::elected()) {
 #pragma unroll
                     for (int k = 0; k < T / 16; ++k)
                         tc::mma_ts(tmem + to, tmem + weights + k / 4 * apart + k % 4 * 8, tc::smem_desc(ring + slot * TILE_BYTES + k * 2048, BOX_BYTES), ID_ACC,
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                 __syncwarp();
             };
             auto done = [&](uint64_t *bar) {
-                if (lane == 0) tc::commit(bar);
+                if (tc::elected()) tc::commit(bar);
             };
             auto slot_of = [](int n) { return n % SLOTS; };
             auto wait_tile = [&](int n) {

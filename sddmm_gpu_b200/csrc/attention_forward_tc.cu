@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
             bool begun[2] = {false, false};
             unsigned n_p[2] = {0, 0};
             auto scores = [&](int t, int stage) {  // S of tile t
-                if (lane == 0) {
+                if (tc::elected()) {
     #pragma unroll
                     for (int k = 0; k < DP / 16; ++k) {
                         const uint32_t o = k / 4 * BOX_BYTES + k % 4 * 32;
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                     tc::fence_after();
                     for (int t = 0; t < 2; ++t)
                         if (active(t, all.tile(0))) scores(t, 0);
-                    if (lane == 0) tc::commit(&empty[0]);
+                    if (tc::elected()) tc::commit(&empty[0]);
                 }
             }
             for (int u = 0; u < all.n && ok; ++u) {
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                         ok = tc::warp_wait(&p_ready[t], n_p[t]++ & 1);
                         if (!ok) break;
                         tc::fence_after();
-                        if (lane == 0) {
+                        if (tc::elected()) {
     #pragma unroll
                             for (int k = 0; k < T / 16; ++k)
                                 tc::mma_ts(tmem + O_COLUMN + t * T, tmem + t * T + k * 8, tc::smem_desc(ring + vs * TILE_BYTES + k * 2048, BOX_BYTES), ID_O,
@@ -173,12 +173,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                     }
                 }
                 if (!ok) break;
-                if (lane == 0) {
+                if (tc::elected()) {
                     tc::commit(&empty[vs]);
                     if (more) tc::commit(&empty[ks]);
                 }
             }
-            if (lane == 0) {
+            if (tc::elected()) {
                 tc::commit(&o_full[0]);
                 tc::commit(&o_full[1]);
             }

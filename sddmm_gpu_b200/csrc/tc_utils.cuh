@@ -50,6 +50,14 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
                  "l"(b), "r"(idesc), "r"((uint32_t)add)
                  : "memory");
 }
+// One thread of a converged warp, the same one every time.  The compiler keeps what such a region computes in uniform registers, which is where
+// tcgen05.mma takes its descriptors from; behind a test of the lane number every MMA waits for its operands to be moved there.
+__device__ __forceinline__ bool elected()
+{
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
+}
 // Arrives on the barrier when all MMAs that this thread has issued are complete.
 __device__ __forceinline__ void commit(uint64_t *bar)
 {

@@ -61,5 +61,5 @@ def test_null_handles_are_refused():
     assert L.sddmm_attention_backward(None, none, none, none, none, None, none, none, none, none, None, 0, 0) == api.INVALID_ARG
     assert L.sddmm_attention_destroy(None) == api.OK
     assert L.sddmm_attention_last_kernel(None) == b"none"
-    assert L.sddmm_rotary(None, C.POINTER(api.RotaryDesc)(), None, 1, 0) == api.INVALID_ARG
+    assert L.sddmm_rotary(None, None, None, 1, 0) == api.INVALID_ARG
     assert L.sddmm_rotary_frequencies(8, 1e4, 1.0, 0.0, 1.0, 32.0, None) == api.INVALID_ARG
