@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                 if (lane == 0) mbar_arrive(&p_ready);  // the next tile's scores may come
             }
             // weights; with a cap, x leaves as weight times (1 - tanh^2), and w holds the weights
-            const int a = lo - c0, n = hi - lo, pr = pre - c0;
+            const unsigned seen[2] = {open ? ~0u : seen_bits(lo, hi, pre, c0), open ? ~0u : seen_bits(lo, hi, pre, c0 + 32)};
             const float away = KV ? (float)(off + c0 - (r0 + row)) : (float)(c0 - (off + r0 + row));
             uint32_t w[32];
 #pragma unroll
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                     if (BIAS) z = fmaf(-slope, fabsf(away + (float)(u + v)), CAP ? z : z * c);
                     e[v] = tc::ex2(CAP || BIAS ? z - l2[v] : fmaf(z, c, -l2[v]));
                     x[u + v] = CAP ? e[v] * slope_of_cap : e[v];
-                    if (!open && !(u + v < pr || (n >= 0 && (unsigned)(u + v - a) <= (unsigned)n))) e[v] = x[u + v] = 0.f;
+                    if (!(seen[u / 32] & 1u << (u + v) % 32)) e[v] = x[u + v] = 0.f;
                 }
                 if (KV) w[u / 2] = tc::pack<E>(e[0], e[1]);
             }
@@ -367,10 +367,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                 float2 d = make_float2(delta, delta);
                 if (KV) d = *reinterpret_cast<const float2 *>(my_delta + u);
                 float g0 = x[u] * (y[u] - d.x), g1 = x[u + 1] * (y[u + 1] - d.y);
-                if (!open) {  // hidden: zero whatever dP holds
-                    if (x[u] == 0.f) g0 = 0.f;
-                    if (x[u + 1] == 0.f) g1 = 0.f;
-                }
+                // hidden: zero whatever dP holds
+                g0 = seen[u / 32] & 1u << u % 32 ? g0 : 0.f;
+                g1 = seen[u / 32] & 2u << u % 32 ? g1 : 0.f;
                 w[u / 2] = tc::pack<E>(g0, g1);
             }
             tc::tmem_st32(mine + (KV ? DP_AT + 64 * half : DS_AT + 64 * (j & 1) + 32 * half), w);
@@ -388,8 +387,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             const uint32_t from_column = KV ? (half ? DK_AT : DV_AT) : DQ_AT + half * COLUMNS;
             const int first = KV ? 0 : half * COLUMNS;
             const float by = KV && !half ? 1.f : p.scale;
-            E *dst = static_cast<E *>(to.data) + ((int64_t)(KV ? s.k0 : s.q0) + r0 + row) * to.row + head * to.head;
-            bool wrong = false;
+            float zero = 0.f;  // NaN as soon as a result is not finite
+            // the block's own tiles are done with
+            unsigned char *const stage = smem + (KV ? half * TILE_BYTES + (warp & 3) * 32 * DP * 2 : warp * 32 * DP);
 #pragma unroll
             for (int b = 0; b < COLUMNS / 32; ++b) {
                 float o[32];
@@ -397,22 +397,17 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                     tc::tmem_ld32(reinterpret_cast<uint32_t *>(o), mine + from_column + 32 * b);
                     tc::wait_ld();
                 }
-                uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
                     o[i] = count > 0 ? o[i] * by : 0.f;
-                    wrong = wrong || (!isfinite(o[i]) && first + 32 * b + i < p.head_dim);
+                    zero = fmaf(o[i], 0.f, zero);
                 }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) w[i] = tc::pack<E>(o[2 * i], o[2 * i + 1]);
-                if (row < n_rows) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (first + 32 * b + 8 * i < p.head_dim)
-                            *reinterpret_cast<uint4 *>(dst + first + 32 * b + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-                }
+                tc::stage_32<E, COLUMNS>(stage, 32 * b, o);
             }
-            const unsigned rows = __ballot_sync(0xffffffffu, wrong && row < n_rows);
+            const int row0 = (warp & 3) * 32;
+            tc::store_staged<E, COLUMNS>(stage, static_cast<E *>(to.data) + ((int64_t)(KV ? s.k0 : s.q0) + r0 + row0) * to.row + head * to.head + first, to.row,
+                                         n_rows - row0, p.head_dim - first);
+            const unsigned rows = __ballot_sync(0xffffffffu, zero != 0.f && row < n_rows);
             if (lane == 0 && rows) atomicOr(&bad[warp & 3], rows);
         }
     }

@@ -64,6 +64,15 @@ MASK_FN bool key_seen(Window w, const Sequence &s, int pos, int j)
 {
     return j < s.nk && (j < s.prefix || ((w.left < 0 || j >= pos - w.left) && (w.right < 0 || j <= pos + w.right)));
 }
+// Bits of 32 places from `at` on: those in [lo, hi], and those below pre.
+MASK_FN unsigned seen_bits(int lo, int hi, int pre, int at)
+{
+    const int a = lo - at, b = hi - at, c = pre - at;
+    const unsigned up = a <= 0 ? 0xffffffffu : a > 31 ? 0u : 0xffffffffu << a;
+    const unsigned down = b >= 31 ? 0xffffffffu : b < 0 ? 0u : 0xffffffffu >> (31 - b);
+    const unsigned first = c >= 32 ? 0xffffffffu : c <= 0 ? 0u : 0xffffffffu >> (32 - c);
+    return (up & down) | first;
+}
 // The queries [i0, i1) of a sequence that may see a key of [k0, k1): all where the prefix reaches in.
 MASK_FN void queries_of(Window w, const Sequence &s, int k0, int k1, int &i0, int &i1)
 {

@@ -99,6 +99,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *v)
         TC_R8(TC_IN, v, 24), "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t *v, uint32_t taddr)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : TC_R8(TC_OUT, v, 0), TC_R8(TC_OUT, v, 8)
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v)
 {
     asm volatile(
@@ -149,6 +157,80 @@ __device__ __forceinline__ float rcp(float x)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// ---- two fp32 values in 64 bits: one instruction for both ----
+using F2 = unsigned long long;
+using dev::ffma2;
+__device__ __forceinline__ F2 two(float a, float b)
+{
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split(F2 x, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ F2 add2(F2 a, F2 b)
+{
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b)
+{
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max3_abs(float a, float b, float c)
+{
+    float r;
+    asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of both values without the special function unit, x <= 8: x = n + f, |f| <= 1/2, from adding and taking away 1.5 x 2^23; 2^f as a
+// polynomial (Chebyshev interpolation of degree 5: off by 2.5e-7 of the value); 2^n by its exponent, which is 0 for n = -127: from -126.5 down to -inf the result is 0.  NaN stays NaN.
+__device__ __forceinline__ F2 ex2_poly(F2 x)
+{
+    float a, b;
+    split(x, a, b);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-127.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-127.f));
+    x = two(a, b);
+    const float big = 12582912.f;
+    const F2 r = add2(x, two(big, big)), f = add2(x, mul2(add2(r, two(-big, -big)), two(-1.f, -1.f)));
+    F2 p = two(0.00134004327f, 0.00134004327f);
+    p = ffma2(p, f, two(0.00967603736f, 0.00967603736f));
+    p = ffma2(p, f, two(0.0555032715f, 0.0555032715f));
+    p = ffma2(p, f, two(0.240221068f, 0.240221068f));
+    p = ffma2(p, f, two(0.693147182f, 0.693147182f));
+    p = ffma2(p, f, two(1.0f, 1.0f));
+    split(r, a, b);
+    return mul2(p, two(__uint_as_float((__float_as_uint(a) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(b) << 23) + 0x3f800000u)));
+}
+constexpr float TANH_RANGE = 0.6f;
+// tanh(y) / y from u = y^2, |y| <= 0.6 (Chebyshev interpolation in u; tanh is off by 9e-8), times `by`, whose products with the coefficients are given.
+struct TanhCoefficients {
+    F2 c[5];
+};
+__device__ __forceinline__ TanhCoefficients tanh_coefficients(float by)
+{
+    constexpr float C[5] = {0.99999994f, -0.33332324f, 0.133103579f, -0.0521096252f, 0.0154866902f};
+    TanhCoefficients t;
+#pragma unroll
+    for (int i = 0; i < 5; ++i) t.c[i] = two(C[i] * by, C[i] * by);
+    return t;
+}
+__device__ __forceinline__ F2 tanh_over_y(F2 u, const TanhCoefficients &t)
+{
+    F2 p = t.c[4];
+#pragma unroll
+    for (int i = 3; i >= 0; --i) p = ffma2(p, u, t.c[i]);
+    return p;
+}
 // Two values in a word, the first in its lower half.
 template <class T> __device__ __forceinline__ uint32_t pack(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b)
@@ -162,6 +244,40 @@ template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b)
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
+}
+
+// Results of a warp, a row a thread, to global memory: through a piece of shared memory (32 rows of COLUMNS 16-bit values) that the warp has to
+// itself, so that a store instruction writes whole rows and not 16 bytes of each of 32 rows (which took 16,000 clocks a block).
+template <int COLUMNS>
+__device__ __forceinline__ uint4 *staged(unsigned char *stage, int row, int piece)  // 16-byte piece of a row, spread over the banks
+{
+    return reinterpret_cast<uint4 *>(stage + row * COLUMNS * 2 + (piece ^ (row & (COLUMNS / 8 < 8 ? COLUMNS / 8 - 1 : 7))) * 16);
+}
+template <class E, int COLUMNS>
+__device__ __forceinline__ void stage_32(unsigned char *stage, int column, const float (&v)[32])
+{
+    const int row = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        *staged<COLUMNS>(stage, row, column / 8 + i) = make_uint4(pack<E>(v[8 * i], v[8 * i + 1]), pack<E>(v[8 * i + 2], v[8 * i + 3]),
+                                                                   pack<E>(v[8 * i + 4], v[8 * i + 5]), pack<E>(v[8 * i + 6], v[8 * i + 7]));
+}
+// dst: the warp's first row, at the first of COLUMNS columns; `rows` rows and `columns` columns (a multiple of 8) exist.
+template <class E, int COLUMNS>
+__device__ __forceinline__ void store_staged(const unsigned char *stage, E *dst, int64_t row_stride, int rows, int columns)
+{
+    __syncwarp();
+    constexpr int PIECES = COLUMNS / 8, AT_ONCE = 32 / PIECES;
+    const int lane = threadIdx.x & 31, piece = lane % PIECES;
+    uint4 v[32 / AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < 32 / AT_ONCE; ++i) v[i] = *staged<COLUMNS>(const_cast<unsigned char *>(stage), i * AT_ONCE + lane / PIECES, piece);
+#pragma unroll
+    for (int i = 0; i < 32 / AT_ONCE; ++i) {
+        const int row = i * AT_ONCE + lane / PIECES;
+        if (row < rows && piece * 8 < columns) *reinterpret_cast<uint4 *>(dst + row * row_stride + piece * 8) = v[i];
+    }
+    __syncwarp();
 }
 
 }  // namespace tc

@@ -28,6 +28,13 @@ static long check(Window w, const Sequence &s)
             if (n > 0 && t.tile(n) <= t.tile(n - 1)) ++bad;
         }
         for (int k = 0; k < (int)visits.size(); ++k) {
+            for (int i = i0; i < i1; ++i) {  // as bits: the places that a query sees
+                const int pos = s.nk - s.nq + i;
+                const int lo = w.left < 0 ? 0 : max_of(0, pos - w.left), hi = w.right < 0 ? s.nk - 1 : min_of(s.nk - 1, pos + w.right);
+                const unsigned bits = seen_bits(lo, hi, s.prefix, k * T);
+                for (int j = 0; j < 32; ++j)
+                    if ((bits >> j & 1u) != (unsigned)(k * T + j < s.nk && seen(w, s, i, k * T + j))) ++bad;
+            }
             bool any = false, all = true;
             for (int i = i0; i < i1; ++i)
                 for (int j = k * T; j < k * T + T; ++j) {
