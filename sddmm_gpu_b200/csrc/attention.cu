@@ -15,6 +15,7 @@ struct sddmm_attention_s {
     sddmm_handle_s *h = nullptr;
     AttentionParams p{};
     FewPlan few{};
+    GeneralParts parts{};
     const char *last_kernel = "none";
 };
 
@@ -55,6 +56,9 @@ int check_array(sddmm_handle_s *h, const sddmm_head_array *a, const char *name, 
     }
     return SDDMM_OK;
 }
+
+// delta of the backward pass, first in its workspace
+int64_t delta_bytes(const AttentionParams &p) { return ((int64_t)sizeof(float) * p.q_heads * p.q_rows + 15) / 16 * 16; }
 
 bool capturing(cudaStream_t s)
 {
@@ -130,6 +134,7 @@ int sddmm_attention_plan(sddmm_handle_t h, const sddmm_attention_desc *d, sddmm_
     a->h = h;
     a->p = p;
     a->few = plan_attention_few(p, h->sm_count);
+    a->parts = plan_general_parts(p, h->sm_count);
     *out = a;
     return SDDMM_OK;
 }
@@ -143,7 +148,7 @@ int sddmm_attention_destroy(sddmm_attention_t a)
 int sddmm_attention_workspace(sddmm_attention_t a, int backward, int64_t *bytes)
 {
     if (!a || !bytes) return SDDMM_INVALID_ARG;
-    *bytes = backward ? (int64_t)sizeof(float) * a->p.q_heads * a->p.q_rows : a->few.bytes;
+    *bytes = backward ? delta_bytes(a->p) + a->parts.bytes : a->few.bytes;
     return SDDMM_OK;
 }
 
@@ -202,12 +207,13 @@ int sddmm_attention_backward(sddmm_attention_t a, const sddmm_head_array *Q, con
     if (need > 0 && (workspace_bytes < need || !on_device(workspace, h->device) || (uintptr_t)workspace % 16))
         return bad(h, "workspace: sddmm_attention_workspace() bytes of device memory, 16-byte aligned");
     p.delta = static_cast<float *>(workspace);
+    p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + delta_bytes(p));
     if (!(flags & SDDMM_FLAG_ASYNC) && capturing(h->stream)) return bad(h, "a captured call must be asynchronous");
     if (p.n_seqs == 0 || (p.max_q == 0 && p.max_k == 0)) return SDDMM_OK;
     bool taken = false;
     const cudaError_t e = launch_attention_backward_tc(p, &taken, h->stream);
     if (taken) return finish(a, e, "attention_backward_tc", 2, flags);
-    return finish(a, launch_attention_backward_general(p, h->stream), "attention_backward_general", 2, flags);
+    return finish(a, launch_attention_backward_general(p, a->parts, h->stream), "attention_backward_general", 2 + (a->parts.n_q > 1) + (a->parts.n_kv > 1), flags);
 }
 
 const char *sddmm_attention_last_kernel(sddmm_attention_t a) { return a ? a->last_kernel : "none"; }

@@ -112,6 +112,13 @@ cudaError_t launch_attention_few_tc(const AttentionParams &p, const FewPlan &f, 
 cudaError_t launch_attention_forward_tc(const AttentionParams &p, bool *taken, cudaStream_t s);
 cudaError_t launch_attention_backward_tc(const AttentionParams &p, bool *taken, cudaStream_t s);
 cudaError_t launch_attention_forward_general(const AttentionParams &p, cudaStream_t s);
-cudaError_t launch_attention_backward_general(const AttentionParams &p, cudaStream_t s);
+// How the general backward kernels cut the tiles that a block goes through (1: not), for dQ and for dK and dV; bytes of the parts' sums
+// (16-byte aligned, p.part_o).
+struct GeneralParts {
+    int n_q, tiles_q, n_kv, tiles_kv;
+    int64_t bytes;
+};
+GeneralParts plan_general_parts(const AttentionParams &p, int sm_count);
+cudaError_t launch_attention_backward_general(const AttentionParams &p, const GeneralParts &parts, cudaStream_t s);
 
 }  // namespace sddmm

@@ -9,6 +9,7 @@
 //
 // What bounds it: the FMA pipe and the shared-memory loads that feed it (two 128-bit loads per 16 FMAs).
 #include "attention_strict.cuh"
+#include "device_utils.cuh"
 
 namespace sddmm {
 
@@ -34,38 +35,58 @@ __device__ __forceinline__ void load_rows(float *dst, const HeadArray &a, int64_
     }
 }
 __device__ __forceinline__ float4 at4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
-__device__ __forceinline__ void fma4(float4 &a, float x, float4 v)
+using F2 = unsigned long long;  // two fp32 values: one FMA instruction for both
+using dev::ffma2;
+using dev::fold2;
+__device__ __forceinline__ F2 twice(float x)
 {
-    a.x = fmaf(x, v.x, a.x);
-    a.y = fmaf(x, v.y, a.y);
-    a.z = fmaf(x, v.z, a.z);
-    a.w = fmaf(x, v.w, a.w);
+    F2 r;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(x));
+    return r;
 }
-// acc[r][c] = row ty + 16 r of x times row tx + 16 c of y
+__device__ __forceinline__ ulonglong2 pairs(const float *p) { return *reinterpret_cast<const ulonglong2 *>(p); }
+// acc[r][c] = row ty + 16 r of x times row tx + 16 c of y, D columns
 template <int DP>
-__device__ __forceinline__ void rows_times_rows(float (&acc)[4][4], const float *x, const float *y, int ty, int tx)
+__device__ __forceinline__ void rows_times_rows(float (&acc)[4][4], const float *x, const float *y, int ty, int tx, int D)
 {
+    F2 sum[4][4] = {};
+#pragma unroll 2
+    for (int d = 0; d < D; d += 4) {
+        ulonglong2 a[4], b[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r) a[r] = pairs(x + (ty + 16 * r) * (DP + 4) + d);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[r][c] = 0.f;
-#pragma unroll 4
-    for (int d = 0; d < DP; d += 4) {
-        float4 a[4], b[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) a[r] = at4(x + (ty + 16 * r) * (DP + 4) + d);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) b[c] = at4(y + (tx + 16 * c) * (DP + 4) + d);
+        for (int c = 0; c < 4; ++c) b[c] = pairs(y + (tx + 16 * c) * (DP + 4) + d);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                acc[r][c] = fmaf(a[r].w, b[c].w, fmaf(a[r].z, b[c].z, fmaf(a[r].y, b[c].y, fmaf(a[r].x, b[c].x, acc[r][c]))));
+            for (int c = 0; c < 4; ++c) sum[r][c] = ffma2(a[r].y, b[c].y, ffma2(a[r].x, b[c].x, sum[r][c]));
     }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[r][c] = fold2(sum[r][c]);
+}
+// Four columns of a row.
+struct Quad {
+    F2 a, b;
+};
+__device__ __forceinline__ float4 open(Quad q)
+{
+    float4 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(q.a));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.z), "=f"(v.w) : "l"(q.b));
+    return v;
+}
+__device__ __forceinline__ void add_times(Quad &acc, float w, ulonglong2 v)
+{
+    const F2 ww = twice(w);
+    acc.a = ffma2(ww, v.x, acc.a);
+    acc.b = ffma2(ww, v.y, acc.b);
 }
 // acc[r][c] += sum_j w[row ty + 16 r][j] * x[j][4 tx + 64 c ..]
 template <int DP>
-__device__ __forceinline__ void weights_times_rows(float4 (&acc)[4][DP / 64], const float *w, const float *x, int ty, int tx)
+__device__ __forceinline__ void weights_times_rows(Quad (&acc)[4][DP / 64], const float *w, const float *x, int ty, int tx)
 {
 #pragma unroll 2
     for (int j = 0; j < B; j += 4) {
@@ -76,26 +97,26 @@ __device__ __forceinline__ void weights_times_rows(float4 (&acc)[4][DP / 64], co
         for (int u = 0; u < 4; ++u)
 #pragma unroll
             for (int c = 0; c < DP / 64; ++c) {
-                const float4 v = at4(x + (j + u) * (DP + 4) + 4 * tx + 64 * c);
+                const ulonglong2 v = pairs(x + (j + u) * (DP + 4) + 4 * tx + 64 * c);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) fma4(acc[r][c], u == 0 ? p[r].x : u == 1 ? p[r].y : u == 2 ? p[r].z : p[r].w, v);
+                for (int r = 0; r < 4; ++r) add_times(acc[r][c], u == 0 ? p[r].x : u == 1 ? p[r].y : u == 2 ? p[r].z : p[r].w, v);
             }
     }
 }
 // acc[r][c] += sum_i w[i][4 ty + r] * x[i][4 tx + 64 c ..]
 template <int DP>
-__device__ __forceinline__ void weights_t_times_rows(float4 (&acc)[4][DP / 64], const float *w, const float *x, int ty, int tx)
+__device__ __forceinline__ void weights_t_times_rows(Quad (&acc)[4][DP / 64], const float *w, const float *x, int ty, int tx)
 {
 #pragma unroll 4
     for (int i = 0; i < B; ++i) {
         const float4 p = at4(w + i * PS + 4 * ty);
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
-            const float4 v = at4(x + i * (DP + 4) + 4 * tx + 64 * c);
-            fma4(acc[0][c], p.x, v);
-            fma4(acc[1][c], p.y, v);
-            fma4(acc[2][c], p.z, v);
-            fma4(acc[3][c], p.w, v);
+            const ulonglong2 v = pairs(x + i * (DP + 4) + 4 * tx + 64 * c);
+            add_times(acc[0][c], p.x, v);
+            add_times(acc[1][c], p.y, v);
+            add_times(acc[2][c], p.z, v);
+            add_times(acc[3][c], p.w, v);
         }
     }
 }
@@ -142,7 +163,7 @@ __global__ void __launch_bounds__(THREADS) attention_forward_general_kernel(cons
     load_rows<T, DP>(sq, p.q, (int64_t)s.q0 + i0, n, head, p.head_dim);
     const Reach reach = reach_of(p.window, s, i0, i0 + n);
     const KeyTiles tiles = key_tiles<B>(reach);
-    float4 o[4][DP / 64] = {};
+    Quad o[4][DP / 64] = {};
     float top[4], sum[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) top[r] = -INFINITY, sum[r] = 0.f;
@@ -153,7 +174,7 @@ __global__ void __launch_bounds__(THREADS) attention_forward_general_kernel(cons
         load_rows<T, DP>(sv, p.v, (int64_t)s.k0 + j0, m, kv, p.head_dim);
         __syncthreads();
         float x[4][4];
-        rows_times_rows<DP>(x, sq, sk, ty, tx);
+        rows_times_rows<DP>(x, sq, sk, ty, tx, p.head_dim);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int pos = reach.first_pos + ty + 16 * r;
@@ -179,10 +200,9 @@ __global__ void __launch_bounds__(THREADS) attention_forward_general_kernel(cons
             top[r] = now;
 #pragma unroll
             for (int c = 0; c < DP / 64; ++c) {
-                o[r][c].x *= shrink;
-                o[r][c].y *= shrink;
-                o[r][c].z *= shrink;
-                o[r][c].w *= shrink;
+                const F2 by = twice(shrink);
+                o[r][c].a = ffma2(o[r][c].a, by, 0ull);
+                o[r][c].b = ffma2(o[r][c].b, by, 0ull);
             }
         }
         __syncthreads();
@@ -196,7 +216,7 @@ __global__ void __launch_bounds__(THREADS) attention_forward_general_kernel(cons
         const int64_t row = (int64_t)s.q0 + i0 + i;
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
-            const float4 v = o[r][c];
+            const float4 v = open(o[r][c]);
             collect(&bad, not_finite(v), i);
             store4<T>(p.o, row, head, 4 * tx + 64 * c, p.head_dim, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         }
@@ -213,6 +233,26 @@ __global__ void __launch_bounds__(THREADS) attention_forward_general_kernel(cons
     }
 }
 
+// Where the blocks alone would leave multiprocessors idle, the tiles that a block goes through are cut into parts, a block each, which leave
+// their sums in the workspace (parts x rows x heads x head_dim) for attention_sum_parts_kernel.
+struct Part {
+    int first, end;  // tiles
+    bool alone;      // no other part: the block stores its results itself
+};
+__device__ __forceinline__ Part part_of(const AttentionParams &p, int tiles, int part)
+{
+    const int each = p.chunk_tiles, n = max(1, (tiles + each - 1) / each);
+    return Part{part * each, part < n ? min(tiles, (part + 1) * each) : -1, n == 1};  // (end -1: there is no such part)
+}
+// The tiles of queries that see keys [j0, j0 + m): `per_head` from `from` on, for every head of the group.
+__device__ __forceinline__ void query_tiles(const AttentionParams &p, const Sequence &s, int j0, int m, int &from, int &per_head)
+{
+    int to;
+    queries_of(p.window, s, j0, j0 + m, from, to);
+    from /= B;
+    per_head = to > from * B ? (to + B - 1) / B - from : 0;
+}
+
 // dQ of 64 queries; leaves delta for attention_dkv_general_kernel.
 template <class T, int DP>
 __global__ void __launch_bounds__(THREADS) attention_dq_general_kernel(const AttentionParams p)
@@ -222,11 +262,17 @@ __global__ void __launch_bounds__(THREADS) attention_dq_general_kernel(const Att
     __shared__ float bad_lse[B], bad_delta[B];
     if (threadIdx.x == 0) bad = 0;
     float *sq = sm, *sdo = sq + B * (DP + 4), *sk = sdo + B * (DP + 4), *sv = sk + B * (DP + 4), *sds = sv + B * (DP + 4);
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = blockIdx.x % p.q_heads, kv = head / p.group;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const unsigned block_of = blockIdx.x / p.n_splits, part = blockIdx.x % p.n_splits, blocks = gridDim.x / p.n_splits;
+    const int head = block_of % p.q_heads, kv = head / p.group;
     Sequence s;
     int seq, block;
-    if (!find_block<B>(p, (gridDim.x - 1 - blockIdx.x) / p.q_heads, false, s, seq, block)) return;
+    if (!find_block<B>(p, (blocks - 1 - block_of) / p.q_heads, false, s, seq, block)) return;
     const int i0 = block * B, n = min(B, s.nq - i0);
+    const Reach reach = reach_of(p.window, s, i0, i0 + n);
+    const KeyTiles tiles = key_tiles<B>(reach);
+    const Part mine = part_of(p, tiles.n, part);
+    if (mine.end < 0) return;
     const float slope = p.slopes ? __ldg(p.slopes + head) : 0.f;
     load_rows<T, DP>(sq, p.q, (int64_t)s.q0 + i0, n, head, p.head_dim);
     load_rows<T, DP>(sdo, p.d_o, (int64_t)s.q0 + i0, n, head, p.head_dim);
@@ -244,21 +290,19 @@ __global__ void __launch_bounds__(THREADS) attention_dq_general_kernel(const Att
         if (tx == 0) {
             bad_lse[i] = lse[r];
             bad_delta[i] = delta[r];
-            if (i < n) p.delta[at] = delta[r];
+            if (i < n && part == 0) p.delta[at] = delta[r];
         }
     }
-    const Reach reach = reach_of(p.window, s, i0, i0 + n);
-    const KeyTiles tiles = key_tiles<B>(reach);
-    float4 dq[4][DP / 64] = {};
-    for (int t = 0; t < tiles.n; ++t) {
+    Quad dq[4][DP / 64] = {};
+    for (int t = mine.first; t < mine.end; ++t) {
         const int j0 = tiles.tile(t) * B, m = min(B, s.nk - j0);
         __syncthreads();
         load_rows<T, DP>(sk, p.k, (int64_t)s.k0 + j0, m, kv, p.head_dim);
         load_rows<T, DP>(sv, p.v, (int64_t)s.k0 + j0, m, kv, p.head_dim);
         __syncthreads();
         float x[4][4], dp[4][4];
-        rows_times_rows<DP>(x, sq, sk, ty, tx);
-        rows_times_rows<DP>(dp, sdo, sv, ty, tx);
+        rows_times_rows<DP>(x, sq, sk, ty, tx, p.head_dim);
+        rows_times_rows<DP>(dp, sdo, sv, ty, tx, p.head_dim);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int pos = reach.first_pos + ty + 16 * r;
@@ -277,11 +321,17 @@ __global__ void __launch_bounds__(THREADS) attention_dq_general_kernel(const Att
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        if (ty + 16 * r >= n) continue;
+        const int i = ty + 16 * r;
+        if (i >= n) continue;
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
-            collect(&bad, not_finite(dq[r][c]), ty + 16 * r);
-            store4<T>(p.dq, (int64_t)s.q0 + i0 + ty + 16 * r, head, 4 * tx + 64 * c, p.head_dim, dq[r][c]);
+            const float4 v = open(dq[r][c]);
+            if (mine.alone) {
+                collect(&bad, not_finite(v), i);
+                store4<T>(p.dq, (int64_t)s.q0 + i0 + i, head, 4 * tx + 64 * c, p.head_dim, v);
+            } else if (4 * tx + 64 * c < p.head_dim) {
+                *reinterpret_cast<float4 *>(p.part_o + ((part * p.q_rows + s.q0 + i0 + i) * p.q_heads + head) * p.head_dim + 4 * tx + 64 * c) = v;
+            }
         }
     }
     __syncthreads();
@@ -300,51 +350,53 @@ __global__ void __launch_bounds__(THREADS) attention_dkv_general_kernel(const At
     __shared__ unsigned long long bad;
     if (threadIdx.x == 0) bad = 0;
     float *sk = sm, *sv = sk + B * (DP + 4), *sq = sv + B * (DP + 4), *sdo = sq + B * (DP + 4), *sp = sdo + B * (DP + 4), *sds = sp + B * PS;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, kv = blockIdx.x % p.kv_heads;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const unsigned block_of = blockIdx.x / p.n_splits, part = blockIdx.x % p.n_splits;
+    const int kv = block_of % p.kv_heads;
     Sequence s;
     int seq, block;
     // the first keys of a causal sequence are seen by the most queries: they go first
-    if (!find_block<B>(p, blockIdx.x / p.kv_heads, true, s, seq, block)) return;
+    if (!find_block<B>(p, block_of / p.kv_heads, true, s, seq, block)) return;
     const int j0 = block * B, m = min(B, s.nk - j0);
+    int from, per_head;
+    query_tiles(p, s, j0, m, from, per_head);
+    const Part mine = part_of(p, per_head * p.group, part);
+    if (mine.end < 0) return;
     load_rows<T, DP>(sk, p.k, (int64_t)s.k0 + j0, m, kv, p.head_dim);
     load_rows<T, DP>(sv, p.v, (int64_t)s.k0 + j0, m, kv, p.head_dim);
-    int from, to;
-    queries_of(p.window, s, j0, j0 + m, from, to);
-    float4 dk[4][DP / 64] = {}, dv[4][DP / 64] = {};
-    for (int head = kv * p.group; head < (kv + 1) * p.group; ++head) {
+    Quad dk[4][DP / 64] = {}, dv[4][DP / 64] = {};
+    for (int t = mine.first; t < mine.end; ++t) {
+        const int head = kv * p.group + t / per_head, i0 = (from + t % per_head) * B, n = min(B, s.nq - i0);
         const float slope = p.slopes ? __ldg(p.slopes + head) : 0.f;
-        for (int i0 = from / B * B; i0 < to; i0 += B) {
-            const int n = min(B, s.nq - i0);
-            __syncthreads();
-            load_rows<T, DP>(sq, p.q, (int64_t)s.q0 + i0, n, head, p.head_dim);
-            load_rows<T, DP>(sdo, p.d_o, (int64_t)s.q0 + i0, n, head, p.head_dim);
-            __syncthreads();
-            float x[4][4], dp[4][4];
-            rows_times_rows<DP>(x, sq, sk, ty, tx);
-            rows_times_rows<DP>(dp, sdo, sv, ty, tx);
+        __syncthreads();
+        load_rows<T, DP>(sq, p.q, (int64_t)s.q0 + i0, n, head, p.head_dim);
+        load_rows<T, DP>(sdo, p.d_o, (int64_t)s.q0 + i0, n, head, p.head_dim);
+        __syncthreads();
+        float x[4][4], dp[4][4];
+        rows_times_rows<DP>(x, sq, sk, ty, tx, p.head_dim);
+        rows_times_rows<DP>(dp, sdo, sv, ty, tx, p.head_dim);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = ty + 16 * r, pos = s.nk - s.nq + i0 + i;
-                const int64_t at = (int64_t)head * p.q_rows + s.q0 + i0 + i;
-                const float lse = i < n ? __ldg(p.lse + at) : -INFINITY, delta = i < n ? p.delta[at] : 0.f;
+        for (int r = 0; r < 4; ++r) {
+            const int i = ty + 16 * r, pos = s.nk - s.nq + i0 + i;
+            const int64_t at = (int64_t)head * p.q_rows + s.q0 + i0 + i;
+            const float lse = i < n ? __ldg(p.lse + at) : -INFINITY, delta = i < n ? p.delta[at] : 0.f;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int j = j0 + tx + 16 * c;
-                    float dcap;
-                    const float v = score(p, slope, x[r][c], pos, j, dcap);
-                    float e = 0.f, ds = 0.f;
-                    if (lse != -INFINITY && key_seen(p.window, s, pos, j)) {
-                        e = exp2f((v - lse) * LOG2E);
-                        ds = e * (dp[r][c] - delta) * dcap * p.scale;
-                    }
-                    sp[i * PS + tx + 16 * c] = e;
-                    sds[i * PS + tx + 16 * c] = ds;
+            for (int c = 0; c < 4; ++c) {
+                const int j = j0 + tx + 16 * c;
+                float dcap;
+                const float v = score(p, slope, x[r][c], pos, j, dcap);
+                float e = 0.f, ds = 0.f;
+                if (lse != -INFINITY && key_seen(p.window, s, pos, j)) {
+                    e = exp2f((v - lse) * LOG2E);
+                    ds = e * (dp[r][c] - delta) * dcap * p.scale;
                 }
+                sp[i * PS + tx + 16 * c] = e;
+                sds[i * PS + tx + 16 * c] = ds;
             }
-            __syncthreads();
-            weights_t_times_rows<DP>(dv, sp, sdo, ty, tx);
-            weights_t_times_rows<DP>(dk, sds, sq, ty, tx);
         }
+        __syncthreads();
+        weights_t_times_rows<DP>(dv, sp, sdo, ty, tx);
+        weights_t_times_rows<DP>(dk, sds, sq, ty, tx);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -352,15 +404,72 @@ __global__ void __launch_bounds__(THREADS) attention_dkv_general_kernel(const At
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
             const int64_t row = (int64_t)s.k0 + j0 + 4 * ty + r;
-            collect(&bad, not_finite(dk[r][c]) || not_finite(dv[r][c]), 4 * ty + r);
-            store4<T>(p.dk, row, kv, 4 * tx + 64 * c, p.head_dim, dk[r][c]);
-            store4<T>(p.dv, row, kv, 4 * tx + 64 * c, p.head_dim, dv[r][c]);
+            const float4 a = open(dk[r][c]), b = open(dv[r][c]);
+            if (mine.alone) {
+                collect(&bad, not_finite(a) || not_finite(b), 4 * ty + r);
+                store4<T>(p.dk, row, kv, 4 * tx + 64 * c, p.head_dim, a);
+                store4<T>(p.dv, row, kv, 4 * tx + 64 * c, p.head_dim, b);
+            } else if (4 * tx + 64 * c < p.head_dim) {
+                float *to = p.part_o + (((2 * part) * p.k_rows + row) * p.kv_heads + kv) * p.head_dim + 4 * tx + 64 * c;
+                *reinterpret_cast<float4 *>(to) = a;
+                *reinterpret_cast<float4 *>(to + p.k_rows * p.kv_heads * p.head_dim) = b;
+            }
         }
     }
     __syncthreads();
     int turn = 0;
     for (unsigned long long left = bad; left; left &= left - 1, ++turn)
         if (turn % (THREADS / 32) == (int)threadIdx.x / 32) strict::dkv_row<T>(p, s, kv, j0 + __ffsll((long long)left) - 1);
+}
+
+// The parts' sums of 64 rows added in order; KV: dK and dV, else dQ.
+template <class T, bool KV>
+__global__ void __launch_bounds__(THREADS) attention_sum_parts_kernel(const AttentionParams p)
+{
+    __shared__ unsigned long long bad;
+    if (threadIdx.x == 0) bad = 0;
+    const int heads = KV ? p.kv_heads : p.q_heads, head = blockIdx.x % heads;
+    Sequence s;
+    int seq, block;
+    if (!find_block<B>(p, blockIdx.x / heads, KV, s, seq, block)) return;
+    const int r0 = block * B, rows = min(B, (KV ? s.nk : s.nq) - r0);
+    int tiles;
+    if (KV) {
+        int from, per_head;
+        query_tiles(p, s, r0, rows, from, per_head);
+        tiles = per_head * p.group;
+    } else {
+        tiles = key_tiles<B>(reach_of(p.window, s, r0, r0 + rows)).n;
+    }
+    const int parts = (tiles + p.chunk_tiles - 1) / p.chunk_tiles;
+    if (parts <= 1) return;
+    __syncthreads();
+    const int quads = p.head_dim / 4;
+    const int64_t array = (KV ? p.k_rows : p.q_rows) * heads * p.head_dim;
+    for (int i = threadIdx.x; i < rows * quads; i += THREADS) {
+        const int r = i / quads, c = i % quads * 4;
+        const int64_t row = (int64_t)(KV ? s.k0 : s.q0) + r0 + r;
+#pragma unroll
+        for (int x = 0; x < (KV ? 2 : 1); ++x) {
+            const float *from = p.part_o + x * array + (row * heads + head) * p.head_dim + c;
+            float4 sum = at4(from);
+            for (int k = 1; k < parts; ++k) {
+                const float4 v = at4(from + k * array * (KV ? 2 : 1));
+                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            }
+            collect(&bad, not_finite(sum), r);
+            store4<T>(KV ? (x ? p.dv : p.dk) : p.dq, row, head, c, p.head_dim, sum);
+        }
+    }
+    __syncthreads();
+    int turn = 0;
+    for (unsigned long long left = bad; left; left &= left - 1, ++turn) {
+        const int r = __ffsll((long long)left) - 1;
+        if (turn % (THREADS / 32) != (int)threadIdx.x / 32) continue;
+        const int64_t at = (int64_t)head * p.q_rows + s.q0 + r0 + r;
+        if (KV) strict::dkv_row<T>(p, s, head, r0 + r);
+        else strict::dq_row<T>(p, s, head, r0 + r, __ldg(p.lse + at), p.delta[at]);
+    }
 }
 
 template <class Kern>
@@ -382,33 +491,68 @@ cudaError_t forward_of(const AttentionParams &p, cudaStream_t s)
     return launch(attention_forward_general_kernel<T, DP>, optin, grid, smem_of(DP, 3, 1), p, s);
 }
 template <class T, int DP>
-cudaError_t backward_of(const AttentionParams &p, cudaStream_t s)
+cudaError_t backward_of(const AttentionParams &p0, const GeneralParts &parts, cudaStream_t s)
 {
-    static SmemOptinCache optin_q, optin_kv;
-    const unsigned grid_q = (unsigned)(p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, B));
-    const unsigned grid_kv = (unsigned)(p.kv_heads * most_blocks(p.k_rows, p.n_seqs, p.max_k, B));
-    const cudaError_t e = launch(attention_dq_general_kernel<T, DP>, optin_q, grid_q, smem_of(DP, 4, 1), p, s);
-    return e != cudaSuccess ? e : launch(attention_dkv_general_kernel<T, DP>, optin_kv, grid_kv, smem_of(DP, 4, 2), p, s);
+    static SmemOptinCache optin_q, optin_kv, none;
+    const unsigned grid_q = (unsigned)(p0.q_heads * most_blocks(p0.q_rows, p0.n_seqs, p0.max_q, B));
+    const unsigned grid_kv = (unsigned)(p0.kv_heads * most_blocks(p0.k_rows, p0.n_seqs, p0.max_k, B));
+    AttentionParams p = p0;
+    p.n_splits = parts.n_q;
+    p.chunk_tiles = parts.tiles_q;
+    cudaError_t e = launch(attention_dq_general_kernel<T, DP>, optin_q, grid_q * parts.n_q, smem_of(DP, 4, 1), p, s);
+    if (e == cudaSuccess && parts.n_q > 1) e = launch(attention_sum_parts_kernel<T, false>, none, grid_q, 0, p, s);
+    if (e != cudaSuccess) return e;
+    p.n_splits = parts.n_kv;
+    p.chunk_tiles = parts.tiles_kv;
+    e = launch(attention_dkv_general_kernel<T, DP>, optin_kv, grid_kv * parts.n_kv, smem_of(DP, 4, 2), p, s);
+    if (e == cudaSuccess && parts.n_kv > 1) e = launch(attention_sum_parts_kernel<T, true>, none, grid_kv, 0, p, s);
+    return e;
 }
 
+// parts null: forward
 template <class T>
-cudaError_t by_width(bool backward, const AttentionParams &p, cudaStream_t s)
+cudaError_t by_width(const GeneralParts *parts, const AttentionParams &p, cudaStream_t s)
 {
-    if (p.head_dim <= 64) return backward ? backward_of<T, 64>(p, s) : forward_of<T, 64>(p, s);
-    return backward ? backward_of<T, 128>(p, s) : forward_of<T, 128>(p, s);
+    if (p.head_dim <= 64) return parts ? backward_of<T, 64>(p, *parts, s) : forward_of<T, 64>(p, s);
+    return parts ? backward_of<T, 128>(p, *parts, s) : forward_of<T, 128>(p, s);
 }
-cudaError_t by_type(bool backward, const AttentionParams &p, cudaStream_t s)
+cudaError_t by_type(const GeneralParts *parts, const AttentionParams &p, cudaStream_t s)
 {
     switch (p.dtype) {
-    case 0: return by_width<float>(backward, p, s);
-    case 1: return by_width<__half>(backward, p, s);
-    default: return by_width<__nv_bfloat16>(backward, p, s);
+    case 0: return by_width<float>(parts, p, s);
+    case 1: return by_width<__half>(parts, p, s);
+    default: return by_width<__nv_bfloat16>(parts, p, s);
     }
 }
 
 }  // namespace
 
-cudaError_t launch_attention_forward_general(const AttentionParams &p, cudaStream_t s) { return by_type(false, p, s); }
-cudaError_t launch_attention_backward_general(const AttentionParams &p, cudaStream_t s) { return by_type(true, p, s); }
+GeneralParts plan_general_parts(const AttentionParams &p, int sm_count)
+{
+    // Parts until there are four blocks for a multiprocessor (a causal mask leaves some with little to do), of two tiles at least, and at
+    // most 256 MB of sums.
+    auto cut = [&](int64_t blocks, int64_t tiles, int64_t bytes_of_one, int &n, int &each) {
+        n = 1;
+        each = (int)(tiles > 0 ? tiles : 1);
+        if (blocks <= 0 || tiles <= 2) return;
+        int64_t want = (4ll * sm_count + blocks - 1) / blocks;
+        if (want > (256ll << 20) / (bytes_of_one > 0 ? bytes_of_one : 1)) want = (256ll << 20) / (bytes_of_one > 0 ? bytes_of_one : 1);
+        if (want > (tiles + 1) / 2) want = (tiles + 1) / 2;
+        if (want <= 1) return;
+        each = (int)((tiles + want - 1) / want);
+        n = (int)((tiles + each - 1) / each);
+    };
+    GeneralParts g{1, 1 << 30, 1, 1 << 30, 0};
+    if (p.dtype != 0) return g;  // (16-bit types come here for their strides alone: no workspace for that)
+    const int64_t bytes_q = 4 * p.q_rows * p.q_heads * p.head_dim, bytes_kv = 8 * p.k_rows * p.kv_heads * p.head_dim;
+    cut(p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, B), (p.max_k + B - 1) / B, bytes_q, g.n_q, g.tiles_q);
+    cut(p.kv_heads * most_blocks(p.k_rows, p.n_seqs, p.max_k, B), (int64_t)((p.max_q + B - 1) / B) * p.group, bytes_kv, g.n_kv, g.tiles_kv);
+    const int64_t q = g.n_q > 1 ? g.n_q * bytes_q : 0, kv = g.n_kv > 1 ? g.n_kv * bytes_kv : 0;
+    g.bytes = q > kv ? q : kv;  // one behind the other
+    return g;
+}
+
+cudaError_t launch_attention_forward_general(const AttentionParams &p, cudaStream_t s) { return by_type(nullptr, p, s); }
+cudaError_t launch_attention_backward_general(const AttentionParams &p, const GeneralParts &parts, cudaStream_t s) { return by_type(&parts, p, s); }
 
 }  // namespace sddmm
