@@ -19,6 +19,10 @@ namespace {
 
 constexpr int KEYS = 16, WARPS = 4, STAGES = 3, ROWS = 16;
 constexpr float RAISE = 8.f;
+#ifndef MOST_TILES
+#define MOST_TILES 64
+#endif
+constexpr int RESIDENT = 2, LEAST_TILES = 16;
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
 {
@@ -66,7 +70,6 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attention_few_kernel(const Atte
     constexpr int ROW_BYTES = DP * 2, PIECES = DP / 8, TILE_BYTES = KEYS * ROW_BYTES, STAGE_BYTES = 2 * TILE_BYTES;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ float w_most[WARPS][ROWS], w_sum[WARPS][ROWS], r_lse[ROWS];
-    __shared__ unsigned bad;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned b = blockIdx.x / p.n_splits, chunk = blockIdx.x % p.n_splits;
     const int tile = b % row_tiles, kv = b / row_tiles % p.kv_heads, seq = b / row_tiles / p.kv_heads;
@@ -77,7 +80,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attention_few_kernel(const Atte
     if ((int)chunk >= ch.n) return;
     const int first = chunk * p.chunk_tiles, end = min(ch.keys.n, first + p.chunk_tiles);
     const int D = p.head_dim;
-    if (threadIdx.x == 0) bad = 0;
+    if (p.n_splits > 1 && threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
 
     // ---- the ring: this warp's tiles first + warp, + 4, ... ----
     const int mine = max(0, (end - first - warp + WARPS - 1) / WARPS);
@@ -267,49 +270,68 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attention_few_kernel(const Atte
     }
 }
 
-// The parts of one row added up, a block for a row: warps take chunks in turn.
+// The parts of one row added up, a block for a row: warps take chunks in turn, eight at once, so that all of a row's parts are asked for
+// before the first is used.
 template <class E>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionParams p)
 {
-    constexpr int JOIN_WARPS = 8;
-    __shared__ float part[JOIN_WARPS][128], weight[JOIN_WARPS];
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // this grid may have been started before the parts were written
+    constexpr int JOIN_WARPS = 8, AT_ONCE = 8;
+    __shared__ float part[JOIN_WARPS][128], w_most[JOIN_WARPS], w_sum[JOIN_WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.head_dim;
     const int head = blockIdx.x % p.q_heads, i = blockIdx.x / p.q_heads % p.max_q, seq = blockIdx.x / p.q_heads / p.max_q;
     const Sequence s = sequence_of(p, seq);
     if (i >= s.nq) return;
     const int n = chunks_of(p, s, (i * p.group + head % p.group) / ROWS).n;
     if (n == 1) return;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // this grid may have been started before the parts were written
     const int64_t stride = (int64_t)p.q_rows * p.q_heads, at = ((int64_t)s.q0 + i) * p.q_heads + head;
-    float top = -INFINITY;
-    for (int c = lane; c < n; c += 32) top = fmaxf(top, p.part_lse[c * stride + at]);
+    float y[4] = {}, top = -INFINITY, total = 0.f;
+    for (int c0 = warp; c0 < n; c0 += JOIN_WARPS * AT_ONCE) {
+        float l[AT_ONCE];
+        float4 v[AT_ONCE];
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float base = top == -INFINITY ? 0.f : top;
-    float y[4] = {}, total = 0.f;
-#pragma unroll 4
-    for (int c = warp; c < n; c += JOIN_WARPS) {
-        const float w = tc::ex2(p.part_lse[c * stride + at] - base);
-        total += w;
-        if (4 * lane < D) {
-            const float4 v = *reinterpret_cast<const float4 *>(p.part_o + (c * stride + at) * D + 4 * lane);
-            y[0] = fmaf(w, v.x, y[0]), y[1] = fmaf(w, v.y, y[1]), y[2] = fmaf(w, v.z, y[2]), y[3] = fmaf(w, v.w, y[3]);
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const int c = c0 + k * JOIN_WARPS;
+            l[k] = c < n ? p.part_lse[c * stride + at] : -INFINITY;
+            v[k] = c < n && 4 * lane < D ? *reinterpret_cast<const float4 *>(p.part_o + (c * stride + at) * D + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float now = top;
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) now = fmaxf(now, l[k]);
+        const float base = now == -INFINITY ? 0.f : now, shrink = tc::ex2(top - base);
+        top = now;
+        total *= shrink;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) y[x] *= shrink;
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const float w = tc::ex2(l[k] - base);
+            total += w;
+            y[0] = fmaf(w, v[k].x, y[0]), y[1] = fmaf(w, v[k].y, y[1]), y[2] = fmaf(w, v[k].z, y[2]), y[3] = fmaf(w, v[k].w, y[3]);
         }
     }
     *reinterpret_cast<float4 *>(&part[warp][4 * lane]) = make_float4(y[0], y[1], y[2], y[3]);
-    if (lane == 0) weight[warp] = total;
+    if (lane == 0) w_most[warp] = top, w_sum[warp] = total;
     __syncthreads();
     if (warp != 0) return;
+    top = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < JOIN_WARPS; ++v) top = fmaxf(top, w_most[v]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float by[JOIN_WARPS];
     total = 0.f;
 #pragma unroll
-    for (int v = 0; v < JOIN_WARPS; ++v) total += weight[v];
+    for (int v = 0; v < JOIN_WARPS; ++v) {
+        by[v] = tc::ex2(w_most[v] - base);
+        total += by[v] * w_sum[v];
+    }
     const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : NAN;
     const float lse = total == 0.f ? -INFINITY : (base + log2f(total)) * LN2;
     bool wrong = false;
     for (int d = lane; d < D; d += 32) {
         float x = 0.f;
 #pragma unroll
-        for (int v = 0; v < JOIN_WARPS; ++v) x += part[v][d];
+        for (int v = 0; v < JOIN_WARPS; ++v) x = fmaf(by[v], part[v][d], x);
         x *= inv;
         wrong = wrong || !isfinite(x);
         static_cast<E *>(p.o.data)[((int64_t)s.q0 + i) * p.o.row + head * p.o.head + d] = from_f<E>(x);
@@ -362,10 +384,15 @@ FewPlan plan_attention_few(const AttentionParams &p, int sm_count)
     if (p.dtype == 0 || (int64_t)p.max_q * p.group > MOST_FEW_ROWS || p.max_q == 0 || p.n_seqs == 0) return f;
     const int64_t row_tiles = (p.max_q * p.group + ROWS - 1) / ROWS, blocks = row_tiles * p.kv_heads * p.n_seqs;
     const int64_t tiles = (p.max_k + KEYS - 1) / KEYS + 1;  // (+ 1: prefix and window may begin inside tiles)
-    int64_t chunk = 16;                                      // 256 keys
     auto bytes_of = [&](int64_t n) { return n == 1 ? 0 : n * p.q_rows * p.q_heads * (int64_t)(p.head_dim + 1) * 4; };
     auto n_of = [&](int64_t c) { return tiles <= c ? (int64_t)1 : (tiles + c - 1) / c; };
-    while (n_of(chunk) > 1 && (n_of(2 * chunk) * blocks >= 8ll * sm_count || bytes_of(n_of(chunk)) > (1ll << 30))) chunk *= 2;
+    // As many chunks as fill whole waves of resident blocks (RESIDENT for a multiprocessor), of MOST_TILES key tiles at most: longer ones leave
+    // the last block of ragged sequences alone, shorter ones spend their time beginning and ending.
+    const int64_t resident = (int64_t)RESIDENT * sm_count, waves = (tiles * blocks + resident * MOST_TILES - 1) / (resident * MOST_TILES);
+    const int64_t want = resident * waves / blocks > 1 ? resident * waves / blocks : 1;
+    int64_t chunk = ((tiles + want - 1) / want + WARPS - 1) / WARPS * WARPS;
+    if (chunk < LEAST_TILES) chunk = LEAST_TILES;
+    while (n_of(chunk) > 1 && bytes_of(n_of(chunk)) > (1ll << 30)) chunk *= 2;
     const int64_t n = n_of(chunk);
     if (n * blocks > INT32_MAX || (int64_t)p.n_seqs * p.max_q * p.q_heads > INT32_MAX) return f;
     f.chunk_tiles = (int)chunk;
