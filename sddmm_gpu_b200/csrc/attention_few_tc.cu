@@ -22,7 +22,8 @@ constexpr float RAISE = 8.f;
 #ifndef MOST_TILES
 #define MOST_TILES 64
 #endif
-constexpr int RESIDENT = 2, LEAST_TILES = 16;
+constexpr int LEAST_TILES = 16;
+constexpr int resident_blocks(int head_dim) { return head_dim <= 64 ? 4 : 2; }  // of a multiprocessor, by registers
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
 {
@@ -65,13 +66,14 @@ __device__ __forceinline__ Chunks chunks_of(const AttentionParams &p, const Sequ
 }
 
 template <class E, int DP, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(WARPS * 32, 2) attention_few_kernel(const AttentionParams p, int row_tiles)
+__global__ void __launch_bounds__(WARPS * 32, resident_blocks(DP)) attention_few_kernel(const AttentionParams p, int row_tiles)
 {
     constexpr int ROW_BYTES = DP * 2, PIECES = DP / 8, TILE_BYTES = KEYS * ROW_BYTES, STAGE_BYTES = 2 * TILE_BYTES;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ float w_most[WARPS][ROWS], w_sum[WARPS][ROWS], r_lse[ROWS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const unsigned b = blockIdx.x / p.n_splits, chunk = blockIdx.x % p.n_splits;
+    // first chunks first: those that a short sequence does not have come last
+    const unsigned heads_and_rows = gridDim.x / p.n_splits, b = blockIdx.x % heads_and_rows, chunk = blockIdx.x / heads_and_rows;
     const int tile = b % row_tiles, kv = b / row_tiles % p.kv_heads, seq = b / row_tiles / p.kv_heads;
     const Sequence s = sequence_of(p, seq);
     const int rows = s.nq * p.group, r0 = tile * ROWS;
@@ -231,7 +233,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attention_few_kernel(const Atte
     const bool last = ch.n == 1;
 #pragma unroll
     for (int x = 0; x < ROWS / WARPS; ++x) {
-        const int r = warp * (ROWS / WARPS) + x;
+        const int r = warp + x * WARPS;
         if (r0 + r >= rows) break;
         const int i = (r0 + r) / p.group, head = kv * p.group + (r0 + r) % p.group;
         float top = -INFINITY, total = 0.f;
@@ -386,9 +388,9 @@ FewPlan plan_attention_few(const AttentionParams &p, int sm_count)
     const int64_t tiles = (p.max_k + KEYS - 1) / KEYS + 1;  // (+ 1: prefix and window may begin inside tiles)
     auto bytes_of = [&](int64_t n) { return n == 1 ? 0 : n * p.q_rows * p.q_heads * (int64_t)(p.head_dim + 1) * 4; };
     auto n_of = [&](int64_t c) { return tiles <= c ? (int64_t)1 : (tiles + c - 1) / c; };
-    // As many chunks as fill whole waves of resident blocks (RESIDENT for a multiprocessor), of MOST_TILES key tiles at most: longer ones leave
+    // As many chunks as fill whole waves of resident blocks, of MOST_TILES key tiles at most: longer ones leave
     // the last block of ragged sequences alone, shorter ones spend their time beginning and ending.
-    const int64_t resident = (int64_t)RESIDENT * sm_count, waves = (tiles * blocks + resident * MOST_TILES - 1) / (resident * MOST_TILES);
+    const int64_t resident = (int64_t)resident_blocks(p.head_dim) * sm_count, waves = (tiles * blocks + resident * MOST_TILES - 1) / (resident * MOST_TILES);
     const int64_t want = resident * waves / blocks > 1 ? resident * waves / blocks : 1;
     int64_t chunk = ((tiles + want - 1) / want + WARPS - 1) / WARPS * WARPS;
     if (chunk < LEAST_TILES) chunk = LEAST_TILES;
