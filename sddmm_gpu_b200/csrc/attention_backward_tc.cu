@@ -10,10 +10,10 @@
 // fp32 array of its own.  P and dS are rounded to the operands' type, as every operand of the tensor cores is; fp16 thus
 // limits |P (dP - delta)| to 65,504.
 //
-//   warps 0-7  a row of the block in every thread, a half of the tile's columns in each group of four warps: scores from tensor
-//              memory, weights and score gradients back to it;
-//   warp 8     one thread issues the products; the second operand of the last ones is the streamed tile as it lies, MN-major;
-//   warp 9     one thread brings the tiles by tile copies.
+//   warps 0-15  a row of the block in every thread, a quarter of the tile's columns in each group of four warps: scores from tensor
+//               memory, weights and score gradients back to it;
+//   warp 16     one thread issues the products; the second operand of the last ones is the streamed tile as it lies, MN-major;
+//   warp 17     one thread brings the tiles by tile copies.
 //
 // dQ: score gradients have a place of their own in tensor memory (two, in turn), so the next tile's scores are computed as soon as the
 // last ones have been read.  dK, dV: tensor memory is full (S, dP, dV, dK); P and dS take the place of S and dP, and the
@@ -30,14 +30,17 @@ namespace {
 using tc::mbar_arrive;
 using tc::mbar_fence_init;
 using tc::mbar_init;
+using tc::F2;
 
 constexpr int T = 128;
-constexpr int ROW_WARPS = 8, MMA_WARP = 8, LOAD_WARP = 9, THREADS = 384;
+constexpr int ROW_WARPS = 16, MMA_WARP = 16, LOAD_WARP = 17, THREADS = 640;
+constexpr int MINE = 32;  // columns of a thread
 constexpr uint32_t TMEM_COLUMNS = 512, S_AT = 0, DP_AT = 128;
 // dQ: accumulator, then two places of 64 columns for score gradients.  dK, dV: the two accumulators.
 constexpr uint32_t DQ_AT = 256, DS_AT = 384, DV_AT = 256, DK_AT = 384;
-#define ROW_REGISTERS "216"
-#define OTHER_REGISTERS "72"
+// Registers of a thread: 96 at launch (640 threads), shared out anew: 4 x 104 + 64 = 5 x 96.
+#define ROW_REGISTERS "104"
+#define OTHER_REGISTERS "64"
 
 struct alignas(64) Maps {
     CUtensorMap q, k, v, d_o;
@@ -46,7 +49,7 @@ struct alignas(64) Maps {
 template <int DP, bool KV> struct Shape {
     static constexpr int BOXES = DP / 64, TILE_BYTES = T * DP * 2, BOX_BYTES = T * 128;
     static constexpr int SLOTS = DP == 64 ? 8 : KV ? 4 : 5;                        // of one streamed tile
-    static constexpr int STATS = KV ? ROW_WARPS * 2 * 64 * 4 : 0;                  // lse and delta of a warp's 64 columns
+    static constexpr int STATS = KV ? ROW_WARPS * 2 * MINE * 4 : 0;                // lse and delta of a warp's columns
     static constexpr int SMEM = (2 + SLOTS) * TILE_BYTES + STATS;
 };
 
@@ -60,7 +63,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
     // dQ: s_full = scores and dP there, p_ready = they have been read
     __shared__ uint64_t own_full, full[SLOTS], empty[SLOTS], s_full, dp_full, p_ready, ds_ready, acc_full, tail;
     __shared__ uint32_t tmem_holder, bad[4];
-    __shared__ float row_lse[T], row_delta[2][T];
+    __shared__ float row_lse[T], row_delta[T];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int heads = KV ? p.kv_heads : p.q_heads, head = blockIdx.x % heads, kv = KV ? head : head / p.group;
     Sequence s;
@@ -99,23 +102,38 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
     }
     if (threadIdx.x < 4) bad[threadIdx.x] = 0;
     if (warp == MMA_WARP) tc::tmem_alloc(&tmem_holder, TMEM_COLUMNS);
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane;  // of warps 0-7
+    const int group = warp >> 2, row = (warp & 3) * 32 + lane;  // of warps 0-15: columns MINE * group .. of that row
     if (!KV && warp < ROW_WARPS) {
-        // half of a row's delta in each thread
-        float d = 0.f;
-        if (row < n_rows) {
-            const int64_t at = (int64_t)s.q0 + r0 + row;
-            const E *o = static_cast<const E *>(p.o.data) + at * p.o.row + head * p.o.head;
-            const E *d_o = static_cast<const E *>(p.d_o.data) + at * p.d_o.row + head * p.d_o.head;
-            for (int c = half * (DP / 2); c < min(p.head_dim, (half + 1) * (DP / 2)); c += 8) {
-                uint4 x = *reinterpret_cast<const uint4 *>(o + c), y = *reinterpret_cast<const uint4 *>(d_o + c);
-                const E *xe = reinterpret_cast<const E *>(&x), *ye = reinterpret_cast<const E *>(&y);
+        // delta: 16 bytes of O and dO in each lane, DP / 8 lanes a row, all rows of the warp asked for at once
+        constexpr int LANES = DP / 8, AT_ONCE = 32 / LANES, TURNS = T / ROW_WARPS / AT_ONCE;
+        uint4 o[TURNS], d_o[TURNS];
+        const int c = lane % LANES * 8;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) d = fmaf(to_f(xe[e]), to_f(ye[e]), d);
+        for (int k = 0; k < TURNS; ++k) {
+            const int r = warp * (T / ROW_WARPS) + k * AT_ONCE + lane / LANES;
+            const int64_t at = (int64_t)s.q0 + r0 + r;
+            o[k] = d_o[k] = make_uint4(0, 0, 0, 0);
+            if (r < n_rows && c < p.head_dim) {
+                o[k] = *reinterpret_cast<const uint4 *>(static_cast<const E *>(p.o.data) + at * p.o.row + head * p.o.head + c);
+                d_o[k] = *reinterpret_cast<const uint4 *>(static_cast<const E *>(p.d_o.data) + at * p.d_o.row + head * p.d_o.head + c);
             }
-            if (half == 0) row_lse[row] = __ldg(p.lse + (int64_t)head * p.q_rows + at);
         }
-        row_delta[half][row] = d;
+#pragma unroll
+        for (int k = 0; k < TURNS; ++k) {
+            const int r = warp * (T / ROW_WARPS) + k * AT_ONCE + lane / LANES;
+            const E *a = reinterpret_cast<const E *>(&o[k]), *b = reinterpret_cast<const E *>(&d_o[k]);
+            float d = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d = fmaf(to_f(a[e]), to_f(b[e]), d);
+#pragma unroll
+            for (int x = LANES / 2; x >= 1; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
+            if (lane % LANES == 0) {
+                const int64_t at = (int64_t)head * p.q_rows + s.q0 + r0 + r;
+                row_delta[r] = d;
+                row_lse[r] = r < n_rows ? __ldg(p.lse + at) : -INFINITY;
+                if (r < n_rows) p.delta[at] = d;
+            }
+        }
     }
     tc::fence_before();
     __syncthreads();
@@ -167,24 +185,26 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                 for (int n = issued > SLOTS ? issued - SLOTS : 0; n < issued; ++n) (void)tc::wait(&full[n % SLOTS], (n / SLOTS) & 1);
         } else if (warp == MMA_WARP) {
             constexpr uint32_t ID_S = tc::instr_desc(BF16, T, T, false, false), ID_ACC = tc::instr_desc(BF16, T, DP, false, true);
+            const uint64_t own_desc = tc::smem_desc(base, 16), rows_desc = tc::smem_desc(ring, 16), tile_desc = tc::smem_desc(ring, BOX_BYTES);
             // own tile x (0 or 1) times the streamed tile of a slot, rows by rows
             auto rows_by_rows = [&](uint32_t to, int x, int slot) {
+                const uint64_t a = own_desc + x * (TILE_BYTES >> 4), b = rows_desc + __shfl_sync(0xffffffffu, slot, 0) * (TILE_BYTES >> 4);
                 if (tc::elected()) {
 #pragma unroll
                     for (int k = 0; k < DP / 16; ++k) {
-                        const uint32_t o = k / 4 * BOX_BYTES + k % 4 * 32;
-                        tc::mma_ss(tmem + to, tc::smem_desc(base + x * TILE_BYTES + o, 16), tc::smem_desc(ring + slot * TILE_BYTES + o, 16), ID_S, k > 0);
+                        const int o = (k / 4 * BOX_BYTES + k % 4 * 32) >> 4;
+                        tc::mma_ss(tmem + to, a + o, b + o, ID_S, k > 0);
                     }
                 }
                 __syncwarp();
             };
-            // accumulator += weights (two runs of 32 columns, `apart` columns from one to the next) times the streamed tile
+            // accumulator += weights (runs of 16 columns, `apart` columns from one to the next) times the streamed tile
             auto weights_by_tile = [&](uint32_t to, uint32_t weights, uint32_t apart, int slot, bool add) {
+                const uint64_t b = tile_desc + __shfl_sync(0xffffffffu, slot, 0) * (TILE_BYTES >> 4);
                 if (tc::elected()) {
 #pragma unroll
                     for (int k = 0; k < T / 16; ++k)
-                        tc::mma_ts(tmem + to, tmem + weights + k / 4 * apart + k % 4 * 8, tc::smem_desc(ring + slot * TILE_BYTES + k * 2048, BOX_BYTES), ID_ACC,
-                                   add || k > 0);
+                        tc::mma_ts(tmem + to, tmem + weights + k / 2 * apart + k % 2 * 8, b + k * (2048 >> 4), ID_ACC, add || k > 0);
                 }
                 __syncwarp();
             };
@@ -216,7 +236,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                     ok = tc::warp_wait(&p_ready, j & 1);
                     if (!ok) break;
                     tc::fence_after();
-                    weights_by_tile(DV_AT, S_AT, 64, slot_of(n + 1), j > 0);
+                    weights_by_tile(DV_AT, S_AT, MINE, slot_of(n + 1), j > 0);
                     done(&empty[slot_of(n + 1)]);
                     if (more) {
                         if (!wait_tile(n + 2)) break;
@@ -226,7 +246,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                     ok = tc::warp_wait(&ds_ready, j & 1);
                     if (!ok) break;
                     tc::fence_after();
-                    weights_by_tile(DK_AT, DP_AT, 64, slot_of(n), j > 0);
+                    weights_by_tile(DK_AT, DP_AT, MINE, slot_of(n), j > 0);
                     done(&empty[slot_of(n)]);
                     if (more) {
                         if (!wait_tile(n + 3)) break;
@@ -247,7 +267,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                     ok = tc::warp_wait(&ds_ready, j & 1);
                     if (!ok) break;
                     tc::fence_after();
-                    weights_by_tile(DQ_AT, DS_AT + 64 * (j & 1), 32, slot_of(n), j > 0);
+                    weights_by_tile(DQ_AT, DS_AT + 64 * (j & 1), MINE / 2, slot_of(n), j > 0);
                     done(&empty[slot_of(n)]);
                 }
             }
@@ -259,12 +279,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 " ROW_REGISTERS ";");
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const float c = CAP ? 2.f * LOG2E * p.scale / p.cap : p.scale * LOG2E, top_of = p.cap * LOG2E;
+        const float c = CAP ? p.scale / p.cap : p.scale * LOG2E, top_of = p.cap * LOG2E;
+        const tc::TanhCoefficients tanh_c = tc::tanh_coefficients(1.f);
         float slope = BIAS && !KV ? __ldg(p.slopes + head) * LOG2E : 0.f;
         const int off = s.nk - s.nq;
         // what a row sees: columns [lo, hi] of the other side, and the first `pre`
         int lo, hi, pre;
-        float lse2 = 0.f, delta = 0.f;
+        float lse2 = 0.f, delta = 0.f;  // dQ: of the row, negative
         if (KV) {
             const int j = r0 + row;
             pre = j < s.prefix ? s.nq : 0;
@@ -276,30 +297,24 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             pre = s.prefix;
             lo = p.window.left < 0 ? 0 : max(0, pos - p.window.left);
             hi = p.window.right < 0 ? s.nk - 1 : min(s.nk - 1, pos + p.window.right);
-            const float lse = row < n_rows ? row_lse[row] : -INFINITY;
-            delta = row_delta[0][row] + row_delta[1][row];
-            lse2 = lse == -INFINITY ? INFINITY : lse * LOG2E;  // a row that has seen nothing: weights of zero
-            if (half == 0 && row < n_rows) p.delta[(int64_t)head * p.q_rows + s.q0 + r0 + row] = delta;
+            delta = -row_delta[row];
+            lse2 = row_lse[row] == -INFINITY ? -INFINITY : -row_lse[row] * LOG2E;  // a row that has seen nothing: weights of zero
         }
-        float *const my_lse = reinterpret_cast<float *>(smem + (2 + SLOTS) * TILE_BYTES) + warp * 128, *const my_delta = my_lse + 64;
-        float ahead[4] = {};
-        auto fetch = [&](int j) {  // lse and delta of this warp's 64 columns of tile j
-            const int i = tile_at(j) + 64 * half + lane;
+        float *const my_lse = reinterpret_cast<float *>(smem + (2 + SLOTS) * TILE_BYTES) + warp * 2 * MINE, *const my_delta = my_lse + MINE;
+        float next_lse = 0.f, next_delta = 0.f;
+        auto fetch = [&](int j) {  // lse and delta, negative, of this warp's columns of tile j, one a lane
+            const int i = tile_at(j) + MINE * group + lane;
             const int64_t at = (int64_t)head_at(j) * p.q_rows + s.q0 + i;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const bool in = i + 32 * x < s.nq;
-                const float l = in ? __ldg(p.lse + at + 32 * x) : -INFINITY;
-                ahead[x] = l == -INFINITY ? INFINITY : l * LOG2E;
-                ahead[2 + x] = in ? __ldg(p.delta + at + 32 * x) : 0.f;
-            }
+            const float l = i < s.nq ? __ldg(p.lse + at) : -INFINITY;
+            next_lse = l == -INFINITY ? -INFINITY : -l * LOG2E;
+            next_delta = i < s.nq ? -__ldg(p.delta + at) : 0.f;
         };
         if (KV && count > 0) fetch(0);
         for (int j = 0; j < count && ok; ++j) {
-            const int t0 = tile_at(j), c0 = t0 + 64 * half;
+            const int t0 = tile_at(j), c0 = t0 + MINE * group;
             if (KV) {
                 __syncwarp();
-                my_lse[lane] = ahead[0], my_lse[lane + 32] = ahead[1], my_delta[lane] = ahead[2], my_delta[lane + 32] = ahead[3];
+                my_lse[lane] = next_lse, my_delta[lane] = next_delta;
                 __syncwarp();
                 if (BIAS) slope = __ldg(p.slopes + head_at(j)) * LOG2E;
                 if (j + 1 < count) fetch(j + 1);
@@ -307,50 +322,81 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             bool open;
             if (KV) open = n_rows == T && t0 + T <= s.nq && tile_is_open<T>(p.window, s, reach_of(p.window, s, t0, t0 + T), r0);
             else open = tile_is_open<T>(p.window, s, reach, t0);
+            const unsigned seen = open ? ~0u : seen_bits(lo, hi, pre, c0);
             ok = tc::warp_wait(&s_full, j & 1);
             if (!ok) break;
             tc::fence_after();
-            float x[64], y[64];
-            tc::tmem_ld32(reinterpret_cast<uint32_t *>(x), mine + S_AT + 64 * half);
-            tc::tmem_ld32(reinterpret_cast<uint32_t *>(x) + 32, mine + S_AT + 64 * half + 32);
-            if (!KV) {
-                tc::tmem_ld32(reinterpret_cast<uint32_t *>(y), mine + DP_AT + 64 * half);
-                tc::tmem_ld32(reinterpret_cast<uint32_t *>(y) + 32, mine + DP_AT + 64 * half + 32);
-            }
+            F2 x[MINE / 2], y[MINE / 2];  // two columns each
+            tc::tmem_ld32(reinterpret_cast<uint32_t *>(x), mine + S_AT + MINE * group);
+            if (!KV) tc::tmem_ld32(reinterpret_cast<uint32_t *>(y), mine + DP_AT + MINE * group);
             tc::wait_ld();
             if (!KV) {
                 tc::fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_ready);  // the next tile's scores may come
             }
-            // weights; with a cap, x leaves as weight times (1 - tanh^2), and w holds the weights
-            const unsigned seen[2] = {open ? ~0u : seen_bits(lo, hi, pre, c0), open ? ~0u : seen_bits(lo, hi, pre, c0 + 32)};
             const float away = KV ? (float)(off + c0 - (r0 + row)) : (float)(c0 - (off + r0 + row));
-            uint32_t w[32];
+            bool small = true;
+            if (CAP) {
+                float size = 0.f;
 #pragma unroll
-            for (int u = 0; u < 64; u += 2) {
-                float l2[2] = {lse2, lse2}, e[2];
-                if (KV) {
-                    const float2 l = *reinterpret_cast<const float2 *>(my_lse + u);
-                    l2[0] = l.x, l2[1] = l.y;
+                for (int u = 0; u < MINE / 2; ++u) {
+                    float a, b;
+                    tc::split(x[u], a, b);
+                    size = tc::max3_abs(size, a, b);
                 }
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    float z = x[u + v], slope_of_cap = 1.f;
-                    if (CAP) {
-                        const float g = tc::rcp(1.f + tc::ex2(z * c));  // tanh = 1 - 2 g
-                        z = fmaf(-2.f * top_of, g, top_of);
-                        slope_of_cap = 4.f * g * (1.f - g);
-                    }
-                    if (BIAS) z = fmaf(-slope, fabsf(away + (float)(u + v)), CAP ? z : z * c);
-                    e[v] = tc::ex2(CAP || BIAS ? z - l2[v] : fmaf(z, c, -l2[v]));
-                    x[u + v] = CAP ? e[v] * slope_of_cap : e[v];
-                    if (!(seen[u / 32] & 1u << (u + v) % 32)) e[v] = x[u + v] = 0.f;
-                }
-                if (KV) w[u / 2] = tc::pack<E>(e[0], e[1]);
+                small = __all_sync(0xffffffffu, size * c <= tc::TANH_RANGE);
             }
+            // weights into w; x leaves as weight, with a cap times 1 - tanh^2
+            uint32_t w[MINE / 2];
+            auto weigh = [&](auto all_seen, auto is_small) {
+#pragma unroll
+                for (int u = 0; u < MINE / 2; ++u) {
+                    const F2 l2 = KV ? *reinterpret_cast<const F2 *>(my_lse + 2 * u) : tc::two(lse2, lse2);
+                    F2 z = x[u], dcap = 0;
+                    if (CAP) {
+                        F2 th;
+                        if (decltype(is_small)::value) {
+                            const F2 v = tc::mul2(z, tc::two(c, c));
+                            th = tc::mul2(v, tc::tanh_over_y(tc::mul2(v, v), tanh_c));
+                        } else {
+                            float a, b;  // tanh(y) = 1 - 2 / (1 + e^2y)
+                            tc::split(z, a, b);
+                            a = fmaf(-2.f, tc::rcp(1.f + tc::ex2(a * (2.f * LOG2E * c))), 1.f);
+                            b = fmaf(-2.f, tc::rcp(1.f + tc::ex2(b * (2.f * LOG2E * c))), 1.f);
+                            th = tc::two(a, b);
+                        }
+                        dcap = tc::ffma2(tc::mul2(th, tc::two(-1.f, -1.f)), th, tc::two(1.f, 1.f));
+                        z = tc::mul2(th, tc::two(top_of, top_of));
+                    }
+                    if (BIAS) {
+                        const F2 far = tc::two(-slope * fabsf(away + 2.f * u), -slope * fabsf(away + (2.f * u + 1.f)));
+                        z = CAP ? tc::add2(z, far) : tc::ffma2(z, tc::two(c, c), far);
+                    }
+                    z = CAP || BIAS ? tc::add2(z, l2) : tc::ffma2(z, tc::two(c, c), l2);
+                    float e0, e1;
+                    tc::split(z, e0, e1);
+                    e0 = tc::ex2(e0), e1 = tc::ex2(e1);
+                    if (!decltype(all_seen)::value) {
+                        e0 = seen & 1u << 2 * u ? e0 : 0.f;
+                        e1 = seen & 2u << 2 * u ? e1 : 0.f;
+                    }
+                    x[u] = tc::two(e0, e1);
+                    if (KV) w[u] = tc::pack<E>(e0, e1);
+                    if (CAP) {
+                        x[u] = tc::mul2(x[u], dcap);
+                        if (!decltype(all_seen)::value) {  // (the slope of a hidden score may be NaN)
+                            tc::split(x[u], e0, e1);
+                            x[u] = tc::two(seen & 1u << 2 * u ? e0 : 0.f, seen & 2u << 2 * u ? e1 : 0.f);
+                        }
+                    }
+                }
+            };
+            if (open && small) weigh(std::true_type(), std::true_type());
+            else if (small) weigh(std::false_type(), std::true_type());
+            else weigh(std::false_type(), std::false_type());
             if (KV) {
-                tc::tmem_st32(mine + S_AT + 64 * half, w);
+                tc::tmem_st16(mine + S_AT + MINE * group, w);
                 tc::wait_st();
                 tc::fence_before();
                 __syncwarp();
@@ -358,21 +404,22 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                 ok = tc::warp_wait(&dp_full, j & 1);
                 if (!ok) break;
                 tc::fence_after();
-                tc::tmem_ld32(reinterpret_cast<uint32_t *>(y), mine + DP_AT + 64 * half);
-                tc::tmem_ld32(reinterpret_cast<uint32_t *>(y) + 32, mine + DP_AT + 64 * half + 32);
+                tc::tmem_ld32(reinterpret_cast<uint32_t *>(y), mine + DP_AT + MINE * group);
                 tc::wait_ld();
             }
 #pragma unroll
-            for (int u = 0; u < 64; u += 2) {
-                float2 d = make_float2(delta, delta);
-                if (KV) d = *reinterpret_cast<const float2 *>(my_delta + u);
-                float g0 = x[u] * (y[u] - d.x), g1 = x[u + 1] * (y[u + 1] - d.y);
-                // hidden: zero whatever dP holds
-                g0 = seen[u / 32] & 1u << u % 32 ? g0 : 0.f;
-                g1 = seen[u / 32] & 2u << u % 32 ? g1 : 0.f;
-                w[u / 2] = tc::pack<E>(g0, g1);
+            for (int u = 0; u < MINE / 2; ++u) {
+                const F2 d = KV ? *reinterpret_cast<const F2 *>(my_delta + 2 * u) : tc::two(delta, delta);
+                float g0, g1;
+                tc::split(tc::mul2(x[u], tc::add2(y[u], d)), g0, g1);
+                w[u] = tc::pack<E>(g0, g1);
             }
-            tc::tmem_st32(mine + (KV ? DP_AT + 64 * half : DS_AT + 64 * (j & 1) + 32 * half), w);
+            if (!open) {
+                // hidden: zero whatever dP holds
+#pragma unroll
+                for (int u = 0; u < MINE / 2; ++u) w[u] &= (seen & 1u << 2 * u ? 0xffffu : 0u) | (seen & 2u << 2 * u ? 0xffff0000u : 0u);
+            }
+            tc::tmem_st16(mine + (KV ? DP_AT + MINE * group : DS_AT + 64 * (j & 1) + MINE / 2 * group), w);
             tc::wait_st();
             tc::fence_before();
             __syncwarp();
@@ -381,32 +428,33 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
         if (ok) ok = tc::warp_wait(&acc_full, 0);
         if (ok) {
             tc::fence_after();
-            // dQ: half of the columns in each group of warps; dK, dV: an array in each
-            constexpr int COLUMNS = KV ? DP : DP / 2;
-            const HeadArray &to = KV ? (half ? p.dk : p.dv) : p.dq;
-            const uint32_t from_column = KV ? (half ? DK_AT : DV_AT) : DQ_AT + half * COLUMNS;
-            const int first = KV ? 0 : half * COLUMNS;
-            const float by = KV && !half ? 1.f : p.scale;
+            // dQ: the columns shared out over the groups of warps; dK, dV: an array in two groups each
+            constexpr int COLUMNS = KV ? DP / 2 : DP / 4 < 32 ? 32 : DP / 4;
+            const HeadArray &to = KV ? (group < 2 ? p.dv : p.dk) : p.dq;
+            const int first = COLUMNS * (KV ? group & 1 : group);
+            const uint32_t from_column = (KV ? (group < 2 ? DV_AT : DK_AT) : DQ_AT) + first;
+            const float by = KV && group < 2 ? 1.f : p.scale;
             float zero = 0.f;  // NaN as soon as a result is not finite
-            // the block's own tiles are done with
-            unsigned char *const stage = smem + (KV ? half * TILE_BYTES + (warp & 3) * 32 * DP * 2 : warp * 32 * DP);
+            if (first < DP) {
+                unsigned char *const stage = smem + warp * 32 * COLUMNS * 2;  // the block's own tiles are done with
 #pragma unroll
-            for (int b = 0; b < COLUMNS / 32; ++b) {
-                float o[32];
-                if (count > 0) {
-                    tc::tmem_ld32(reinterpret_cast<uint32_t *>(o), mine + from_column + 32 * b);
-                    tc::wait_ld();
-                }
+                for (int b = 0; b < COLUMNS / 32; ++b) {
+                    float o[32];
+                    if (count > 0) {
+                        tc::tmem_ld32(reinterpret_cast<uint32_t *>(o), mine + from_column + 32 * b);
+                        tc::wait_ld();
+                    }
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    o[i] = count > 0 ? o[i] * by : 0.f;
-                    zero = fmaf(o[i], 0.f, zero);
+                    for (int i = 0; i < 32; ++i) {
+                        o[i] = count > 0 ? o[i] * by : 0.f;
+                        zero = fmaf(o[i], 0.f, zero);
+                    }
+                    tc::stage_32<E, COLUMNS>(stage, 32 * b, o);
                 }
-                tc::stage_32<E, COLUMNS>(stage, 32 * b, o);
+                const int row0 = (warp & 3) * 32;
+                tc::store_staged<E, COLUMNS>(stage, static_cast<E *>(to.data) + ((int64_t)(KV ? s.k0 : s.q0) + r0 + row0) * to.row + head * to.head + first,
+                                             to.row, n_rows - row0, p.head_dim - first);
             }
-            const int row0 = (warp & 3) * 32;
-            tc::store_staged<E, COLUMNS>(stage, static_cast<E *>(to.data) + ((int64_t)(KV ? s.k0 : s.q0) + r0 + row0) * to.row + head * to.head + first, to.row,
-                                         n_rows - row0, p.head_dim - first);
             const unsigned rows = __ballot_sync(0xffffffffu, zero != 0.f && row < n_rows);
             if (lane == 0 && rows) atomicOr(&bad[warp & 3], rows);
         }
@@ -421,7 +469,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                 if (turn % ROW_WARPS == (unsigned)warp) {
                     const int r = 32 * q + __ffs(left) - 1;
                     if (KV) strict::dkv_row<E>(p, s, kv, r0 + r);
-                    else strict::dq_row<E>(p, s, head, r0 + r, row_lse[r], row_delta[0][r] + row_delta[1][r]);
+                    else strict::dq_row<E>(p, s, head, r0 + r, row_lse[r], row_delta[r]);
                 }
 }
 
