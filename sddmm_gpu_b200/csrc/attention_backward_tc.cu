@@ -103,38 +103,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
     if (threadIdx.x < 4) bad[threadIdx.x] = 0;
     if (warp == MMA_WARP) tc::tmem_alloc(&tmem_holder, TMEM_COLUMNS);
     const int group = warp >> 2, row = (warp & 3) * 32 + lane;  // of warps 0-15: columns MINE * group .. of that row
-    if (!KV && warp < ROW_WARPS) {
-        // delta: 16 bytes of O and dO in each lane, DP / 8 lanes a row, all rows of the warp asked for at once
-        constexpr int LANES = DP / 8, AT_ONCE = 32 / LANES, TURNS = T / ROW_WARPS / AT_ONCE;
-        uint4 o[TURNS], d_o[TURNS];
-        const int c = lane % LANES * 8;
-#pragma unroll
-        for (int k = 0; k < TURNS; ++k) {
-            const int r = warp * (T / ROW_WARPS) + k * AT_ONCE + lane / LANES;
-            const int64_t at = (int64_t)s.q0 + r0 + r;
-            o[k] = d_o[k] = make_uint4(0, 0, 0, 0);
-            if (r < n_rows && c < p.head_dim) {
-                o[k] = *reinterpret_cast<const uint4 *>(static_cast<const E *>(p.o.data) + at * p.o.row + head * p.o.head + c);
-                d_o[k] = *reinterpret_cast<const uint4 *>(static_cast<const E *>(p.d_o.data) + at * p.d_o.row + head * p.d_o.head + c);
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < TURNS; ++k) {
-            const int r = warp * (T / ROW_WARPS) + k * AT_ONCE + lane / LANES;
-            const E *a = reinterpret_cast<const E *>(&o[k]), *b = reinterpret_cast<const E *>(&d_o[k]);
-            float d = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) d = fmaf(to_f(a[e]), to_f(b[e]), d);
-#pragma unroll
-            for (int x = LANES / 2; x >= 1; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
-            if (lane % LANES == 0) {
-                const int64_t at = (int64_t)head * p.q_rows + s.q0 + r0 + r;
-                row_delta[r] = d;
-                row_lse[r] = r < n_rows ? __ldg(p.lse + at) : -INFINITY;
-                if (r < n_rows) p.delta[at] = d;
-            }
-        }
-    }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -170,11 +138,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                 if (cut) {
                     ok = tc::warp_wait(&tail, tails++ & 1);
                     if (!ok) break;
-                    const int first = there - t0;
-                    for (int i = lane; i < (T - first) * BOXES * 8; i += 32) {
-                        const int b = i / ((T - first) * 8), r = first + i / 8 % (T - first);
-                        *reinterpret_cast<uint4 *>(smem + (2 + slot) * TILE_BYTES + b * BOX_BYTES + r * 128 + i % 8 * 16) = make_uint4(0, 0, 0, 0);
-                    }
+                    tc::zero_rows<T, BOXES>(smem + (2 + slot) * TILE_BYTES, there - t0);
                     tc::fence_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&full[slot]);
@@ -278,6 +242,41 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 " ROW_REGISTERS ";");
+        if (!KV) {
+            // delta: 16 bytes of O and dO in each lane, DP / 8 lanes a row, all rows of the warp asked for at once
+            constexpr int LANES = DP / 8, AT_ONCE = 32 / LANES, TURNS = T / ROW_WARPS / AT_ONCE;
+            uint4 o[TURNS], d_o[TURNS];
+            float l[TURNS];
+            const int c = lane % LANES * 8;
+#pragma unroll
+            for (int k = 0; k < TURNS; ++k) {
+                const int r = warp * (T / ROW_WARPS) + k * AT_ONCE + lane / LANES;
+                const int64_t at = (int64_t)s.q0 + r0 + r;
+                o[k] = d_o[k] = make_uint4(0, 0, 0, 0);
+                l[k] = r < n_rows ? __ldg(p.lse + (int64_t)head * p.q_rows + at) : -INFINITY;
+                if (r < n_rows && c < p.head_dim) {
+                    o[k] = *reinterpret_cast<const uint4 *>(static_cast<const E *>(p.o.data) + at * p.o.row + head * p.o.head + c);
+                    d_o[k] = *reinterpret_cast<const uint4 *>(static_cast<const E *>(p.d_o.data) + at * p.d_o.row + head * p.d_o.head + c);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < TURNS; ++k) {
+                const int r = warp * (T / ROW_WARPS) + k * AT_ONCE + lane / LANES;
+                const E *a = reinterpret_cast<const E *>(&o[k]), *b = reinterpret_cast<const E *>(&d_o[k]);
+                float d = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d = fmaf(to_f(a[e]), to_f(b[e]), d);
+#pragma unroll
+                for (int x = LANES / 2; x >= 1; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
+                if (lane % LANES == 0) {
+                    const int64_t at = (int64_t)head * p.q_rows + s.q0 + r0 + r;
+                    row_delta[r] = d;
+                    row_lse[r] = l[k];
+                    if (r < n_rows) p.delta[at] = d;
+                }
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(ROW_WARPS * 32) : "memory");  // (all row warps come here, and nothing before can keep one)
+        }
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const float c = CAP ? p.scale / p.cap : p.scale * LOG2E, top_of = p.cap * LOG2E;
         const tc::TanhCoefficients tanh_c = tc::tanh_coefficients(1.f);

@@ -151,11 +151,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                 if (cut) {  // the last tile of a sequence, at most once
                     ok = tc::warp_wait(&tail, 0);
                     if (!ok) break;
-                    const int first = s.nk - j0;
-                    for (int i = lane; i < (KT - first) * BOXES * 8; i += 32) {
-                        const int b = i / ((KT - first) * 8), r = first + i / 8 % (KT - first);
-                        *reinterpret_cast<uint4 *>(smem + slot + b * BOX + r * 128 + i % 8 * 16) = make_uint4(0, 0, 0, 0);
-                    }
+                    tc::zero_rows<KT, BOXES>(smem + slot, s.nk - j0);
                     tc::fence_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&full[v][stage]);

@@ -128,6 +128,16 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, i
         : "memory");
 }
 
+// Rows [first, ROWS) of a tile set to zero by a warp (whole rows, so the swizzle does not matter).
+template <int ROWS, int BOXES>
+__device__ __forceinline__ void zero_rows(unsigned char *tile, int first)
+{
+    const int lane = threadIdx.x & 31;
+    for (int r = first + lane / 8; r < ROWS; r += 4)
+#pragma unroll
+        for (int b = 0; b < BOXES; ++b) *reinterpret_cast<uint4 *>(tile + b * ROWS * 128 + r * 128 + lane % 8 * 16) = make_uint4(0, 0, 0, 0);
+}
+
 // Bounded wait of a thread.  try_wait suspends the thread by itself, so there is no sleep between polls; the limit is wall-clock time, with
 // a count behind it.
 static __device__ __forceinline__ bool wait_long(uint64_t *bar, unsigned parity)
