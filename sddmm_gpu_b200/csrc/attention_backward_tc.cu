@@ -48,20 +48,21 @@ struct alignas(64) Maps {
 
 template <int DP, bool KV> struct Shape {
     static constexpr int BOXES = DP / 64, TILE_BYTES = T * DP * 2, BOX_BYTES = T * 128;
-    static constexpr int SLOTS = DP == 64 ? 8 : KV ? 4 : 5;                        // of one streamed tile
-    static constexpr int STATS = KV ? ROW_WARPS * 2 * MINE * 4 : 0;                // lse and delta of a warp's columns
-    static constexpr int SMEM = (2 + SLOTS) * TILE_BYTES + STATS;
+    // The streamed tiles: K or Q is used by S and again, an iteration later, by the last product; V or dO is done with earlier in
+    // the dQ kernel.  With one ring of five for both, V waited for the slot of a K (3,270 clocks a tile of dQ instead of 2,600).
+    static constexpr int SLOTS0 = DP == 64 ? 4 : 3, SLOTS1 = DP == 64 ? 4 : 2;
+    static constexpr int SMEM = (2 + SLOTS0 + SLOTS1) * TILE_BYTES;
 };
 
 template <class E, int DP, bool CAP, bool BIAS, bool KV>
 __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const AttentionParams p, const __grid_constant__ Maps maps)
 {
     using Sh = Shape<DP, KV>;
-    constexpr int BOXES = Sh::BOXES, TILE_BYTES = Sh::TILE_BYTES, BOX_BYTES = Sh::BOX_BYTES, SLOTS = Sh::SLOTS;
+    constexpr int BOXES = Sh::BOXES, TILE_BYTES = Sh::TILE_BYTES, BOX_BYTES = Sh::BOX_BYTES, SLOTS0 = Sh::SLOTS0, SLOTS1 = Sh::SLOTS1;
     constexpr bool BF16 = !std::is_same<E, __half>::value;
-    extern __shared__ __align__(1024) unsigned char smem[];  // the block's two tiles, the ring, lse and delta
+    extern __shared__ __align__(1024) unsigned char smem[];  // the block's two tiles, the two rings
     // dQ: s_full = scores and dP there, p_ready = they have been read
-    __shared__ uint64_t own_full, full[SLOTS], empty[SLOTS], s_full, dp_full, p_ready, ds_ready, acc_full, tail;
+    __shared__ uint64_t own_full, full[SLOTS0 + SLOTS1], empty[SLOTS0 + SLOTS1], s_full, dp_full, p_ready, ds_ready, acc_full, tail;
     __shared__ uint32_t tmem_holder, bad[4];
     __shared__ float row_lse[T], row_delta[T];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -86,13 +87,16 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
         keys = key_tiles<T>(reach);
         count = keys.n;
     }
+    // streamed tile n: even ones K or Q, odd ones V or dO; its slot, and the how manieth of that slot it is
+    auto slot_of = [](int n) { return n & 1 ? SLOTS0 + n / 2 % SLOTS1 : n / 2 % SLOTS0; };
+    auto turn_of = [](int n) { return n & 1 ? n / 2 / SLOTS1 : n / 2 / SLOTS0; };
     auto tile_at = [&](int j) { return (KV ? from + j % per_head : keys.tile(j)) * T; };
     auto head_at = [&](int j) { return KV ? kv * p.group + j / per_head : head; };
 
     if (threadIdx.x == 0) {
         mbar_init(&own_full, 1);
         mbar_init(&tail, 1);
-        for (int i = 0; i < SLOTS; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+        for (int i = 0; i < SLOTS0 + SLOTS1; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
         mbar_init(&s_full, 1);
         mbar_init(&dp_full, 1);
         mbar_init(&p_ready, ROW_WARPS);
@@ -123,8 +127,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             int issued = 0;
             unsigned tails = 0;
             for (int n = 0; n < 2 * count && ok; ++n) {
-                const int slot = n % SLOTS, t0 = tile_at(n / 2), of = KV ? head_at(n / 2) : kv;
-                if (n >= SLOTS) ok = tc::warp_wait(&empty[slot], (n / SLOTS - 1) & 1);
+                const int slot = slot_of(n), turn = turn_of(n), t0 = tile_at(n / 2), of = KV ? head_at(n / 2) : kv;
+                if (turn > 0) ok = tc::warp_wait(&empty[slot], (turn - 1) & 1);
                 if (!ok) break;
                 // rows behind the sequence's end, where they meet zero weights in a product: zeros (0 x NaN is NaN)
                 const bool second = n & 1, cut = (KV || !second) && t0 + T > there;
@@ -146,7 +150,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             }
             // copies of a role that gave up still land in this block's shared memory: wait for them
             if (!ok)
-                for (int n = issued > SLOTS ? issued - SLOTS : 0; n < issued; ++n) (void)tc::wait(&full[n % SLOTS], (n / SLOTS) & 1);
+                for (int n = max(0, issued - 2 * max(SLOTS0, SLOTS1)); n < issued; ++n) (void)tc::wait(&full[slot_of(n)], turn_of(n) & 1);
         } else if (warp == MMA_WARP) {
             constexpr uint32_t ID_S = tc::instr_desc(BF16, T, T, false, false), ID_ACC = tc::instr_desc(BF16, T, DP, false, true);
             const uint64_t own_desc = tc::smem_desc(base, 16), rows_desc = tc::smem_desc(ring, 16), tile_desc = tc::smem_desc(ring, BOX_BYTES);
@@ -175,9 +179,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             auto done = [&](uint64_t *bar) {
                 if (tc::elected()) tc::commit(bar);
             };
-            auto slot_of = [](int n) { return n % SLOTS; };
             auto wait_tile = [&](int n) {
-                ok = ok && tc::warp_wait(&full[n % SLOTS], (n / SLOTS) & 1);
+                ok = ok && tc::warp_wait(&full[slot_of(n)], turn_of(n) & 1);
                 tc::fence_after();
                 return ok;
             };
@@ -219,11 +222,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                     }
                 } else {
                     if (more) {
-                        if (!wait_tile(n + 2) || !wait_tile(n + 3)) break;
+                        if (!wait_tile(n + 2)) break;
                         ok = tc::warp_wait(&p_ready, j & 1);
                         if (!ok) break;
                         tc::fence_after();
                         rows_by_rows(S_AT, 0, slot_of(n + 2));
+                        if (!wait_tile(n + 3)) break;
                         rows_by_rows(DP_AT, 1, slot_of(n + 3));
                         done(&s_full);
                         done(&empty[slot_of(n + 3)]);
@@ -299,24 +303,25 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             delta = -row_delta[row];
             lse2 = row_lse[row] == -INFINITY ? -INFINITY : -row_lse[row] * LOG2E;  // a row that has seen nothing: weights of zero
         }
-        float *const my_lse = reinterpret_cast<float *>(smem + (2 + SLOTS) * TILE_BYTES) + warp * 2 * MINE, *const my_delta = my_lse + MINE;
-        float next_lse = 0.f, next_delta = 0.f;
-        auto fetch = [&](int j) {  // lse and delta, negative, of this warp's columns of tile j, one a lane
-            const int i = tile_at(j) + MINE * group + lane;
-            const int64_t at = (int64_t)head_at(j) * p.q_rows + s.q0 + i;
+        // dK, dV: lse and delta, negative, of this warp's columns, one a lane; the next tile's are fetched a tile ahead
+        float my_lse = 0.f, my_delta = 0.f, next_lse = 0.f, next_delta = 0.f;
+        int next_tile = from * T, next_head = kv * p.group;
+        auto fetch = [&]() {
+            const int i = next_tile + MINE * group + lane;
+            const int64_t at = (int64_t)next_head * p.q_rows + s.q0 + i;
             const float l = i < s.nq ? __ldg(p.lse + at) : -INFINITY;
             next_lse = l == -INFINITY ? -INFINITY : -l * LOG2E;
             next_delta = i < s.nq ? -__ldg(p.delta + at) : 0.f;
         };
-        if (KV && count > 0) fetch(0);
+        if (KV && count > 0) fetch();
         for (int j = 0; j < count && ok; ++j) {
-            const int t0 = tile_at(j), c0 = t0 + MINE * group;
+            const int t0 = KV ? next_tile : tile_at(j), c0 = t0 + MINE * group;
             if (KV) {
-                __syncwarp();
-                my_lse[lane] = next_lse, my_delta[lane] = next_delta;
-                __syncwarp();
-                if (BIAS) slope = __ldg(p.slopes + head_at(j)) * LOG2E;
-                if (j + 1 < count) fetch(j + 1);
+                my_lse = next_lse, my_delta = next_delta;
+                if (BIAS) slope = __ldg(p.slopes + next_head) * LOG2E;
+                next_tile += T;
+                if (next_tile == (from + per_head) * T) next_tile = from * T, ++next_head;
+                if (j + 1 < count) fetch();
             }
             bool open;
             if (KV) open = n_rows == T && t0 + T <= s.nq && tile_is_open<T>(p.window, s, reach_of(p.window, s, t0, t0 + T), r0);
@@ -351,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             auto weigh = [&](auto all_seen, auto is_small) {
 #pragma unroll
                 for (int u = 0; u < MINE / 2; ++u) {
-                    const F2 l2 = KV ? *reinterpret_cast<const F2 *>(my_lse + 2 * u) : tc::two(lse2, lse2);
+                    const F2 l2 = KV ? tc::two(__shfl_sync(0xffffffffu, my_lse, 2 * u), __shfl_sync(0xffffffffu, my_lse, 2 * u + 1)) : tc::two(lse2, lse2);
                     F2 z = x[u], dcap = 0;
                     if (CAP) {
                         F2 th;
@@ -408,7 +413,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             }
 #pragma unroll
             for (int u = 0; u < MINE / 2; ++u) {
-                const F2 d = KV ? *reinterpret_cast<const F2 *>(my_delta + 2 * u) : tc::two(delta, delta);
+                const F2 d = KV ? tc::two(__shfl_sync(0xffffffffu, my_delta, 2 * u), __shfl_sync(0xffffffffu, my_delta, 2 * u + 1)) : tc::two(delta, delta);
                 float g0, g1;
                 tc::split(tc::mul2(x[u], tc::add2(y[u], d)), g0, g1);
                 w[u] = tc::pack<E>(g0, g1);
