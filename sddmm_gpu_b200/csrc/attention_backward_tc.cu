@@ -13,7 +13,8 @@
 //   warps 0-15  a row of the block in every thread, a quarter of the tile's columns in each group of four warps: scores from tensor
 //               memory, weights and score gradients back to it;
 //   warp 16     one thread issues the products; the second operand of the last ones is the streamed tile as it lies, MN-major;
-//   warp 17     one thread brings the tiles by tile copies.
+//   warp 17     one thread brings the tiles by tile copies;
+//   warp 18     (dK, dV) brings lse and delta of the tile's queries, negative, two tiles ahead.
 //
 // dQ: score gradients have a place of their own in tensor memory (two, in turn), so the next tile's scores are computed as soon as the
 // last ones have been read.  dK, dV: tensor memory is full (S, dP, dV, dK); P and dS take the place of S and dP, and the
@@ -33,7 +34,7 @@ using tc::mbar_init;
 using tc::F2;
 
 constexpr int T = 128;
-constexpr int ROW_WARPS = 16, MMA_WARP = 16, LOAD_WARP = 17, THREADS = 640;
+constexpr int ROW_WARPS = 16, MMA_WARP = 16, LOAD_WARP = 17, STATS_WARP = 18, THREADS = 640;
 constexpr int MINE = 32;  // columns of a thread
 constexpr uint32_t TMEM_COLUMNS = 512, S_AT = 0, DP_AT = 128;
 // dQ: accumulator, then two places of 64 columns for score gradients.  dK, dV: the two accumulators.
@@ -54,6 +55,8 @@ template <int DP, bool KV> struct Shape {
     static constexpr int SMEM = (2 + SLOTS0 + SLOTS1) * TILE_BYTES;
 };
 
+__device__ __forceinline__ F2 pick(const ulonglong2 &v, int second) { return second ? v.y : v.x; }
+
 template <class E, int DP, bool CAP, bool BIAS, bool KV>
 __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const AttentionParams p, const __grid_constant__ Maps maps)
 {
@@ -61,10 +64,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
     constexpr int BOXES = Sh::BOXES, TILE_BYTES = Sh::TILE_BYTES, BOX_BYTES = Sh::BOX_BYTES, SLOTS0 = Sh::SLOTS0, SLOTS1 = Sh::SLOTS1;
     constexpr bool BF16 = !std::is_same<E, __half>::value;
     extern __shared__ __align__(1024) unsigned char smem[];  // the block's two tiles, the two rings
-    // dQ: s_full = scores and dP there, p_ready = they have been read
-    __shared__ uint64_t own_full, full[SLOTS0 + SLOTS1], empty[SLOTS0 + SLOTS1], s_full, dp_full, p_ready, ds_ready, acc_full, tail;
+    // dQ: s_full = scores and dP there, p_ready = they have been read.  ds_ready, of even and odd tiles: in the dQ kernel a warp may be done with
+    // the next tile before another is done with this one, and its arrival must not count for this one.
+    __shared__ uint64_t own_full, full[SLOTS0 + SLOTS1], empty[SLOTS0 + SLOTS1], s_full, dp_full, p_ready, ds_ready[2], acc_full, tail, stats_full[2];
     __shared__ uint32_t tmem_holder, bad[4];
-    __shared__ float row_lse[T], row_delta[T];
+    __shared__ __align__(16) float stats[KV ? 4 : 2][T];  // dQ: lse and delta of the rows; else of the columns, of two tiles
+    float *const row_lse = stats[0], *const row_delta = stats[1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int heads = KV ? p.kv_heads : p.q_heads, head = blockIdx.x % heads, kv = KV ? head : head / p.group;
     Sequence s;
@@ -100,8 +105,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
         mbar_init(&s_full, 1);
         mbar_init(&dp_full, 1);
         mbar_init(&p_ready, ROW_WARPS);
-        mbar_init(&ds_ready, ROW_WARPS);
+        mbar_init(&ds_ready[0], ROW_WARPS);
+        mbar_init(&ds_ready[1], ROW_WARPS);
         mbar_init(&acc_full, 1);
+        mbar_init(&stats_full[0], 1);
+        mbar_init(&stats_full[1], 1);
         mbar_fence_init();
     }
     if (threadIdx.x < 4) bad[threadIdx.x] = 0;
@@ -151,6 +159,24 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             // copies of a role that gave up still land in this block's shared memory: wait for them
             if (!ok)
                 for (int n = max(0, issued - 2 * max(SLOTS0, SLOTS1)); n < issued; ++n) (void)tc::wait(&full[slot_of(n)], turn_of(n) & 1);
+        } else if (KV && warp == STATS_WARP) {
+            int tile = from * T, of = kv * p.group;
+            for (int j = 0; j < count && ok; ++j) {
+                if (j >= 2) ok = tc::warp_wait(&ds_ready[j & 1], (j - 2) >> 1 & 1);  // of tile j - 2: the rows are done with its values
+                if (!ok) break;
+                const int64_t at = (int64_t)of * p.q_rows + s.q0;
+#pragma unroll
+                for (int x = 0; x < T / 32; ++x) {
+                    const int i = tile + 32 * x + lane;
+                    const float l = i < s.nq ? __ldg(p.lse + at + i) : -INFINITY, d = i < s.nq ? __ldg(p.delta + at + i) : 0.f;
+                    stats[(2 * j & 2)][32 * x + lane] = l == -INFINITY ? -INFINITY : -l * LOG2E;  // nothing seen: weights of zero
+                    stats[(2 * j & 2) + 1][32 * x + lane] = -d;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&stats_full[j & 1]);
+                tile += T;
+                if (tile == (from + per_head) * T) tile = from * T, ++of;
+            }
         } else if (warp == MMA_WARP) {
             constexpr uint32_t ID_S = tc::instr_desc(BF16, T, T, false, false), ID_ACC = tc::instr_desc(BF16, T, DP, false, true);
             const uint64_t own_desc = tc::smem_desc(base, 16), rows_desc = tc::smem_desc(ring, 16), tile_desc = tc::smem_desc(ring, BOX_BYTES);
@@ -210,7 +236,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                         rows_by_rows(S_AT, 0, slot_of(n + 2));
                         done(&s_full);
                     }
-                    ok = tc::warp_wait(&ds_ready, j & 1);
+                    ok = tc::warp_wait(&ds_ready[j & 1], j >> 1 & 1);
                     if (!ok) break;
                     tc::fence_after();
                     weights_by_tile(DK_AT, DP_AT, MINE, slot_of(n), j > 0);
@@ -232,7 +258,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                         done(&s_full);
                         done(&empty[slot_of(n + 3)]);
                     }
-                    ok = tc::warp_wait(&ds_ready, j & 1);
+                    ok = tc::warp_wait(&ds_ready[j & 1], j >> 1 & 1);
                     if (!ok) break;
                     tc::fence_after();
                     weights_by_tile(DQ_AT, DS_AT + 64 * (j & 1), MINE / 2, slot_of(n), j > 0);
@@ -283,7 +309,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
         }
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const float c = CAP ? p.scale / p.cap : p.scale * LOG2E, top_of = p.cap * LOG2E;
-        const tc::TanhCoefficients tanh_c = tc::tanh_coefficients(1.f);
+        const tc::Tanh tanh_c = tc::tanh_polynomial(c, 1.f);
         float slope = BIAS && !KV ? __ldg(p.slopes + head) * LOG2E : 0.f;
         const int off = s.nk - s.nq;
         // what a row sees: columns [lo, hi] of the other side, and the first `pre`
@@ -303,31 +329,21 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             delta = -row_delta[row];
             lse2 = row_lse[row] == -INFINITY ? -INFINITY : -row_lse[row] * LOG2E;  // a row that has seen nothing: weights of zero
         }
-        // dK, dV: lse and delta, negative, of this warp's columns, one a lane; the next tile's are fetched a tile ahead
-        float my_lse = 0.f, my_delta = 0.f, next_lse = 0.f, next_delta = 0.f;
-        int next_tile = from * T, next_head = kv * p.group;
-        auto fetch = [&]() {
-            const int i = next_tile + MINE * group + lane;
-            const int64_t at = (int64_t)next_head * p.q_rows + s.q0 + i;
-            const float l = i < s.nq ? __ldg(p.lse + at) : -INFINITY;
-            next_lse = l == -INFINITY ? -INFINITY : -l * LOG2E;
-            next_delta = i < s.nq ? -__ldg(p.delta + at) : 0.f;
-        };
-        if (KV && count > 0) fetch();
+        int next_tile = from * T, next_head = kv * p.group;  // dK, dV
         for (int j = 0; j < count && ok; ++j) {
             const int t0 = KV ? next_tile : tile_at(j), c0 = t0 + MINE * group;
+            const float *const my_lse = stats[2 * j & 2] + MINE * group, *const my_delta = stats[(2 * j & 2) + 1] + MINE * group;
             if (KV) {
-                my_lse = next_lse, my_delta = next_delta;
                 if (BIAS) slope = __ldg(p.slopes + next_head) * LOG2E;
                 next_tile += T;
                 if (next_tile == (from + per_head) * T) next_tile = from * T, ++next_head;
-                if (j + 1 < count) fetch();
             }
             bool open;
             if (KV) open = n_rows == T && t0 + T <= s.nq && tile_is_open<T>(p.window, s, reach_of(p.window, s, t0, t0 + T), r0);
             else open = tile_is_open<T>(p.window, s, reach, t0);
             const unsigned seen = open ? ~0u : seen_bits(lo, hi, pre, c0);
-            ok = tc::warp_wait(&s_full, j & 1);
+            if (KV) ok = tc::warp_wait(&stats_full[j & 1], j >> 1 & 1);
+            ok = ok && tc::warp_wait(&s_full, j & 1);
             if (!ok) break;
             tc::fence_after();
             F2 x[MINE / 2], y[MINE / 2];  // two columns each
@@ -349,20 +365,19 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                     tc::split(x[u], a, b);
                     size = tc::max3_abs(size, a, b);
                 }
-                small = __all_sync(0xffffffffu, size * c <= tc::TANH_RANGE);
+                small = __all_sync(0xffffffffu, size <= tanh_c.range);
             }
             // weights into w; x leaves as weight, with a cap times 1 - tanh^2
             uint32_t w[MINE / 2];
             auto weigh = [&](auto all_seen, auto is_small) {
 #pragma unroll
                 for (int u = 0; u < MINE / 2; ++u) {
-                    const F2 l2 = KV ? tc::two(__shfl_sync(0xffffffffu, my_lse, 2 * u), __shfl_sync(0xffffffffu, my_lse, 2 * u + 1)) : tc::two(lse2, lse2);
+                    const F2 l2 = KV ? pick(reinterpret_cast<const ulonglong2 *>(my_lse)[u / 2], u & 1) : tc::two(lse2, lse2);
                     F2 z = x[u], dcap = 0;
                     if (CAP) {
                         F2 th;
                         if (decltype(is_small)::value) {
-                            const F2 v = tc::mul2(z, tc::two(c, c));
-                            th = tc::mul2(v, tc::tanh_over_y(tc::mul2(v, v), tanh_c));
+                            th = tc::tanh2(z, tanh_c);
                         } else {
                             float a, b;  // tanh(y) = 1 - 2 / (1 + e^2y)
                             tc::split(z, a, b);
@@ -370,14 +385,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                             b = fmaf(-2.f, tc::rcp(1.f + tc::ex2(b * (2.f * LOG2E * c))), 1.f);
                             th = tc::two(a, b);
                         }
-                        dcap = tc::ffma2(tc::mul2(th, tc::two(-1.f, -1.f)), th, tc::two(1.f, 1.f));
-                        z = tc::mul2(th, tc::two(top_of, top_of));
+                        dcap = tc::ffma2(tc::mul2(th, th), tc::two(-1.f, -1.f), tc::two(1.f, 1.f));
+                        z = BIAS ? tc::mul2(th, tc::two(top_of, top_of)) : tc::ffma2(th, tc::two(top_of, top_of), l2);
                     }
                     if (BIAS) {
                         const F2 far = tc::two(-slope * fabsf(away + 2.f * u), -slope * fabsf(away + (2.f * u + 1.f)));
                         z = CAP ? tc::add2(z, far) : tc::ffma2(z, tc::two(c, c), far);
                     }
-                    z = CAP || BIAS ? tc::add2(z, l2) : tc::ffma2(z, tc::two(c, c), l2);
+                    if (BIAS) z = tc::add2(z, l2);
+                    else if (!CAP) z = tc::ffma2(z, tc::two(c, c), l2);
                     float e0, e1;
                     tc::split(z, e0, e1);
                     e0 = tc::ex2(e0), e1 = tc::ex2(e1);
@@ -413,7 +429,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             }
 #pragma unroll
             for (int u = 0; u < MINE / 2; ++u) {
-                const F2 d = KV ? tc::two(__shfl_sync(0xffffffffu, my_delta, 2 * u), __shfl_sync(0xffffffffu, my_delta, 2 * u + 1)) : tc::two(delta, delta);
+                const F2 d = KV ? pick(reinterpret_cast<const ulonglong2 *>(my_delta)[u / 2], u & 1) : tc::two(delta, delta);
                 float g0, g1;
                 tc::split(tc::mul2(x[u], tc::add2(y[u], d)), g0, g1);
                 w[u] = tc::pack<E>(g0, g1);
@@ -427,7 +443,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             tc::wait_st();
             tc::fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&ds_ready);
+            if (lane == 0) mbar_arrive(&ds_ready[j & 1]);
         }
         if (ok) ok = tc::warp_wait(&acc_full, 0);
         if (ok) {

@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
         const uint32_t my_scores = mine + t * T + half * COLUMNS, my_weights = mine + Sh::P_AT + t * Sh::P_TILE + half * Sh::P_APART;
         const float slope = BIAS ? __ldg(p.slopes + head) * LOG2E : 0.f;
         const float c = CAP ? p.scale / p.cap : p.scale * LOG2E, top_of = p.cap * LOG2E;
-        const tc::TanhCoefficients tanh_c = tc::tanh_coefficients(top_of);
+        const tc::Tanh tanh_c = tc::tanh_polynomial(c, top_of);
         const int pos = s.nk - s.nq + i;
         const int lo = p.window.left < 0 ? 0 : max(0, pos - p.window.left), hi = p.window.right < 0 ? s.nk - 1 : min(s.nk - 1, pos + p.window.right);
         float most = -INFINITY, sum = 0.f;  // in units of log 2
@@ -280,12 +280,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                     tc::split(x[j], a, b);
                     size = tc::max3_abs(size, a, b);
                 }
-                if (__all_sync(0xffffffffu, size * c <= tc::TANH_RANGE)) {
+                if (__all_sync(0xffffffffu, size <= tanh_c.range)) {
 #pragma unroll
-                    for (int j = 0; j < COLUMNS / 2; ++j) {
-                        const F2 y = tc::mul2(x[j], tc::two(c, c));
-                        x[j] = tc::mul2(y, tc::tanh_over_y(tc::mul2(y, y), tanh_c));
-                    }
+                    for (int j = 0; j < COLUMNS / 2; ++j) x[j] = tc::tanh2(x[j], tanh_c);
                 } else {
                     // cap tanh(y) = cap - 2 cap / (1 + e^2y)
                     const float c2 = 2.f * LOG2E * c;

@@ -221,25 +221,32 @@ __device__ __forceinline__ F2 ex2_poly(F2 x)
     split(r, a, b);
     return mul2(p, two(__uint_as_float((__float_as_uint(a) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(b) << 23) + 0x3f800000u)));
 }
-constexpr float TANH_RANGE = 0.6f;
-// tanh(y) / y from u = y^2, |y| <= 0.6 (Chebyshev interpolation in u; tanh is off by 9e-8), times `by`, whose products with the coefficients are given.
-struct TanhCoefficients {
-    F2 c[5];
+// tanh(c x) = x (a polynomial in x^2), where |c x| <= 0.6: Chebyshev interpolation of tanh(y) / y in y^2, off by 9e-8, its coefficients
+// times by c^(2i + 1).  A c below 2e-4 would take the last of them under the normal numbers: `range` 0, and no x is in it.
+struct Tanh {
+    F2 a[5];
+    float range;  // of |x|
 };
-__device__ __forceinline__ TanhCoefficients tanh_coefficients(float by)
+__device__ __forceinline__ Tanh tanh_polynomial(float c, float by)
 {
     constexpr float C[5] = {0.99999994f, -0.33332324f, 0.133103579f, -0.0521096252f, 0.0154866902f};
-    TanhCoefficients t;
+    Tanh t;
+    float power = c * by;
 #pragma unroll
-    for (int i = 0; i < 5; ++i) t.c[i] = two(C[i] * by, C[i] * by);
+    for (int i = 0; i < 5; ++i) {
+        t.a[i] = two(C[i] * power, C[i] * power);
+        power *= c * c;
+    }
+    t.range = c >= 2e-4f ? 0.6f / c : 0.f;
     return t;
 }
-__device__ __forceinline__ F2 tanh_over_y(F2 u, const TanhCoefficients &t)
+__device__ __forceinline__ F2 tanh2(F2 x, const Tanh &t)
 {
-    F2 p = t.c[4];
+    const F2 u = mul2(x, x);
+    F2 p = t.a[4];
 #pragma unroll
-    for (int i = 3; i >= 0; --i) p = ffma2(p, u, t.c[i]);
-    return p;
+    for (int i = 3; i >= 0; --i) p = ffma2(p, u, t.a[i]);
+    return mul2(p, x);
 }
 // Two values in a word, the first in its lower half.
 template <class T> __device__ __forceinline__ uint32_t pack(float a, float b);

@@ -97,6 +97,23 @@ def test_long_band_with_global_tokens(engine, dtype):
     _check_backward(engine, p).close()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d,q,window,prefix,cap", [(64, [2300], (256, 256), 80, 0.0), (128, [900, 130, 1500], (-1, 0), 0, 0.0),
+                                                   (128, [1, 700, 64], (90, 0), 7, 20.0), (64, [640] * 6, (-1, -1), 0, 0.0)])
+def test_the_same_bits_every_time(engine, dtype, d, q, window, prefix, cap):
+    # warps that run ahead of one another do so differently every time
+    p = Problem(dtype, d, 4, 2, q, window=window, prefix=prefix, cap=cap)
+    plan, O, l = _forward(engine, p)
+    first = [torch.empty_like(t) for t in (p.Q, p.K, p.V)]
+    plan.backward(p.Q, p.K, p.V, O, l, p.dO, *first)
+    O2, l2, again = torch.empty_like(O), torch.empty_like(l), [torch.empty_like(t) for t in first]
+    for _ in range(60):
+        plan.forward(p.Q, p.K, p.V, O2, l2)
+        plan.backward(p.Q, p.K, p.V, O, l, p.dO, *again)
+        assert torch.equal(O, O2) and torch.equal(l, l2) and all(torch.equal(a, b) for a, b in zip(first, again))
+    plan.close()
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 def test_scores_far_apart(engine, dtype):
     # weights that are nearly one-hot, maxima that move along the row
