@@ -15,7 +15,7 @@ struct sddmm_attention_s {
     sddmm_handle_s *h = nullptr;
     AttentionParams p{};
     FewPlan few{};
-    GeneralParts parts{};
+    Parts parts = ONE_PART;
     const char *last_kernel = "none";
 };
 
@@ -134,7 +134,7 @@ int sddmm_attention_plan(sddmm_handle_t h, const sddmm_attention_desc *d, sddmm_
     a->h = h;
     a->p = p;
     a->few = plan_attention_few(p, h->sm_count);
-    a->parts = plan_general_parts(p, h->sm_count);
+    a->parts = p.dtype == SDDMM_F32 ? plan_attention_parts(p, 64, 4, h->sm_count) : plan_attention_parts(p, 128, 1, h->sm_count);
     *out = a;
     return SDDMM_OK;
 }
@@ -211,9 +211,12 @@ int sddmm_attention_backward(sddmm_attention_t a, const sddmm_head_array *Q, con
     if (!(flags & SDDMM_FLAG_ASYNC) && capturing(h->stream)) return bad(h, "a captured call must be asynchronous");
     if (p.n_seqs == 0 || (p.max_q == 0 && p.max_k == 0)) return SDDMM_OK;
     bool taken = false;
-    const cudaError_t e = launch_attention_backward_tc(p, &taken, h->stream);
-    if (taken) return finish(a, e, "attention_backward_tc", 2, flags);
-    return finish(a, launch_attention_backward_general(p, a->parts, h->stream), "attention_backward_general", 2 + (a->parts.n_q > 1) + (a->parts.n_kv > 1), flags);
+    const int launches = 2 + (a->parts.n_q > 1) + (a->parts.n_kv > 1);
+    const cudaError_t e = launch_attention_backward_tc(p, a->parts, &taken, h->stream);
+    if (taken) return finish(a, e, "attention_backward_tc", launches, flags);
+    // (16-bit types come to the general kernel for their strides or alignment alone)
+    if (p.dtype == SDDMM_F32) return finish(a, launch_attention_backward_general(p, a->parts, h->stream), "attention_backward_general", launches, flags);
+    return finish(a, launch_attention_backward_general(p, ONE_PART, h->stream), "attention_backward_general", 2, flags);
 }
 
 const char *sddmm_attention_last_kernel(sddmm_attention_t a) { return a ? a->last_kernel : "none"; }

@@ -110,15 +110,37 @@ FewPlan plan_attention_few(const AttentionParams &p, int sm_count);
 cudaError_t launch_attention_few_tc(const AttentionParams &p, const FewPlan &f, void *workspace, bool *taken, cudaStream_t s);
 // On the tensor cores; *taken false, and nothing launched, where the call's type, strides or alignment do not allow it.
 cudaError_t launch_attention_forward_tc(const AttentionParams &p, bool *taken, cudaStream_t s);
-cudaError_t launch_attention_backward_tc(const AttentionParams &p, bool *taken, cudaStream_t s);
 cudaError_t launch_attention_forward_general(const AttentionParams &p, cudaStream_t s);
-// How the general backward kernels cut the tiles that a block goes through (1: not), for dQ and for dK and dV; bytes of the parts' sums
-// (16-byte aligned, p.part_o).
-struct GeneralParts {
+// Where the blocks of a backward kernel alone would leave multiprocessors idle, the tiles that a block goes through are cut into parts, a
+// block each, which leave their sums in the workspace (parts x rows x heads x head_dim, dK and dV behind one another) for
+// launch_attention_sum_parts().  Most parts of a block, tiles of a part, bytes of the sums (16-byte aligned, p.part_o).
+struct Parts {
     int n_q, tiles_q, n_kv, tiles_kv;
     int64_t bytes;
 };
-GeneralParts plan_general_parts(const AttentionParams &p, int sm_count);
-cudaError_t launch_attention_backward_general(const AttentionParams &p, const GeneralParts &parts, cudaStream_t s);
+constexpr Parts ONE_PART{1, 1 << 30, 1, 1 << 30, 0};
+Parts plan_attention_parts(const AttentionParams &p, int tile, int per_sm, int sm_count);
+// tile: rows of a block; 64 for fp32, 128 for 16-bit types
+cudaError_t launch_attention_sum_parts(const AttentionParams &p, bool kv, int tile, cudaStream_t s);
+struct Part {
+    int first, end;  // tiles
+    bool alone;      // no other part: the block stores its results itself
+};
+__device__ __forceinline__ Part part_of(const AttentionParams &p, int tiles, int part)
+{
+    const int each = p.chunk_tiles, n = max(1, (tiles + each - 1) / each);
+    return Part{part * each, part < n ? min(tiles, (part + 1) * each) : -1, n == 1};  // (end -1: there is no such part)
+}
+// The tiles of T queries that see keys [j0, j0 + m): `per_head` from `from` on, for every head of the group.
+template <int T>
+__device__ __forceinline__ void query_tiles(const AttentionParams &p, const Sequence &s, int j0, int m, int &from, int &per_head)
+{
+    int to;
+    queries_of(p.window, s, j0, j0 + m, from, to);
+    from /= T;
+    per_head = to > from * T ? (to + T - 1) / T - from : 0;
+}
+cudaError_t launch_attention_backward_general(const AttentionParams &p, const Parts &parts, cudaStream_t s);
+cudaError_t launch_attention_backward_tc(const AttentionParams &p, const Parts &parts, bool *taken, cudaStream_t s);
 
 }  // namespace sddmm

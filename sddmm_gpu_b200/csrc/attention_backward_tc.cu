@@ -71,32 +71,33 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
     __shared__ __align__(16) float stats[KV ? 4 : 2][T];  // dQ: lse and delta of the rows; else of the columns, of two tiles
     float *const row_lse = stats[0], *const row_delta = stats[1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int heads = KV ? p.kv_heads : p.q_heads, head = blockIdx.x % heads, kv = KV ? head : head / p.group;
+    const unsigned blocks = gridDim.x / p.n_splits, block_of = blockIdx.x / p.n_splits, part = blockIdx.x % p.n_splits;
+    const int heads = KV ? p.kv_heads : p.q_heads, head = block_of % heads, kv = KV ? head : head / p.group;
     Sequence s;
     int seq, block;
     // causal sequences: the last queries see the most keys, the first keys are seen by the most queries
-    if (!find_block<T>(p, KV ? blockIdx.x / heads : (gridDim.x - 1 - blockIdx.x) / heads, KV, s, seq, block)) return;
+    if (!find_block<T>(p, KV ? block_of / heads : (blocks - 1 - block_of) / heads, KV, s, seq, block)) return;
     const int r0 = block * T, n_rows = min(T, (KV ? s.nk : s.nq) - r0);
     // the tiles of the other side
     Reach reach = {};
     KeyTiles keys = {};
-    int from = 0, per_head = 0, count;
+    int from = 0, per_head = 0, tiles;
     if (KV) {
-        int to;
-        queries_of(p.window, s, r0, r0 + n_rows, from, to);
-        from /= T;
-        per_head = to > from * T ? (to + T - 1) / T - from : 0;
-        count = per_head * p.group;
+        query_tiles<T>(p, s, r0, n_rows, from, per_head);
+        tiles = per_head * p.group;
     } else {
         reach = reach_of(p.window, s, r0, r0 + n_rows);
         keys = key_tiles<T>(reach);
-        count = keys.n;
+        tiles = keys.n;
     }
+    const Part mine_of = part_of(p, tiles, part);
+    if (mine_of.end < 0) return;
+    const int begin = mine_of.first, count = mine_of.end - begin;
     // streamed tile n: even ones K or Q, odd ones V or dO; its slot, and the how manieth of that slot it is
     auto slot_of = [](int n) { return n & 1 ? SLOTS0 + n / 2 % SLOTS1 : n / 2 % SLOTS0; };
     auto turn_of = [](int n) { return n & 1 ? n / 2 / SLOTS1 : n / 2 / SLOTS0; };
-    auto tile_at = [&](int j) { return (KV ? from + j % per_head : keys.tile(j)) * T; };
-    auto head_at = [&](int j) { return KV ? kv * p.group + j / per_head : head; };
+    auto tile_at = [&](int j) { return (KV ? from + (begin + j) % per_head : keys.tile(begin + j)) * T; };
+    auto head_at = [&](int j) { return KV ? kv * p.group + (begin + j) / per_head : head; };
 
     if (threadIdx.x == 0) {
         mbar_init(&own_full, 1);
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             if (!ok)
                 for (int n = max(0, issued - 2 * max(SLOTS0, SLOTS1)); n < issued; ++n) (void)tc::wait(&full[slot_of(n)], turn_of(n) & 1);
         } else if (KV && warp == STATS_WARP) {
-            int tile = from * T, of = kv * p.group;
+            int tile = count > 0 ? tile_at(0) : 0, of = count > 0 ? head_at(0) : 0;
             for (int j = 0; j < count && ok; ++j) {
                 if (j >= 2) ok = tc::warp_wait(&ds_ready[j & 1], (j - 2) >> 1 & 1);  // of tile j - 2: the rows are done with its values
                 if (!ok) break;
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                     const int64_t at = (int64_t)head * p.q_rows + s.q0 + r0 + r;
                     row_delta[r] = d;
                     row_lse[r] = l[k];
-                    if (r < n_rows) p.delta[at] = d;
+                    if (r < n_rows && part == 0) p.delta[at] = d;
                 }
             }
             asm volatile("bar.sync 1, %0;" ::"n"(ROW_WARPS * 32) : "memory");  // (all row warps come here, and nothing before can keep one)
@@ -329,7 +330,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             delta = -row_delta[row];
             lse2 = row_lse[row] == -INFINITY ? -INFINITY : -row_lse[row] * LOG2E;  // a row that has seen nothing: weights of zero
         }
-        int next_tile = from * T, next_head = kv * p.group;  // dK, dV
+        int next_tile = KV && count > 0 ? tile_at(0) : 0, next_head = KV && count > 0 ? head_at(0) : 0;  // dK, dV
         for (int j = 0; j < count && ok; ++j) {
             const int t0 = KV ? next_tile : tile_at(j), c0 = t0 + MINE * group;
             const float *const my_lse = stats[2 * j & 2] + MINE * group, *const my_delta = stats[(2 * j & 2) + 1] + MINE * group;
@@ -469,13 +470,22 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                         o[i] = count > 0 ? o[i] * by : 0.f;
                         zero = fmaf(o[i], 0.f, zero);
                     }
-                    tc::stage_32<E, COLUMNS>(stage, 32 * b, o);
+                    if (mine_of.alone) {
+                        tc::stage_32<E, COLUMNS>(stage, 32 * b, o);
+                    } else if (row < n_rows) {
+                        const int64_t array = (KV ? p.k_rows : p.q_rows) * heads * p.head_dim;
+                        float *sums = p.part_o + (KV ? 2 * part + (group < 2) : part) * array + (((KV ? s.k0 : s.q0) + (int64_t)r0 + row) * heads + head) * p.head_dim;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            if (first + 32 * b + i < p.head_dim) *reinterpret_cast<float4 *>(sums + first + 32 * b + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
                 }
                 const int row0 = (warp & 3) * 32;
-                tc::store_staged<E, COLUMNS>(stage, static_cast<E *>(to.data) + ((int64_t)(KV ? s.k0 : s.q0) + r0 + row0) * to.row + head * to.head + first,
+                if (mine_of.alone)
+                    tc::store_staged<E, COLUMNS>(stage, static_cast<E *>(to.data) + ((int64_t)(KV ? s.k0 : s.q0) + r0 + row0) * to.row + head * to.head + first,
                                              to.row, n_rows - row0, p.head_dim - first);
             }
-            const unsigned rows = __ballot_sync(0xffffffffu, zero != 0.f && row < n_rows);
+            const unsigned rows = __ballot_sync(0xffffffffu, zero != 0.f && row < n_rows && mine_of.alone);
             if (lane == 0 && rows) atomicOr(&bad[warp & 3], rows);
         }
     }
@@ -494,24 +504,34 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
 }
 
 template <class E, int DP, bool CAP, bool BIAS>
-cudaError_t launch(const AttentionParams &p, const Maps &maps, cudaStream_t s)
+cudaError_t launch(const AttentionParams &p0, const Parts &parts, const Maps &maps, cudaStream_t s)
 {
     static SmemOptinCache optin_q, optin_kv;
     constexpr size_t smem_q = Shape<DP, false>::SMEM, smem_kv = Shape<DP, true>::SMEM;
     cudaError_t e = optin_dynamic_smem(attention_backward_tc_kernel<E, DP, CAP, BIAS, false>, smem_q, optin_q);
     if (e == cudaSuccess) e = optin_dynamic_smem(attention_backward_tc_kernel<E, DP, CAP, BIAS, true>, smem_kv, optin_kv);
     if (e != cudaSuccess) return e;
-    const unsigned grid_q = (unsigned)(p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, T));
-    const unsigned grid_kv = (unsigned)(p.kv_heads * most_blocks(p.k_rows, p.n_seqs, p.max_k, T));
-    if (grid_q) attention_backward_tc_kernel<E, DP, CAP, BIAS, false><<<grid_q, THREADS, smem_q, s>>>(p, maps);
-    if (grid_kv) attention_backward_tc_kernel<E, DP, CAP, BIAS, true><<<grid_kv, THREADS, smem_kv, s>>>(p, maps);
-    return cudaGetLastError();
+    const unsigned grid_q = (unsigned)(p0.q_heads * most_blocks(p0.q_rows, p0.n_seqs, p0.max_q, T));
+    const unsigned grid_kv = (unsigned)(p0.kv_heads * most_blocks(p0.k_rows, p0.n_seqs, p0.max_k, T));
+    AttentionParams p = p0;
+    p.n_splits = parts.n_q;
+    p.chunk_tiles = parts.tiles_q;
+    if (grid_q) attention_backward_tc_kernel<E, DP, CAP, BIAS, false><<<grid_q * parts.n_q, THREADS, smem_q, s>>>(p, maps);
+    e = cudaGetLastError();
+    if (e == cudaSuccess && parts.n_q > 1) e = launch_attention_sum_parts(p, false, T, s);
+    if (e != cudaSuccess) return e;
+    p.n_splits = parts.n_kv;
+    p.chunk_tiles = parts.tiles_kv;
+    if (grid_kv) attention_backward_tc_kernel<E, DP, CAP, BIAS, true><<<grid_kv * parts.n_kv, THREADS, smem_kv, s>>>(p, maps);
+    e = cudaGetLastError();
+    if (e == cudaSuccess && parts.n_kv > 1) e = launch_attention_sum_parts(p, true, T, s);
+    return e;
 }
 template <class E, int DP>
-cudaError_t by_score(const AttentionParams &p, const Maps &maps, cudaStream_t s)
+cudaError_t by_score(const AttentionParams &p, const Parts &parts, const Maps &maps, cudaStream_t s)
 {
-    if (p.cap > 0.f) return p.slopes ? launch<E, DP, true, true>(p, maps, s) : launch<E, DP, true, false>(p, maps, s);
-    return p.slopes ? launch<E, DP, false, true>(p, maps, s) : launch<E, DP, false, false>(p, maps, s);
+    if (p.cap > 0.f) return p.slopes ? launch<E, DP, true, true>(p, parts, maps, s) : launch<E, DP, true, false>(p, parts, maps, s);
+    return p.slopes ? launch<E, DP, false, true>(p, parts, maps, s) : launch<E, DP, false, false>(p, parts, maps, s);
 }
 
 // 16-byte accesses to the rows of an array
@@ -519,7 +539,7 @@ bool wide(const HeadArray &a) { return (uintptr_t)a.data % 16 == 0 && a.row % 8 
 
 }  // namespace
 
-cudaError_t launch_attention_backward_tc(const AttentionParams &p, bool *taken, cudaStream_t s)
+cudaError_t launch_attention_backward_tc(const AttentionParams &p, const Parts &parts, bool *taken, cudaStream_t s)
 {
     Maps maps;
     *taken = p.dtype != 0 && wide(p.o) && wide(p.d_o) && wide(p.dq) && wide(p.dk) && wide(p.dv) &&
@@ -528,8 +548,8 @@ cudaError_t launch_attention_backward_tc(const AttentionParams &p, bool *taken, 
              make_tensor_map(&maps.v, p.v, p.dtype, p.head_dim, p.kv_heads, p.k_rows, T) &&
              make_tensor_map(&maps.d_o, p.d_o, p.dtype, p.head_dim, p.q_heads, p.q_rows, T);
     if (!*taken) return cudaSuccess;
-    if (p.dtype == 1) return p.head_dim <= 64 ? by_score<__half, 64>(p, maps, s) : by_score<__half, 128>(p, maps, s);
-    return p.head_dim <= 64 ? by_score<__nv_bfloat16, 64>(p, maps, s) : by_score<__nv_bfloat16, 128>(p, maps, s);
+    if (p.dtype == 1) return p.head_dim <= 64 ? by_score<__half, 64>(p, parts, maps, s) : by_score<__half, 128>(p, parts, maps, s);
+    return p.head_dim <= 64 ? by_score<__nv_bfloat16, 64>(p, parts, maps, s) : by_score<__nv_bfloat16, 128>(p, parts, maps, s);
 }
 
 }  // namespace sddmm

@@ -233,26 +233,6 @@ __global__ void __launch_bounds__(THREADS) attention_forward_general_kernel(cons
     }
 }
 
-// Where the blocks alone would leave multiprocessors idle, the tiles that a block goes through are cut into parts, a block each, which leave
-// their sums in the workspace (parts x rows x heads x head_dim) for attention_sum_parts_kernel.
-struct Part {
-    int first, end;  // tiles
-    bool alone;      // no other part: the block stores its results itself
-};
-__device__ __forceinline__ Part part_of(const AttentionParams &p, int tiles, int part)
-{
-    const int each = p.chunk_tiles, n = max(1, (tiles + each - 1) / each);
-    return Part{part * each, part < n ? min(tiles, (part + 1) * each) : -1, n == 1};  // (end -1: there is no such part)
-}
-// The tiles of queries that see keys [j0, j0 + m): `per_head` from `from` on, for every head of the group.
-__device__ __forceinline__ void query_tiles(const AttentionParams &p, const Sequence &s, int j0, int m, int &from, int &per_head)
-{
-    int to;
-    queries_of(p.window, s, j0, j0 + m, from, to);
-    from /= B;
-    per_head = to > from * B ? (to + B - 1) / B - from : 0;
-}
-
 // dQ of 64 queries; leaves delta for attention_dkv_general_kernel.
 template <class T, int DP>
 __global__ void __launch_bounds__(THREADS) attention_dq_general_kernel(const AttentionParams p)
@@ -359,7 +339,7 @@ __global__ void __launch_bounds__(THREADS) attention_dkv_general_kernel(const At
     if (!find_block<B>(p, block_of / p.kv_heads, true, s, seq, block)) return;
     const int j0 = block * B, m = min(B, s.nk - j0);
     int from, per_head;
-    query_tiles(p, s, j0, m, from, per_head);
+    query_tiles<B>(p, s, j0, m, from, per_head);
     const Part mine = part_of(p, per_head * p.group, part);
     if (mine.end < 0) return;
     load_rows<T, DP>(sk, p.k, (int64_t)s.k0 + j0, m, kv, p.head_dim);
@@ -422,24 +402,24 @@ __global__ void __launch_bounds__(THREADS) attention_dkv_general_kernel(const At
         if (turn % (THREADS / 32) == (int)threadIdx.x / 32) strict::dkv_row<T>(p, s, kv, j0 + __ffsll((long long)left) - 1);
 }
 
-// The parts' sums of 64 rows added in order; KV: dK and dV, else dQ.
-template <class T, bool KV>
+// The parts' sums of TILE rows added in order; KV: dK and dV, else dQ.
+template <class T, bool KV, int TILE>
 __global__ void __launch_bounds__(THREADS) attention_sum_parts_kernel(const AttentionParams p)
 {
-    __shared__ unsigned long long bad;
-    if (threadIdx.x == 0) bad = 0;
+    __shared__ unsigned long long bad[TILE / 64];
+    if (threadIdx.x < TILE / 64) bad[threadIdx.x] = 0;
     const int heads = KV ? p.kv_heads : p.q_heads, head = blockIdx.x % heads;
     Sequence s;
     int seq, block;
-    if (!find_block<B>(p, blockIdx.x / heads, KV, s, seq, block)) return;
-    const int r0 = block * B, rows = min(B, (KV ? s.nk : s.nq) - r0);
+    if (!find_block<TILE>(p, blockIdx.x / heads, KV, s, seq, block)) return;
+    const int r0 = block * TILE, rows = min(TILE, (KV ? s.nk : s.nq) - r0);
     int tiles;
     if (KV) {
         int from, per_head;
-        query_tiles(p, s, r0, rows, from, per_head);
+        query_tiles<TILE>(p, s, r0, rows, from, per_head);
         tiles = per_head * p.group;
     } else {
-        tiles = key_tiles<B>(reach_of(p.window, s, r0, r0 + rows)).n;
+        tiles = key_tiles<TILE>(reach_of(p.window, s, r0, r0 + rows)).n;
     }
     const int parts = (tiles + p.chunk_tiles - 1) / p.chunk_tiles;
     if (parts <= 1) return;
@@ -453,23 +433,25 @@ __global__ void __launch_bounds__(THREADS) attention_sum_parts_kernel(const Atte
         for (int x = 0; x < (KV ? 2 : 1); ++x) {
             const float *from = p.part_o + x * array + (row * heads + head) * p.head_dim + c;
             float4 sum = at4(from);
+#pragma unroll 4
             for (int k = 1; k < parts; ++k) {
                 const float4 v = at4(from + k * array * (KV ? 2 : 1));
                 sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
             }
-            collect(&bad, not_finite(sum), r);
+            collect(&bad[r / 64], not_finite(sum), r % 64);
             store4<T>(KV ? (x ? p.dv : p.dk) : p.dq, row, head, c, p.head_dim, sum);
         }
     }
     __syncthreads();
     int turn = 0;
-    for (unsigned long long left = bad; left; left &= left - 1, ++turn) {
-        const int r = __ffsll((long long)left) - 1;
-        if (turn % (THREADS / 32) != (int)threadIdx.x / 32) continue;
-        const int64_t at = (int64_t)head * p.q_rows + s.q0 + r0 + r;
-        if (KV) strict::dkv_row<T>(p, s, head, r0 + r);
-        else strict::dq_row<T>(p, s, head, r0 + r, __ldg(p.lse + at), p.delta[at]);
-    }
+    for (int q = 0; q < TILE / 64; ++q)
+        for (unsigned long long left = bad[q]; left; left &= left - 1, ++turn) {
+            const int r = 64 * q + __ffsll((long long)left) - 1;
+            if (turn % (THREADS / 32) != (int)threadIdx.x / 32) continue;
+            const int64_t at = (int64_t)head * p.q_rows + s.q0 + r0 + r;
+            if (KV) strict::dkv_row<T>(p, s, head, r0 + r);
+            else strict::dq_row<T>(p, s, head, r0 + r, __ldg(p.lse + at), p.delta[at]);
+        }
 }
 
 template <class Kern>
@@ -491,32 +473,32 @@ cudaError_t forward_of(const AttentionParams &p, cudaStream_t s)
     return launch(attention_forward_general_kernel<T, DP>, optin, grid, smem_of(DP, 3, 1), p, s);
 }
 template <class T, int DP>
-cudaError_t backward_of(const AttentionParams &p0, const GeneralParts &parts, cudaStream_t s)
+cudaError_t backward_of(const AttentionParams &p0, const Parts &parts, cudaStream_t s)
 {
-    static SmemOptinCache optin_q, optin_kv, none;
+    static SmemOptinCache optin_q, optin_kv;
     const unsigned grid_q = (unsigned)(p0.q_heads * most_blocks(p0.q_rows, p0.n_seqs, p0.max_q, B));
     const unsigned grid_kv = (unsigned)(p0.kv_heads * most_blocks(p0.k_rows, p0.n_seqs, p0.max_k, B));
     AttentionParams p = p0;
     p.n_splits = parts.n_q;
     p.chunk_tiles = parts.tiles_q;
     cudaError_t e = launch(attention_dq_general_kernel<T, DP>, optin_q, grid_q * parts.n_q, smem_of(DP, 4, 1), p, s);
-    if (e == cudaSuccess && parts.n_q > 1) e = launch(attention_sum_parts_kernel<T, false>, none, grid_q, 0, p, s);
+    if (e == cudaSuccess && parts.n_q > 1) e = launch_attention_sum_parts(p, false, B, s);
     if (e != cudaSuccess) return e;
     p.n_splits = parts.n_kv;
     p.chunk_tiles = parts.tiles_kv;
     e = launch(attention_dkv_general_kernel<T, DP>, optin_kv, grid_kv * parts.n_kv, smem_of(DP, 4, 2), p, s);
-    if (e == cudaSuccess && parts.n_kv > 1) e = launch(attention_sum_parts_kernel<T, true>, none, grid_kv, 0, p, s);
+    if (e == cudaSuccess && parts.n_kv > 1) e = launch_attention_sum_parts(p, true, B, s);
     return e;
 }
 
 // parts null: forward
 template <class T>
-cudaError_t by_width(const GeneralParts *parts, const AttentionParams &p, cudaStream_t s)
+cudaError_t by_width(const Parts *parts, const AttentionParams &p, cudaStream_t s)
 {
     if (p.head_dim <= 64) return parts ? backward_of<T, 64>(p, *parts, s) : forward_of<T, 64>(p, s);
     return parts ? backward_of<T, 128>(p, *parts, s) : forward_of<T, 128>(p, s);
 }
-cudaError_t by_type(const GeneralParts *parts, const AttentionParams &p, cudaStream_t s)
+cudaError_t by_type(const Parts *parts, const AttentionParams &p, cudaStream_t s)
 {
     switch (p.dtype) {
     case 0: return by_width<float>(parts, p, s);
@@ -527,32 +509,41 @@ cudaError_t by_type(const GeneralParts *parts, const AttentionParams &p, cudaStr
 
 }  // namespace
 
-GeneralParts plan_general_parts(const AttentionParams &p, int sm_count)
+Parts plan_attention_parts(const AttentionParams &p, int tile, int per_sm, int sm_count)
 {
-    // Parts until there are four blocks for a multiprocessor (a causal mask leaves some with little to do), of two tiles at least, and at
+    // Parts until there are `per_sm` blocks for a multiprocessor (a causal mask leaves some with little to do), of two tiles at least, and at
     // most 256 MB of sums.
     auto cut = [&](int64_t blocks, int64_t tiles, int64_t bytes_of_one, int &n, int &each) {
         n = 1;
         each = (int)(tiles > 0 ? tiles : 1);
         if (blocks <= 0 || tiles <= 2) return;
-        int64_t want = (4ll * sm_count + blocks - 1) / blocks;
+        int64_t want = ((int64_t)per_sm * sm_count + blocks - 1) / blocks;
         if (want > (256ll << 20) / (bytes_of_one > 0 ? bytes_of_one : 1)) want = (256ll << 20) / (bytes_of_one > 0 ? bytes_of_one : 1);
         if (want > (tiles + 1) / 2) want = (tiles + 1) / 2;
         if (want <= 1) return;
         each = (int)((tiles + want - 1) / want);
         n = (int)((tiles + each - 1) / each);
     };
-    GeneralParts g{1, 1 << 30, 1, 1 << 30, 0};
-    if (p.dtype != 0) return g;  // (16-bit types come here for their strides alone: no workspace for that)
+    Parts g{};
     const int64_t bytes_q = 4 * p.q_rows * p.q_heads * p.head_dim, bytes_kv = 8 * p.k_rows * p.kv_heads * p.head_dim;
-    cut(p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, B), (p.max_k + B - 1) / B, bytes_q, g.n_q, g.tiles_q);
-    cut(p.kv_heads * most_blocks(p.k_rows, p.n_seqs, p.max_k, B), (int64_t)((p.max_q + B - 1) / B) * p.group, bytes_kv, g.n_kv, g.tiles_kv);
+    cut(p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, tile), (p.max_k + tile - 1) / tile, bytes_q, g.n_q, g.tiles_q);
+    cut(p.kv_heads * most_blocks(p.k_rows, p.n_seqs, p.max_k, tile), (int64_t)((p.max_q + tile - 1) / tile) * p.group, bytes_kv, g.n_kv, g.tiles_kv);
     const int64_t q = g.n_q > 1 ? g.n_q * bytes_q : 0, kv = g.n_kv > 1 ? g.n_kv * bytes_kv : 0;
     g.bytes = q > kv ? q : kv;  // one behind the other
     return g;
 }
 
+cudaError_t launch_attention_sum_parts(const AttentionParams &p, bool kv, int tile, cudaStream_t s)
+{
+    const unsigned grid = (unsigned)(kv ? p.kv_heads * most_blocks(p.k_rows, p.n_seqs, p.max_k, tile) : p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, tile));
+    if (grid == 0) return cudaSuccess;
+    if (p.dtype == 0) kv ? attention_sum_parts_kernel<float, true, 64><<<grid, THREADS, 0, s>>>(p) : attention_sum_parts_kernel<float, false, 64><<<grid, THREADS, 0, s>>>(p);
+    else if (p.dtype == 1) kv ? attention_sum_parts_kernel<__half, true, 128><<<grid, THREADS, 0, s>>>(p) : attention_sum_parts_kernel<__half, false, 128><<<grid, THREADS, 0, s>>>(p);
+    else kv ? attention_sum_parts_kernel<__nv_bfloat16, true, 128><<<grid, THREADS, 0, s>>>(p) : attention_sum_parts_kernel<__nv_bfloat16, false, 128><<<grid, THREADS, 0, s>>>(p);
+    return cudaGetLastError();
+}
+
 cudaError_t launch_attention_forward_general(const AttentionParams &p, cudaStream_t s) { return by_type(nullptr, p, s); }
-cudaError_t launch_attention_backward_general(const AttentionParams &p, const GeneralParts &parts, cudaStream_t s) { return by_type(&parts, p, s); }
+cudaError_t launch_attention_backward_general(const AttentionParams &p, const Parts &parts, cudaStream_t s) { return by_type(&parts, p, s); }
 
 }  // namespace sddmm
