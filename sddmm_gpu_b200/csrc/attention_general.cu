@@ -6,6 +6,7 @@
 // eight neighbouring rows then meet all banks).  The gradients are two kernels, each with the scores anew: dQ (which also leaves
 // delta_i = dO_i.O_i for the other) and dK, dV, which sums over the query heads of its group.  No atomics: results do not
 // depend on scheduling.
+// A tile's copies are asked for as soon as the last one in its place has been used, and come in under the product in between.
 //
 // What bounds it: the FMA pipe and the shared-memory loads that feed it (two 128-bit loads per 16 FMAs).
 #include "attention_strict.cuh"
@@ -17,23 +18,31 @@ namespace {
 
 constexpr int B = 64, THREADS = 256, PS = B + 4;
 
-// Rows [row0, row0 + n) of one head into shared memory, zeros behind row n and column D.
-template <class T, int DP>
-__device__ __forceinline__ void load_rows(float *dst, const HeadArray &a, int64_t row0, int n, int head, int D)
+// Rows [row0, row0 + n) of one head into shared memory, zeros behind row n; a row of D columns has `stride` = D + 4 floats.  fp32 rows with
+// 16-byte alignment come by asynchronous copies, which the caller waits for (arrived()); others have been stored when this returns.
+template <class T>
+__device__ __forceinline__ void load_rows(float *dst, const HeadArray &a, int64_t row0, int n, int head, int D, int stride)
 {
     const T *src = static_cast<const T *>(a.data) + row0 * a.row + head * a.head;
     const bool vec = sizeof(T) == 4 && (((uintptr_t)src | (uintptr_t)(a.row * 4)) & 15) == 0;
-    for (int i = threadIdx.x; i < B * DP / 4; i += THREADS) {
-        const int r = i / (DP / 4), c = i % (DP / 4) * 4;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < n && c < D) {
-            const T *x = src + r * a.row + c;
-            if (vec) v = __ldg(reinterpret_cast<const float4 *>(x));
-            else v = make_float4(to_f(x[0]), to_f(x[1]), to_f(x[2]), to_f(x[3]));
+    const int quads = D / 4, step = THREADS / quads;  // a thread keeps its columns: `step` rows at once
+    const int c = threadIdx.x % quads * 4;
+    if ((int)threadIdx.x < step * quads)
+        for (int r = threadIdx.x / quads; r < B; r += step) {
+            const T *x = src + (r < n ? r : 0) * a.row + c;
+            float *to = dst + r * stride + c;
+            if (vec) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dev::smem_u32(to)), "l"(x), "r"(r < n ? 16 : 0) : "memory");
+            } else {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r < n) v = make_float4(to_f(x[0]), to_f(x[1]), to_f(x[2]), to_f(x[3]));
+                *reinterpret_cast<float4 *>(to) = v;
+            }
         }
-        *reinterpret_cast<float4 *>(dst + r * (DP + 4) + c) = v;
-    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
 }
+// All of this thread's copies but the last `N` load_rows() have landed.
+template <int N> __device__ __forceinline__ void arrived() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ float4 at4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 using F2 = unsigned long long;  // two fp32 values: one FMA instruction for both
 using dev::ffma2;
@@ -46,17 +55,17 @@ __device__ __forceinline__ F2 twice(float x)
 }
 __device__ __forceinline__ ulonglong2 pairs(const float *p) { return *reinterpret_cast<const ulonglong2 *>(p); }
 // acc[r][c] = row ty + 16 r of x times row tx + 16 c of y, D columns
-template <int DP>
 __device__ __forceinline__ void rows_times_rows(float (&acc)[4][4], const float *x, const float *y, int ty, int tx, int D)
 {
     F2 sum[4][4] = {};
+    const int stride = D + 4;
 #pragma unroll 2
     for (int d = 0; d < D; d += 4) {
         ulonglong2 a[4], b[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) a[r] = pairs(x + (ty + 16 * r) * (DP + 4) + d);
+        for (int r = 0; r < 4; ++r) a[r] = pairs(x + (ty + 16 * r) * stride + d);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) b[c] = pairs(y + (tx + 16 * c) * (DP + 4) + d);
+        for (int c = 0; c < 4; ++c) b[c] = pairs(y + (tx + 16 * c) * stride + d);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -84,9 +93,9 @@ __device__ __forceinline__ void add_times(Quad &acc, float w, ulonglong2 v)
     acc.a = ffma2(ww, v.x, acc.a);
     acc.b = ffma2(ww, v.y, acc.b);
 }
-// acc[r][c] += sum_j w[row ty + 16 r][j] * x[j][4 tx + 64 c ..]
+// acc[r][c] += sum_j w[row ty + 16 r][j] * x[j][4 tx + 64 c ..]; columns from the head's width on are anything
 template <int DP>
-__device__ __forceinline__ void weights_times_rows(Quad (&acc)[4][DP / 64], const float *w, const float *x, int ty, int tx)
+__device__ __forceinline__ void weights_times_rows(Quad (&acc)[4][DP / 64], const float *w, const float *x, int ty, int tx, int stride)
 {
 #pragma unroll 2
     for (int j = 0; j < B; j += 4) {
@@ -97,7 +106,7 @@ __device__ __forceinline__ void weights_times_rows(Quad (&acc)[4][DP / 64], cons
         for (int u = 0; u < 4; ++u)
 #pragma unroll
             for (int c = 0; c < DP / 64; ++c) {
-                const ulonglong2 v = pairs(x + (j + u) * (DP + 4) + 4 * tx + 64 * c);
+                const ulonglong2 v = pairs(x + (j + u) * stride + 4 * tx + 64 * c);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) add_times(acc[r][c], u == 0 ? p[r].x : u == 1 ? p[r].y : u == 2 ? p[r].z : p[r].w, v);
             }
@@ -105,14 +114,14 @@ __device__ __forceinline__ void weights_times_rows(Quad (&acc)[4][DP / 64], cons
 }
 // acc[r][c] += sum_i w[i][4 ty + r] * x[i][4 tx + 64 c ..]
 template <int DP>
-__device__ __forceinline__ void weights_t_times_rows(Quad (&acc)[4][DP / 64], const float *w, const float *x, int ty, int tx)
+__device__ __forceinline__ void weights_t_times_rows(Quad (&acc)[4][DP / 64], const float *w, const float *x, int ty, int tx, int stride)
 {
 #pragma unroll 4
     for (int i = 0; i < B; ++i) {
         const float4 p = at4(w + i * PS + 4 * ty);
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
-            const ulonglong2 v = pairs(x + i * (DP + 4) + 4 * tx + 64 * c);
+            const ulonglong2 v = pairs(x + i * stride + 4 * tx + 64 * c);
             add_times(acc[0][c], p.x, v);
             add_times(acc[1][c], p.y, v);
             add_times(acc[2][c], p.z, v);
@@ -146,13 +155,14 @@ __device__ __forceinline__ void collect(unsigned long long *bits, bool bad, int 
 }
 
 template <class T, int DP>
-__global__ void __launch_bounds__(THREADS) attention_forward_general_kernel(const AttentionParams p)
+__global__ void __launch_bounds__(THREADS, 2) attention_forward_general_kernel(const AttentionParams p)
 {
     extern __shared__ float sm[];
     __shared__ unsigned long long bad;
     __shared__ float bad_lse[B];
     if (threadIdx.x == 0) bad = 0;
-    float *sq = sm, *sk = sq + B * (DP + 4), *sv = sk + B * (DP + 4), *sp = sv + B * (DP + 4);
+    const int stride = p.head_dim + 4;
+    float *sq = sm, *sk = sq + B * stride, *sv = sk + B * stride, *sp = sv + B * stride;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = blockIdx.x % p.q_heads, kv = head / p.group;
     Sequence s;
     int seq, block;
@@ -160,21 +170,24 @@ __global__ void __launch_bounds__(THREADS) attention_forward_general_kernel(cons
     if (!find_block<B>(p, (gridDim.x - 1 - blockIdx.x) / p.q_heads, false, s, seq, block)) return;
     const int i0 = block * B, n = min(B, s.nq - i0);
     const float slope = p.slopes ? __ldg(p.slopes + head) : 0.f;
-    load_rows<T, DP>(sq, p.q, (int64_t)s.q0 + i0, n, head, p.head_dim);
+    load_rows<T>(sq, p.q, (int64_t)s.q0 + i0, n, head, p.head_dim, stride);
     const Reach reach = reach_of(p.window, s, i0, i0 + n);
     const KeyTiles tiles = key_tiles<B>(reach);
     Quad o[4][DP / 64] = {};
     float top[4], sum[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) top[r] = -INFINITY, sum[r] = 0.f;
+    auto fetch = [&](float *to, const HeadArray &a, int t) {
+        const int j0 = tiles.tile(t) * B;
+        load_rows<T>(to, a, (int64_t)s.k0 + j0, min(B, s.nk - j0), kv, p.head_dim, stride);
+    };
+    if (tiles.n > 0) fetch(sk, p.k, 0), fetch(sv, p.v, 0);
     for (int t = 0; t < tiles.n; ++t) {
-        const int j0 = tiles.tile(t) * B, m = min(B, s.nk - j0);
-        __syncthreads();
-        load_rows<T, DP>(sk, p.k, (int64_t)s.k0 + j0, m, kv, p.head_dim);
-        load_rows<T, DP>(sv, p.v, (int64_t)s.k0 + j0, m, kv, p.head_dim);
+        const int j0 = tiles.tile(t) * B;
+        arrived<1>();  // K, and Q
         __syncthreads();
         float x[4][4];
-        rows_times_rows<DP>(x, sq, sk, ty, tx, p.head_dim);
+        rows_times_rows(x, sq, sk, ty, tx, p.head_dim);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int pos = reach.first_pos + ty + 16 * r;
@@ -205,8 +218,13 @@ __global__ void __launch_bounds__(THREADS) attention_forward_general_kernel(cons
                 o[r][c].b = ffma2(o[r][c].b, by, 0ull);
             }
         }
+        arrived<0>();  // V
         __syncthreads();
-        weights_times_rows<DP>(o, sp, sv, ty, tx);
+        const bool more = t + 1 < tiles.n;
+        if (more) fetch(sk, p.k, t + 1);  // under the product with V
+        weights_times_rows<DP>(o, sp, sv, ty, tx, stride);
+        __syncthreads();
+        if (more) fetch(sv, p.v, t + 1);  // under the next scores
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -217,7 +235,7 @@ __global__ void __launch_bounds__(THREADS) attention_forward_general_kernel(cons
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
             const float4 v = open(o[r][c]);
-            collect(&bad, not_finite(v), i);
+            collect(&bad, not_finite(v) && 4 * tx + 64 * c < p.head_dim, i);
             store4<T>(p.o, row, head, 4 * tx + 64 * c, p.head_dim, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         }
         if (tx == 0) {
@@ -235,13 +253,14 @@ __global__ void __launch_bounds__(THREADS) attention_forward_general_kernel(cons
 
 // dQ of 64 queries; leaves delta for attention_dkv_general_kernel.
 template <class T, int DP>
-__global__ void __launch_bounds__(THREADS) attention_dq_general_kernel(const AttentionParams p)
+__global__ void __launch_bounds__(THREADS, 2) attention_dq_general_kernel(const AttentionParams p)
 {
     extern __shared__ float sm[];
     __shared__ unsigned long long bad;
     __shared__ float bad_lse[B], bad_delta[B];
     if (threadIdx.x == 0) bad = 0;
-    float *sq = sm, *sdo = sq + B * (DP + 4), *sk = sdo + B * (DP + 4), *sv = sk + B * (DP + 4), *sds = sv + B * (DP + 4);
+    const int stride = p.head_dim + 4;
+    float *sq = sm, *sdo = sq + B * stride, *sk = sdo + B * stride, *sv = sk + B * stride, *sds = sv + B * stride;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const unsigned block_of = blockIdx.x / p.n_splits, part = blockIdx.x % p.n_splits, blocks = gridDim.x / p.n_splits;
     const int head = block_of % p.q_heads, kv = head / p.group;
@@ -254,16 +273,17 @@ __global__ void __launch_bounds__(THREADS) attention_dq_general_kernel(const Att
     const Part mine = part_of(p, tiles.n, part);
     if (mine.end < 0) return;
     const float slope = p.slopes ? __ldg(p.slopes + head) : 0.f;
-    load_rows<T, DP>(sq, p.q, (int64_t)s.q0 + i0, n, head, p.head_dim);
-    load_rows<T, DP>(sdo, p.d_o, (int64_t)s.q0 + i0, n, head, p.head_dim);
-    load_rows<T, DP>(sk, p.o, (int64_t)s.q0 + i0, n, head, p.head_dim);
+    load_rows<T>(sq, p.q, (int64_t)s.q0 + i0, n, head, p.head_dim, stride);
+    load_rows<T>(sdo, p.d_o, (int64_t)s.q0 + i0, n, head, p.head_dim, stride);
+    load_rows<T>(sk, p.o, (int64_t)s.q0 + i0, n, head, p.head_dim, stride);
+    arrived<0>();
     __syncthreads();
     float delta[4], lse[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int i = ty + 16 * r;
         float d = 0.f;
-        for (int c = tx; c < p.head_dim; c += 16) d = fmaf(sdo[i * (DP + 4) + c], sk[i * (DP + 4) + c], d);
+        for (int c = tx; c < p.head_dim; c += 16) d = fmaf(sdo[i * stride + c], sk[i * stride + c], d);
         delta[r] = over16(d, true);
         const int64_t at = (int64_t)head * p.q_rows + s.q0 + i0 + i;
         lse[r] = i < n ? __ldg(p.lse + at) : -INFINITY;
@@ -274,15 +294,21 @@ __global__ void __launch_bounds__(THREADS) attention_dq_general_kernel(const Att
         }
     }
     Quad dq[4][DP / 64] = {};
+    auto fetch = [&](float *to, const HeadArray &a, int t) {
+        const int j0 = tiles.tile(t) * B;
+        load_rows<T>(to, a, (int64_t)s.k0 + j0, min(B, s.nk - j0), kv, p.head_dim, stride);
+    };
+    __syncthreads();  // (O lay where K is to lie)
+    if (mine.first < mine.end) fetch(sv, p.v, mine.first), fetch(sk, p.k, mine.first);
     for (int t = mine.first; t < mine.end; ++t) {
-        const int j0 = tiles.tile(t) * B, m = min(B, s.nk - j0);
-        __syncthreads();
-        load_rows<T, DP>(sk, p.k, (int64_t)s.k0 + j0, m, kv, p.head_dim);
-        load_rows<T, DP>(sv, p.v, (int64_t)s.k0 + j0, m, kv, p.head_dim);
-        __syncthreads();
+        const int j0 = tiles.tile(t) * B;
         float x[4][4], dp[4][4];
-        rows_times_rows<DP>(x, sq, sk, ty, tx, p.head_dim);
-        rows_times_rows<DP>(dp, sdo, sv, ty, tx, p.head_dim);
+        arrived<1>();
+        __syncthreads();
+        rows_times_rows(dp, sdo, sv, ty, tx, p.head_dim);
+        arrived<0>();
+        __syncthreads();
+        rows_times_rows(x, sq, sk, ty, tx, p.head_dim);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int pos = reach.first_pos + ty + 16 * r;
@@ -297,7 +323,11 @@ __global__ void __launch_bounds__(THREADS) attention_dq_general_kernel(const Att
             }
         }
         __syncthreads();
-        weights_times_rows<DP>(dq, sds, sk, ty, tx);
+        const bool more = t + 1 < mine.end;
+        if (more) fetch(sv, p.v, t + 1);  // under the product with K
+        weights_times_rows<DP>(dq, sds, sk, ty, tx, stride);
+        __syncthreads();
+        if (more) fetch(sk, p.k, t + 1);  // under the next dP
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -307,7 +337,7 @@ __global__ void __launch_bounds__(THREADS) attention_dq_general_kernel(const Att
         for (int c = 0; c < DP / 64; ++c) {
             const float4 v = open(dq[r][c]);
             if (mine.alone) {
-                collect(&bad, not_finite(v), i);
+                collect(&bad, not_finite(v) && 4 * tx + 64 * c < p.head_dim, i);
                 store4<T>(p.dq, (int64_t)s.q0 + i0 + i, head, 4 * tx + 64 * c, p.head_dim, v);
             } else if (4 * tx + 64 * c < p.head_dim) {
                 *reinterpret_cast<float4 *>(p.part_o + ((part * p.q_rows + s.q0 + i0 + i) * p.q_heads + head) * p.head_dim + 4 * tx + 64 * c) = v;
@@ -329,7 +359,8 @@ __global__ void __launch_bounds__(THREADS) attention_dkv_general_kernel(const At
     extern __shared__ float sm[];
     __shared__ unsigned long long bad;
     if (threadIdx.x == 0) bad = 0;
-    float *sk = sm, *sv = sk + B * (DP + 4), *sq = sv + B * (DP + 4), *sdo = sq + B * (DP + 4), *sp = sdo + B * (DP + 4), *sds = sp + B * PS;
+    const int stride = p.head_dim + 4;
+    float *sk = sm, *sv = sk + B * stride, *sq = sv + B * stride, *sdo = sq + B * stride, *sp = sdo + B * stride, *sds = sp + B * PS;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const unsigned block_of = blockIdx.x / p.n_splits, part = blockIdx.x % p.n_splits;
     const int kv = block_of % p.kv_heads;
@@ -342,19 +373,24 @@ __global__ void __launch_bounds__(THREADS) attention_dkv_general_kernel(const At
     query_tiles<B>(p, s, j0, m, from, per_head);
     const Part mine = part_of(p, per_head * p.group, part);
     if (mine.end < 0) return;
-    load_rows<T, DP>(sk, p.k, (int64_t)s.k0 + j0, m, kv, p.head_dim);
-    load_rows<T, DP>(sv, p.v, (int64_t)s.k0 + j0, m, kv, p.head_dim);
+    load_rows<T>(sk, p.k, (int64_t)s.k0 + j0, m, kv, p.head_dim, stride);
+    load_rows<T>(sv, p.v, (int64_t)s.k0 + j0, m, kv, p.head_dim, stride);
     Quad dk[4][DP / 64] = {}, dv[4][DP / 64] = {};
+    auto fetch = [&](float *to, const HeadArray &a, int t) {
+        const int i0 = (from + t % per_head) * B;
+        load_rows<T>(to, a, (int64_t)s.q0 + i0, min(B, s.nq - i0), kv * p.group + t / per_head, p.head_dim, stride);
+    };
+    if (mine.first < mine.end) fetch(sdo, p.d_o, mine.first), fetch(sq, p.q, mine.first);
     for (int t = mine.first; t < mine.end; ++t) {
         const int head = kv * p.group + t / per_head, i0 = (from + t % per_head) * B, n = min(B, s.nq - i0);
         const float slope = p.slopes ? __ldg(p.slopes + head) : 0.f;
-        __syncthreads();
-        load_rows<T, DP>(sq, p.q, (int64_t)s.q0 + i0, n, head, p.head_dim);
-        load_rows<T, DP>(sdo, p.d_o, (int64_t)s.q0 + i0, n, head, p.head_dim);
-        __syncthreads();
         float x[4][4], dp[4][4];
-        rows_times_rows<DP>(x, sq, sk, ty, tx, p.head_dim);
-        rows_times_rows<DP>(dp, sdo, sv, ty, tx, p.head_dim);
+        arrived<1>();
+        __syncthreads();
+        rows_times_rows(dp, sdo, sv, ty, tx, p.head_dim);
+        arrived<0>();
+        __syncthreads();
+        rows_times_rows(x, sq, sk, ty, tx, p.head_dim);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int i = ty + 16 * r, pos = s.nk - s.nq + i0 + i;
@@ -375,8 +411,13 @@ __global__ void __launch_bounds__(THREADS) attention_dkv_general_kernel(const At
             }
         }
         __syncthreads();
-        weights_t_times_rows<DP>(dv, sp, sdo, ty, tx);
-        weights_t_times_rows<DP>(dk, sds, sq, ty, tx);
+        const bool more = t + 1 < mine.end;
+        weights_t_times_rows<DP>(dv, sp, sdo, ty, tx, stride);
+        __syncthreads();
+        if (more) fetch(sdo, p.d_o, t + 1);  // under the product with Q
+        weights_t_times_rows<DP>(dk, sds, sq, ty, tx, stride);
+        __syncthreads();
+        if (more) fetch(sq, p.q, t + 1);  // under the next dP
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -386,7 +427,7 @@ __global__ void __launch_bounds__(THREADS) attention_dkv_general_kernel(const At
             const int64_t row = (int64_t)s.k0 + j0 + 4 * ty + r;
             const float4 a = open(dk[r][c]), b = open(dv[r][c]);
             if (mine.alone) {
-                collect(&bad, not_finite(a) || not_finite(b), 4 * ty + r);
+                collect(&bad, (not_finite(a) || not_finite(b)) && 4 * tx + 64 * c < p.head_dim, 4 * ty + r);
                 store4<T>(p.dk, row, kv, 4 * tx + 64 * c, p.head_dim, a);
                 store4<T>(p.dv, row, kv, 4 * tx + 64 * c, p.head_dim, b);
             } else if (4 * tx + 64 * c < p.head_dim) {
@@ -463,14 +504,14 @@ cudaError_t launch(Kern kern, SmemOptinCache &optin, unsigned grid, size_t smem,
     kern<<<grid, THREADS, smem, s>>>(p);
     return cudaGetLastError();
 }
-constexpr size_t smem_of(int DP, int tiles, int weights) { return ((size_t)tiles * B * (DP + 4) + (size_t)weights * B * PS) * sizeof(float); }
+size_t smem_of(int head_dim, int tiles, int weights) { return ((size_t)tiles * B * (head_dim + 4) + (size_t)weights * B * PS) * sizeof(float); }
 
 template <class T, int DP>
 cudaError_t forward_of(const AttentionParams &p, cudaStream_t s)
 {
     static SmemOptinCache optin;
     const unsigned grid = (unsigned)(p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, B));
-    return launch(attention_forward_general_kernel<T, DP>, optin, grid, smem_of(DP, 3, 1), p, s);
+    return launch(attention_forward_general_kernel<T, DP>, optin, grid, smem_of(p.head_dim, 3, 1), p, s);
 }
 template <class T, int DP>
 cudaError_t backward_of(const AttentionParams &p0, const Parts &parts, cudaStream_t s)
@@ -481,12 +522,12 @@ cudaError_t backward_of(const AttentionParams &p0, const Parts &parts, cudaStrea
     AttentionParams p = p0;
     p.n_splits = parts.n_q;
     p.chunk_tiles = parts.tiles_q;
-    cudaError_t e = launch(attention_dq_general_kernel<T, DP>, optin_q, grid_q * parts.n_q, smem_of(DP, 4, 1), p, s);
+    cudaError_t e = launch(attention_dq_general_kernel<T, DP>, optin_q, grid_q * parts.n_q, smem_of(p.head_dim, 4, 1), p, s);
     if (e == cudaSuccess && parts.n_q > 1) e = launch_attention_sum_parts(p, false, B, s);
     if (e != cudaSuccess) return e;
     p.n_splits = parts.n_kv;
     p.chunk_tiles = parts.tiles_kv;
-    e = launch(attention_dkv_general_kernel<T, DP>, optin_kv, grid_kv * parts.n_kv, smem_of(DP, 4, 2), p, s);
+    e = launch(attention_dkv_general_kernel<T, DP>, optin_kv, grid_kv * parts.n_kv, smem_of(p.head_dim, 4, 2), p, s);
     if (e == cudaSuccess && parts.n_kv > 1) e = launch_attention_sum_parts(p, true, B, s);
     return e;
 }
