@@ -67,10 +67,6 @@ class PlanInfo(C.Structure):
                 ("n_hub_cols", C.c_int64)]
 
 
-class HeadArray(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
-
-
 class AttentionDesc(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("dtype", "head_dim", "q_heads", "kv_heads", "n_seqs", "max_q", "max_k")] + [
         ("q_rows", C.c_int64), ("k_rows", C.c_int64), ("scale", C.c_float), ("softcap", C.c_float), ("window_left", C.c_int32),
@@ -79,7 +75,11 @@ class AttentionDesc(C.Structure):
 
 # sddmm_rotary_desc and sddmm_rotary_part, written with one call each (field by field costs microseconds a call)
 _ROTARY_DESC = struct.Struct("@iiiiqPqPfi")
+_HEADS = struct.Struct("@Pqq")  # sddmm_head_array
 _ROTARY_PART = struct.Struct("@PPqqqqiiPq")
+assert _ROTARY_PART.size == 72
+_LAYOUTS = {"half": ROTARY_HALF, "interleaved": ROTARY_INTERLEAVED}
+_int64 = None  # torch.int64, once torch is there
 
 _lib = None
 
@@ -115,7 +115,7 @@ def lib():
     L.sddmm_attention_plan.argtypes = [vp, C.POINTER(AttentionDesc), C.POINTER(vp)]
     L.sddmm_attention_destroy.argtypes = [vp]
     L.sddmm_attention_workspace.argtypes = [vp, C.c_int, C.POINTER(i64)]
-    heads = C.POINTER(HeadArray)
+    heads = vp
     L.sddmm_attention_forward.argtypes = [vp, heads, heads, heads, heads, vp, vp, i64, u32]
     L.sddmm_attention_backward.argtypes = [vp, heads, heads, heads, heads, vp, heads, heads, heads, heads, vp, i64, u32]
     L.sddmm_attention_last_kernel.restype = C.c_char_p
@@ -365,33 +365,47 @@ class Handle:
             raise ValueError("one to four parts")
         x = parts[0].src
         (n, _, d), dtype, device = x.shape, x.dtype, self.device
+        code, at, first = _dtype(dtype), 0, 0
+        if isinstance(positions, int):
+            first = positions
+        else:
+            at = self._int64_vector(positions, "positions", n)
+        pack, to_buffer, last, last_at = _ROTARY_PART.pack_into, self._rotary_parts, None, 0
         for i, p in enumerate(parts):
             src, dst, rows = p.src, p.dst, p.rows
-            shape, to = src.shape, dst.shape
-            a, b = src.stride(), dst.stride()
-            if len(shape) != 3 or len(to) != 3 or shape[2] != d or shape[1:] != to[1:] or src.dtype != dtype or dst.dtype != dtype or \
-                    d > 1 and (a[2] != 1 or b[2] != 1) or src.get_device() != device or dst.get_device() != device:
+            try:
+                src_rows, heads, width = src.shape
+                dst_rows, dst_heads, dst_width = dst.shape
+                a0, a1, a2 = src.stride()
+                b0, b1, b2 = dst.stride()
+            except ValueError:
+                raise ValueError(f"part {i} must be tensors (rows, heads, head_dim)") from None
+            if width != d or dst_width != d or heads != dst_heads or src.dtype is not dtype or dst.dtype is not dtype or \
+                    d > 1 and (a2 != 1 or b2 != 1) or src.get_device() != device or dst.get_device() != device:
                 raise ValueError(f"part {i} must be tensors (rows, heads, {d}) of {dtype} on cuda:{device} with contiguous heads")
-            if shape[0] != n or rows is None and to[0] != n:
+            if src_rows != n or rows is None and dst_rows != n:
                 raise ValueError(f"part {i} has other rows than the first")
-            if rows is not None:
-                rows = self._int64_vector(rows, "rows", n)
-            _ROTARY_PART.pack_into(self._rotary_parts, i * _ROTARY_PART.size, src.data_ptr(), dst.data_ptr(), a[0], a[1], b[0], b[1],
-                                   shape[1], p.rotate, rows or 0, to[0])
+            if rows is not last:
+                last, last_at = rows, 0 if rows is None else self._int64_vector(rows, "rows", n)
+            pack(to_buffer, 72 * i, src.data_ptr(), dst.data_ptr(), a0, a1, b0, b1, heads, p.rotate, last_at, dst_rows)
+        if layout not in _LAYOUTS:
+            raise ValueError(f"layout {layout!r}: half or interleaved")
         f = frequencies
         if type(f) is not np.ndarray or f.dtype != np.float64 or not f.flags.c_contiguous:
             f = np.ascontiguousarray(f, np.float64)
-        first, at = (positions, 0) if isinstance(positions, int) else (0, self._int64_vector(positions, "positions", n))
-        _ROTARY_DESC.pack_into(self._rotary_desc, 0, _dtype(dtype), d, 2 * f.shape[0], ("half", "interleaved").index(layout), n, at,
-                               first, f.__array_interface__["data"][0], magnitude, inverse)
+        _ROTARY_DESC.pack_into(self._rotary_desc, 0, code, d, 2 * f.shape[0], _LAYOUTS[layout], n, at, first,
+                               f.__array_interface__["data"][0], magnitude, inverse)
         self._follow_torch_stream(x)
-        st = lib().sddmm_rotary(self._h, self._rotary_desc, self._rotary_parts, count, flags)
+        st = _lib.sddmm_rotary(self._h, self._rotary_desc, to_buffer, count, flags)
         if st:
             self._check(st)
 
     def _int64_vector(self, a, name, n):
-        import torch
-        if getattr(a, "dtype", None) is not torch.int64 or a.shape != (n,) or not a.is_contiguous() or a.get_device() != self.device:
+        global _int64
+        if _int64 is None:
+            import torch
+            _int64 = torch.int64
+        if getattr(a, "dtype", None) is not _int64 or a.shape != (n,) or not a.is_contiguous() or a.get_device() != self.device:
             raise ValueError(f"{name} must be a contiguous int64 tensor of {n} values on cuda:{self.device}")
         return a.data_ptr()
 
@@ -457,6 +471,9 @@ class Attention:
             self._bytes.append(n.value)
         d = desc
         self._shape_q, self._shape_k = (d.q_rows, d.q_heads, d.head_dim), (d.k_rows, d.kv_heads, d.head_dim)
+        self._device = handle.device
+        self._arrays = C.create_string_buffer(8 * _HEADS.size)  # descriptions of a call's arrays: a handle is one thread's at a time
+        self._at = C.addressof(self._arrays)
 
     def close(self):
         if self._a:
@@ -469,16 +486,19 @@ class Attention:
         except Exception:
             pass
 
-    def _heads(self, t, shape, name):
-        if t.shape != shape or t.dtype != self._dtype or t.stride(2) != 1 and t.shape[2] > 1 or t.get_device() != self.handle.device:
-            raise ValueError(f"{name} must be a tensor {tuple(shape)} of {self._dtype} on cuda:{self.handle.device} with contiguous heads, "
+    def _heads(self, i, t, shape, name):
+        """Address of the description of an array, the i-th of the call."""
+        a, b, c = t.stride()
+        if t.shape != shape or t.dtype is not self._dtype or c != 1 and shape[2] > 1 or t.get_device() != self._device:
+            raise ValueError(f"{name} must be a tensor {tuple(shape)} of {self._dtype} on cuda:{self._device} with contiguous heads, "
                              f"got {tuple(t.shape)} of {t.dtype} on {t.device}, strides {t.stride()}")
-        return HeadArray(t.data_ptr(), t.stride(0), t.stride(1))
+        _HEADS.pack_into(self._arrays, 24 * i, t.data_ptr(), a, b)
+        return self._at + 24 * i
 
     def _lse(self, lse):
-        if lse.shape != (self.desc.q_heads, self.desc.q_rows) or str(lse.dtype) != "torch.float32" or not lse.is_contiguous() or \
-                lse.get_device() != self.handle.device:
-            raise ValueError(f"lse must be a contiguous float32 tensor {(self.desc.q_heads, self.desc.q_rows)} on cuda:{self.handle.device}")
+        if lse.shape != (self.desc.q_heads, self.desc.q_rows) or lse.element_size() != 4 or not lse.is_floating_point() or not lse.is_contiguous() or \
+                lse.get_device() != self._device:
+            raise ValueError(f"lse must be a contiguous float32 tensor {(self.desc.q_heads, self.desc.q_rows)} on cuda:{self._device}")
         return lse.data_ptr()
 
     def _workspace(self, backward, like):
@@ -489,8 +509,8 @@ class Attention:
     def forward(self, Q, K, V, O, lse=None, flags=0):
         """O (and lse, heads x rows, natural log) of the whole batch; returns O."""
         h = self.handle
-        q, k, v, o = (self._heads(Q, self._shape_q, "Q"), self._heads(K, self._shape_k, "K"), self._heads(V, self._shape_k, "V"),
-                      self._heads(O, self._shape_q, "O"))
+        q, k = self._heads(0, Q, self._shape_q, "Q"), self._heads(1, K, self._shape_k, "K")
+        v, o = self._heads(2, V, self._shape_k, "V"), self._heads(3, O, self._shape_q, "O")
         l = None if lse is None else self._lse(lse)
         h._follow_torch_stream(Q)
         w = self._workspace(0, Q)
@@ -502,9 +522,9 @@ class Attention:
     def backward(self, Q, K, V, O, lse, dO, dQ, dK, dV, flags=0):
         """Gradients of sum(O * dO) into dQ, dK, dV; O and lse from forward()."""
         h = self.handle
-        arrays = [self._heads(t, s, n) for t, s, n in (
+        arrays = [self._heads(i, t, s, n) for i, (t, s, n) in enumerate((
             (Q, self._shape_q, "Q"), (K, self._shape_k, "K"), (V, self._shape_k, "V"), (O, self._shape_q, "O"), (dO, self._shape_q, "dO"),
-            (dQ, self._shape_q, "dQ"), (dK, self._shape_k, "dK"), (dV, self._shape_k, "dV"))]
+            (dQ, self._shape_q, "dQ"), (dK, self._shape_k, "dK"), (dV, self._shape_k, "dV")))]
         l = self._lse(lse)
         h._follow_torch_stream(Q)
         w = self._workspace(1, Q)

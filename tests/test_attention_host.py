@@ -54,7 +54,7 @@ def test_frequencies_refused(bad):
 def test_null_handles_are_refused():
     L = api.lib()
     out, n = C.c_void_p(), C.c_int64()
-    none = C.POINTER(api.HeadArray)()
+    none = None
     assert L.sddmm_attention_plan(None, None, C.byref(out)) == api.INVALID_ARG
     assert L.sddmm_attention_workspace(None, 0, C.byref(n)) == api.INVALID_ARG
     assert L.sddmm_attention_forward(None, none, none, none, none, None, None, 0, 0) == api.INVALID_ARG

@@ -1,5 +1,7 @@
 """Attention under described masks on the GPU against its definition in 64 bits (tests/attention_helpers.py)."""
+import ctypes as C
 import math
+import struct
 
 import pytest
 import torch
@@ -50,6 +52,10 @@ def _check_backward(engine, p):
     plan.backward(p.Q, p.K, p.V, O, l, p.dO, *again)
     assert all(torch.equal(a[u], b[u]) for a, b, u in zip(again, (dQ, dK, dV), (used_q, used_k, used_k)))
     return plan
+
+
+def _array(address, row_stride, head_stride):
+    return C.create_string_buffer(struct.pack("@Pqq", address, row_stride, head_stride))   # sddmm_head_array
 
 
 MASKS = [dict(), dict(window=(-1, 0)), dict(window=(37, 0)), dict(window=(20, 50), prefix=9), dict(window=(-1, 0), prefix=70, cap=5.0),
@@ -363,16 +369,16 @@ def test_refusals(engine):
     with pytest.raises(ValueError):
         plan.forward(p.Q, p.K, p.V, O, torch.empty((4, 8), device="cuda"))
     # at the C entry: host memory, no workspace, unknown flags
-    q = api.HeadArray(p.Q.data_ptr(), p.Q.stride(0), p.Q.stride(1))
-    k = api.HeadArray(p.K.data_ptr(), p.K.stride(0), p.K.stride(1))
-    o = api.HeadArray(O.data_ptr(), O.stride(0), O.stride(1))
+    q = _array(p.Q.data_ptr(), p.Q.stride(0), p.Q.stride(1))
+    k = _array(p.K.data_ptr(), p.K.stride(0), p.K.stride(1))
+    o = _array(O.data_ptr(), O.stride(0), O.stride(1))
     l = torch.empty((4, 16), device="cuda")
     L = api.lib()
     host = torch.empty_like(p.Q, device="cpu")
-    bad = api.HeadArray(host.data_ptr(), p.Q.stride(0), p.Q.stride(1))
-    odd = api.HeadArray(p.Q.data_ptr() + 1, p.Q.stride(0), p.Q.stride(1))
-    back = api.HeadArray(p.Q.data_ptr(), -p.Q.stride(0), p.Q.stride(1))
-    tight = api.HeadArray(O.data_ptr(), 64, 32)
+    bad = _array(host.data_ptr(), p.Q.stride(0), p.Q.stride(1))
+    odd = _array(p.Q.data_ptr() + 1, p.Q.stride(0), p.Q.stride(1))
+    back = _array(p.Q.data_ptr(), -p.Q.stride(0), p.Q.stride(1))
+    tight = _array(O.data_ptr(), 64, 32)
     for args in [(bad, k, k, o), (odd, k, k, o), (back, k, k, o), (q, k, k, tight)]:
         assert L.sddmm_attention_forward(plan._a, *args, None, None, 0, 0) == api.INVALID_ARG
     assert L.sddmm_attention_forward(plan._a, q, k, k, o, None, None, 0, 2) == api.INVALID_ARG
