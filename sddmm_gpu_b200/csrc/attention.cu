@@ -14,7 +14,8 @@
 struct sddmm_attention_s {
     sddmm_handle_s *h = nullptr;
     AttentionParams p{};
-    FewPlan few{};
+    ForwardPlan few{}, prompt{};  // of which the quicker one is taken
+    bool by_few = false;
     Parts parts = ONE_PART;
     const char *last_kernel = "none";
 };
@@ -133,7 +134,11 @@ int sddmm_attention_plan(sddmm_handle_t h, const sddmm_attention_desc *d, sddmm_
     if (!a) return SDDMM_OUT_OF_MEMORY;
     a->h = h;
     a->p = p;
-    a->few = plan_attention_few(p, h->sm_count);
+    if (p.dtype != SDDMM_F32) {
+        a->few = plan_attention_few_tc(p, h->sm_count);
+        a->prompt = plan_attention_forward_tc(p, h->sm_count);
+        a->by_few = a->few.n_splits > 0 && a->few.us < a->prompt.us;
+    }
     a->parts = p.dtype == SDDMM_F32 ? plan_attention_parts(p, 64, 4, h->sm_count) : plan_attention_parts(p, 128, 1, h->sm_count);
     *out = a;
     return SDDMM_OK;
@@ -148,7 +153,7 @@ int sddmm_attention_destroy(sddmm_attention_t a)
 int sddmm_attention_workspace(sddmm_attention_t a, int backward, int64_t *bytes)
 {
     if (!a || !bytes) return SDDMM_INVALID_ARG;
-    *bytes = backward ? delta_bytes(a->p) + a->parts.bytes : a->few.bytes;
+    *bytes = backward ? delta_bytes(a->p) + a->parts.bytes : a->by_few ? a->few.bytes : a->prompt.bytes;
     return SDDMM_OK;
 }
 
@@ -173,11 +178,12 @@ int sddmm_attention_forward(sddmm_attention_t a, const sddmm_head_array *Q, cons
         return bad(h, "workspace: sddmm_attention_workspace() bytes of device memory, 16-byte aligned");
     if (!(flags & SDDMM_FLAG_ASYNC) && capturing(h->stream)) return bad(h, "a captured call must be asynchronous");
     if (p.n_seqs == 0 || p.max_q == 0) return SDDMM_OK;
-    bool taken = false;
-    cudaError_t e = launch_attention_few_tc(p, a->few, workspace, &taken, h->stream);
-    if (taken) return finish(a, e, "attention_few_tc", a->few.n_splits > 1 ? 2 : 1, flags);
-    e = launch_attention_forward_tc(p, &taken, h->stream);
-    if (taken) return finish(a, e, "attention_tc", 1, flags);
+    if (p.dtype != SDDMM_F32) {
+        bool taken = false;
+        const ForwardPlan &f = a->by_few ? a->few : a->prompt;
+        const cudaError_t e = a->by_few ? launch_attention_few_tc(p, f, workspace, &taken, h->stream) : launch_attention_forward_tc(p, f, workspace, &taken, h->stream);
+        if (taken) return finish(a, e, a->by_few ? "attention_few_tc" : "attention_tc", f.n_splits > 1 ? 2 : 1, flags);
+    }
     return finish(a, launch_attention_forward_general(p, h->stream), "attention_general", 1, flags);
 }
 

@@ -100,16 +100,20 @@ __device__ __forceinline__ bool find_block(const AttentionParams &p, int index, 
     }
     return false;
 }
-// Few queries of many keys: how the keys are cut, 0 splits where another kernel is to be taken; workspace bytes.
-constexpr int MOST_FEW_ROWS = 64;
-struct FewPlan {
+// How a forward kernel cuts the keys (n_splits 1: not, 0: it does not take the call), bytes of the parts, and about how long it takes.
+struct ForwardPlan {
     int n_splits, chunk_tiles;
     int64_t bytes;
+    double us;
 };
-FewPlan plan_attention_few(const AttentionParams &p, int sm_count);
-cudaError_t launch_attention_few_tc(const AttentionParams &p, const FewPlan &f, void *workspace, bool *taken, cudaStream_t s);
-// On the tensor cores; *taken false, and nothing launched, where the call's type, strides or alignment do not allow it.
-cudaError_t launch_attention_forward_tc(const AttentionParams &p, bool *taken, cudaStream_t s);
+ForwardPlan plan_attention_few_tc(const AttentionParams &p, int sm_count);
+ForwardPlan plan_attention_forward_tc(const AttentionParams &p, int sm_count);
+// *taken false, and nothing launched, where the call's type, strides or alignment do not allow the kernel.
+cudaError_t launch_attention_few_tc(const AttentionParams &p, const ForwardPlan &f, void *workspace, bool *taken, cudaStream_t s);
+cudaError_t launch_attention_forward_tc(const AttentionParams &p, const ForwardPlan &f, void *workspace, bool *taken, cudaStream_t s);
+// Adds up the parts of the prompt kernel, whose blocks have 256 queries and go through tiles of 128 keys.
+constexpr int PROMPT_QUERIES = 256, PROMPT_KEYS = 128;
+cudaError_t launch_attention_join(const AttentionParams &p, cudaStream_t s);
 cudaError_t launch_attention_forward_general(const AttentionParams &p, cudaStream_t s);
 // Where the blocks of a backward kernel alone would leave multiprocessors idle, the tiles that a block goes through are cut into parts, a
 // block each, which leave their sums in the workspace (parts x rows x heads x head_dim, dK and dV behind one another) for

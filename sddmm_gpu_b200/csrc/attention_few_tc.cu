@@ -7,6 +7,7 @@
 // its own in shared memory (16-byte asynchronous copies, zeros behind the sequence's end, three stages), keeps maximum, sum and
 // output in registers, and waits for no other warp before the end.  The warps' parts are added in order; where a sequence has several
 // chunks the parts go to the workspace and a second kernel, a block for each row, adds them in order.  Nothing depends on scheduling.
+#include <cmath>
 #include <type_traits>
 
 #include "attention_strict.cuh"
@@ -70,7 +71,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident_blocks(DP)) attention_few
 {
     constexpr int ROW_BYTES = DP * 2, PIECES = DP / 8, TILE_BYTES = KEYS * ROW_BYTES, STAGE_BYTES = 2 * TILE_BYTES;
     extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ float w_most[WARPS][ROWS], w_sum[WARPS][ROWS], r_lse[ROWS];
+    __shared__ float w_most[WARPS][ROWS], w_sum[WARPS][ROWS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // first chunks first: those that a short sequence does not have come last
     const unsigned heads_and_rows = gridDim.x / p.n_splits, b = blockIdx.x % heads_and_rows, chunk = blockIdx.x / heads_and_rows;
@@ -274,7 +275,8 @@ __global__ void __launch_bounds__(WARPS * 32, resident_blocks(DP)) attention_few
 
 // The parts of one row added up, a block for a row: warps take chunks in turn, eight at once, so that all of a row's parts are asked for
 // before the first is used.
-template <class E>
+// TILES: of the tensor-core prompt kernel (parts of the keys of 256 queries), else of the kernel above (of 16 rows).
+template <class E, bool TILES>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionParams p)
 {
     constexpr int JOIN_WARPS = 8, AT_ONCE = 8;
@@ -283,8 +285,14 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
     const int head = blockIdx.x % p.q_heads, i = blockIdx.x / p.q_heads % p.max_q, seq = blockIdx.x / p.q_heads / p.max_q;
     const Sequence s = sequence_of(p, seq);
     if (i >= s.nq) return;
-    const int n = chunks_of(p, s, (i * p.group + head % p.group) / ROWS).n;
-    if (n == 1) return;
+    int n;
+    if (TILES) {
+        const int i0 = i / PROMPT_QUERIES * PROMPT_QUERIES;
+        n = (key_tiles<PROMPT_KEYS>(reach_of(p.window, s, i0, min(s.nq, i0 + PROMPT_QUERIES))).n + p.chunk_tiles - 1) / p.chunk_tiles;
+    } else {
+        n = chunks_of(p, s, (i * p.group + head % p.group) / ROWS).n;
+    }
+    if (n <= 1) return;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // this grid may have been started before the parts were written
     const int64_t stride = (int64_t)p.q_rows * p.q_heads, at = ((int64_t)s.q0 + i) * p.q_heads + head;
     float y[4] = {}, top = -INFINITY, total = 0.f;
@@ -345,6 +353,21 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
     }
 }
 
+template <class E, bool TILES>
+cudaError_t launch_join(const AttentionParams &p, cudaStream_t s)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)((int64_t)p.n_seqs * p.max_q * p.q_heads));
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute early{};  // (24 tokens: 37 us without, 33 with)
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attention_join_kernel<E, TILES>, p);
+}
+
 template <class E, int DP, bool CAP, bool BIAS>
 cudaError_t launch(const AttentionParams &p, cudaStream_t s)
 {
@@ -358,16 +381,7 @@ cudaError_t launch(const AttentionParams &p, cudaStream_t s)
     attention_few_kernel<E, DP, CAP, BIAS><<<grid, WARPS * 32, smem, s>>>(p, row_tiles);
     e = cudaGetLastError();
     if (e != cudaSuccess || p.n_splits == 1) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)((int64_t)p.n_seqs * p.max_q * p.q_heads));
-    cfg.blockDim = dim3(256);
-    cfg.stream = s;
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &early;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_join_kernel<E>, p);
+    return launch_join<E, false>(p, s);
 }
 template <class E, int DP>
 cudaError_t by_score(const AttentionParams &p, cudaStream_t s)
@@ -380,10 +394,10 @@ bool wide(const HeadArray &a) { return (uintptr_t)a.data % 16 == 0 && a.row % 8 
 
 }  // namespace
 
-FewPlan plan_attention_few(const AttentionParams &p, int sm_count)
+ForwardPlan plan_attention_few_tc(const AttentionParams &p, int sm_count)
 {
-    FewPlan f{0, 0, 0};
-    if (p.dtype == 0 || (int64_t)p.max_q * p.group > MOST_FEW_ROWS || p.max_q == 0 || p.n_seqs == 0) return f;
+    ForwardPlan f{0, 1, 0, INFINITY};
+    if (p.dtype == 0 || p.max_q == 0 || p.n_seqs == 0) return f;
     const int64_t row_tiles = (p.max_q * p.group + ROWS - 1) / ROWS, blocks = row_tiles * p.kv_heads * p.n_seqs;
     const int64_t tiles = (p.max_k + KEYS - 1) / KEYS + 1;  // (+ 1: prefix and window may begin inside tiles)
     auto bytes_of = [&](int64_t n) { return n == 1 ? 0 : n * p.q_rows * p.q_heads * (int64_t)(p.head_dim + 1) * 4; };
@@ -400,10 +414,20 @@ FewPlan plan_attention_few(const AttentionParams &p, int sm_count)
     f.chunk_tiles = (int)chunk;
     f.n_splits = (int)n;
     f.bytes = bytes_of(n);
+    // (8 us, and 0.19 for 16 rows x 16 keys on a multiprocessor, however many warps it has; 6 more with a join.  Rows of the sequences, not of
+    // the longest)
+    const int64_t most_rows = (int64_t)p.n_seqs * row_tiles, rows = p.q_rows * p.group / ROWS + p.n_seqs < most_rows ? p.q_rows * p.group / ROWS + p.n_seqs : most_rows;
+    const double units = (double)rows * p.kv_heads * tiles;
+    f.us = 8. + 0.19 * units / sm_count + (n > 1 ? 6. : 0.);
     return f;
 }
 
-cudaError_t launch_attention_few_tc(const AttentionParams &p0, const FewPlan &f, void *workspace, bool *taken, cudaStream_t s)
+cudaError_t launch_attention_join(const AttentionParams &p, cudaStream_t s)
+{
+    return p.dtype == 1 ? launch_join<__half, true>(p, s) : launch_join<__nv_bfloat16, true>(p, s);
+}
+
+cudaError_t launch_attention_few_tc(const AttentionParams &p0, const ForwardPlan &f, void *workspace, bool *taken, cudaStream_t s)
 {
     *taken = f.n_splits > 0 && wide(p0.q) && wide(p0.k) && wide(p0.v) && wide(p0.o);
     if (!*taken) return cudaSuccess;

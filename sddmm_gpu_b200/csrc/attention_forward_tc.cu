@@ -38,6 +38,7 @@ constexpr int T = 128;  // queries of a tile
 constexpr int KT = 128;  // keys of a tile
 constexpr int SOFTMAX_WARPS = 16, MMA_WARP = 16, LOAD_WARP = 17, THREADS = 640;
 constexpr int COLUMNS = KT / 2;  // of a thread
+static_assert(2 * T == PROMPT_QUERIES && KT == PROMPT_KEYS, "the join goes by these");
 constexpr uint32_t TMEM_COLUMNS = 512, O_COLUMN = 256;  // S at 0 and 128
 constexpr float RAISE = 8.f;
 // Registers of a thread: 96 at launch (640 threads), shared out anew: 4 x 104 + 64 = 5 x 96.
@@ -69,7 +70,8 @@ __device__ __forceinline__ bool tile_all(int tile, bool mine)
     return r != 0;
 }
 
-template <class E, int DP, bool CAP, bool BIAS>
+// PARTS: the keys of a block may be cut (a form of its own: what it has to remember cost the other 8 % in registers)
+template <class E, int DP, bool CAP, bool BIAS, bool PARTS>
 __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const AttentionParams p, const __grid_constant__ Maps maps)
 {
     using Sh = Shape<DP>;
@@ -84,13 +86,22 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
     __shared__ uint32_t tmem_holder, bad[8];
     __shared__ float row_most[2][2][2][T], row_sum[2][2][T], row_lse[2 * T];  // [step parity][tile][half]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int head = blockIdx.x % p.q_heads, kv = head / p.group;
+    const unsigned splits = PARTS ? p.n_splits : 1, blocks = gridDim.x / splits, block_of = blockIdx.x / splits, part = PARTS ? blockIdx.x % splits : 0;
+    const int head = block_of % p.q_heads, kv = head / p.group;
     Sequence s;
     int seq, block;
     // the last blocks of a causal sequence have the most keys: they go first
-    if (!find_block<2 * T>(p, (gridDim.x - 1 - blockIdx.x) / p.q_heads, false, s, seq, block)) return;
+    if (!find_block<2 * T>(p, (blocks - 1 - block_of) / p.q_heads, false, s, seq, block)) return;
     const int i0 = block * 2 * T;
-    const KeyTiles all = key_tiles<KT>(reach_of(p.window, s, i0, min(s.nq, i0 + 2 * T)));
+    const KeyTiles of_block = key_tiles<KT>(reach_of(p.window, s, i0, min(s.nq, i0 + 2 * T)));
+    // a part of them where the blocks alone would leave multiprocessors idle: parts are joined as those of few queries are
+    const Part mine_of = PARTS ? part_of(p, of_block.n, part) : Part{0, of_block.n, true};
+    if (mine_of.end < 0) return;
+    struct {
+        KeyTiles keys;
+        int first, n;
+        __device__ __forceinline__ int tile(int u) const { return keys.tile(PARTS ? first + u : u); }
+    } const all{of_block, mine_of.first, mine_of.end - mine_of.first};
     Reach reach[2];
     bool there[2];
 #pragma unroll
@@ -412,14 +423,26 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                     o[j] = n_s > 0 ? o[j] * inv : 0.f;
                     zero = fmaf(o[j], 0.f, zero);
                 }
-                tc::stage_32<E, DP / 2>(stage, 32 * b, o);
+                if (!PARTS || mine_of.alone) {
+                    tc::stage_32<E, DP / 2>(stage, 32 * b, o);
+                } else if (i < s.nq) {
+                    const int first = half * (DP / 2) + 32 * b;
+                    float *to = p.part_o + ((part * p.q_rows + s.q0 + i) * p.q_heads + head) * p.head_dim + first;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        if (first + j < p.head_dim) *reinterpret_cast<float4 *>(to + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                }
             }
             const int row0 = i - lane;
-            tc::store_staged<E, DP / 2>(stage, static_cast<E *>(p.o.data) + ((int64_t)s.q0 + row0) * p.o.row + head * p.o.head + half * (DP / 2), p.o.row, s.nq - row0,
+            if (!PARTS || mine_of.alone)
+                tc::store_staged<E, DP / 2>(stage, static_cast<E *>(p.o.data) + ((int64_t)s.q0 + row0) * p.o.row + head * p.o.head + half * (DP / 2), p.o.row, s.nq - row0,
                                         p.head_dim - half * (DP / 2));
-            if (p.lse && half == 0 && i < s.nq) p.lse[(int64_t)head * p.q_rows + s.q0 + i] = lse;
+            if (half == 0 && i < s.nq) {
+                if (PARTS && !mine_of.alone) p.part_lse[(part * p.q_rows + s.q0 + i) * p.q_heads + head] = sum == 0.f ? -INFINITY : most + log2f(sum);
+                else if (p.lse) p.lse[(int64_t)head * p.q_rows + s.q0 + i] = lse;
+            }
             if (half == 0) row_lse[t * T + row] = lse;
-            const unsigned rows = __ballot_sync(0xffffffffu, zero != 0.f && i < s.nq);
+            const unsigned rows = __ballot_sync(0xffffffffu, zero != 0.f && i < s.nq && (!PARTS || mine_of.alone));
             if (lane == 0 && rows) atomicOr(&bad[t * 4 + (warp & 3)], rows);
         }
     }
@@ -436,17 +459,22 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                 }
 }
 
-template <class E, int DP, bool CAP, bool BIAS>
+template <class E, int DP, bool CAP, bool BIAS, bool PARTS>
 cudaError_t launch(const AttentionParams &p, const Maps &maps, cudaStream_t s)
 {
     constexpr size_t smem = Shape<DP>::SMEM;
     static SmemOptinCache optin;
-    const cudaError_t e = optin_dynamic_smem(attention_forward_tc_kernel<E, DP, CAP, BIAS>, smem, optin);
+    const cudaError_t e = optin_dynamic_smem(attention_forward_tc_kernel<E, DP, CAP, BIAS, PARTS>, smem, optin);
     if (e != cudaSuccess) return e;
     const unsigned grid = (unsigned)(p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, 2 * T));
     if (grid == 0) return cudaSuccess;
-    attention_forward_tc_kernel<E, DP, CAP, BIAS><<<grid, THREADS, smem, s>>>(p, maps);
+    attention_forward_tc_kernel<E, DP, CAP, BIAS, PARTS><<<grid * p.n_splits, THREADS, smem, s>>>(p, maps);
     return cudaGetLastError();
+}
+template <class E, int DP, bool CAP, bool BIAS>
+cudaError_t launch(const AttentionParams &p, const Maps &maps, cudaStream_t s)
+{
+    return p.n_splits > 1 ? launch<E, DP, CAP, BIAS, true>(p, maps, s) : launch<E, DP, CAP, BIAS, false>(p, maps, s);
 }
 template <class E, int DP>
 cudaError_t by_score(const AttentionParams &p, const Maps &maps, cudaStream_t s)
@@ -463,15 +491,42 @@ bool attention_forward_tc_takes(const AttentionParams &p)
     return p.dtype != 0 && (uintptr_t)p.o.data % 16 == 0 && p.o.row % 8 == 0 && p.o.head % 8 == 0 && p.k_rows > 0;
 }
 
-cudaError_t launch_attention_forward_tc(const AttentionParams &p, bool *taken, cudaStream_t s)
+ForwardPlan plan_attention_forward_tc(const AttentionParams &p, int sm_count)
+{
+    // Parts until there is a block for every multiprocessor, of two tiles of keys at least, and at most 256 MB of them.
+    const int64_t blocks = p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, 2 * T), tiles = (p.max_k + KT - 1) / KT;
+    const int64_t bytes = p.q_rows * p.q_heads * (int64_t)(p.head_dim + 1) * 4;
+    ForwardPlan f{1, (int)(tiles > 0 ? tiles : 1), 0, 0.};
+    int64_t want = blocks > 0 ? sm_count / blocks : 1;
+    if (want > tiles / 2) want = tiles / 2;
+    if (bytes > 0 && want > (256ll << 20) / bytes) want = (256ll << 20) / bytes;
+    if (want > 1 && (int64_t)p.n_seqs * p.max_q * p.q_heads <= INT32_MAX) {
+        f.chunk_tiles = (int)((tiles + want - 1) / want);
+        f.n_splits = (int)((tiles + f.chunk_tiles - 1) / f.chunk_tiles);
+        f.bytes = f.n_splits > 1 ? f.n_splits * bytes : 0;
+    }
+    // (8 us and 2.0 a tile of 256 x 128 for every wave of blocks; 6 more with a join, most of it the second launch)
+    const int64_t waves = (blocks * f.n_splits + sm_count - 1) / sm_count;
+    f.us = 8. + 2.0 * (double)waves * f.chunk_tiles + (f.n_splits > 1 ? 6. : 0.);
+    return f;
+}
+
+cudaError_t launch_attention_forward_tc(const AttentionParams &p0, const ForwardPlan &f, void *workspace, bool *taken, cudaStream_t s)
 {
     Maps maps;
+    AttentionParams p = p0;
+    p.n_splits = f.n_splits;
+    p.chunk_tiles = f.chunk_tiles;
+    p.part_o = static_cast<float *>(workspace);
+    p.part_lse = p.part_o + (f.n_splits == 1 ? 0 : (int64_t)f.n_splits * p.q_rows * p.q_heads * p.head_dim);
     *taken = attention_forward_tc_takes(p) && make_tensor_map(&maps.q, p.q, p.dtype, p.head_dim, p.q_heads, p.q_rows, T) &&
              make_tensor_map(&maps.k, p.k, p.dtype, p.head_dim, p.kv_heads, p.k_rows, KT) &&
              make_tensor_map(&maps.v, p.v, p.dtype, p.head_dim, p.kv_heads, p.k_rows, KT);
     if (!*taken) return cudaSuccess;
-    if (p.dtype == 1) return p.head_dim <= 64 ? by_score<__half, 64>(p, maps, s) : by_score<__half, 128>(p, maps, s);
-    return p.head_dim <= 64 ? by_score<__nv_bfloat16, 64>(p, maps, s) : by_score<__nv_bfloat16, 128>(p, maps, s);
+    cudaError_t e;
+    if (p.dtype == 1) e = p.head_dim <= 64 ? by_score<__half, 64>(p, maps, s) : by_score<__half, 128>(p, maps, s);
+    else e = p.head_dim <= 64 ? by_score<__nv_bfloat16, 64>(p, maps, s) : by_score<__nv_bfloat16, 128>(p, maps, s);
+    return e == cudaSuccess && p.n_splits > 1 ? launch_attention_join(p, s) : e;
 }
 
 }  // namespace sddmm
