@@ -15,7 +15,7 @@ struct sddmm_attention_s {
     sddmm_handle_s *h = nullptr;
     AttentionParams p{};
     ForwardPlan few{}, prompt{};  // of which the quicker one is taken
-    bool by_few = false;
+    bool by_few = false, tensor_cores = false;
     Parts parts = ONE_PART;
     const char *last_kernel = "none";
 };
@@ -134,7 +134,9 @@ int sddmm_attention_plan(sddmm_handle_t h, const sddmm_attention_desc *d, sddmm_
     if (!a) return SDDMM_OUT_OF_MEMORY;
     a->h = h;
     a->p = p;
-    if (p.dtype != SDDMM_F32) {
+    // (a cap beyond a million times the scale: its tanh is left to the general kernels' own)
+    a->tensor_cores = p.dtype != SDDMM_F32 && (p.cap == 0.f || p.scale / p.cap >= 1e-6f);
+    if (a->tensor_cores) {
         a->few = plan_attention_few_tc(p, h->sm_count);
         a->prompt = plan_attention_forward_tc(p, h->sm_count);
         a->by_few = a->few.n_splits > 0 && a->few.us < a->prompt.us;
@@ -178,7 +180,7 @@ int sddmm_attention_forward(sddmm_attention_t a, const sddmm_head_array *Q, cons
         return bad(h, "workspace: sddmm_attention_workspace() bytes of device memory, 16-byte aligned");
     if (!(flags & SDDMM_FLAG_ASYNC) && capturing(h->stream)) return bad(h, "a captured call must be asynchronous");
     if (p.n_seqs == 0 || p.max_q == 0) return SDDMM_OK;
-    if (p.dtype != SDDMM_F32) {
+    if (a->tensor_cores) {
         bool taken = false;
         const ForwardPlan &f = a->by_few ? a->few : a->prompt;
         const cudaError_t e = a->by_few ? launch_attention_few_tc(p, f, workspace, &taken, h->stream) : launch_attention_forward_tc(p, f, workspace, &taken, h->stream);
@@ -218,9 +220,9 @@ int sddmm_attention_backward(sddmm_attention_t a, const sddmm_head_array *Q, con
     if (p.n_seqs == 0 || (p.max_q == 0 && p.max_k == 0)) return SDDMM_OK;
     bool taken = false;
     const int launches = 2 + (a->parts.n_q > 1) + (a->parts.n_kv > 1);
-    const cudaError_t e = launch_attention_backward_tc(p, a->parts, &taken, h->stream);
+    const cudaError_t e = a->tensor_cores ? launch_attention_backward_tc(p, a->parts, &taken, h->stream) : cudaSuccess;
     if (taken) return finish(a, e, "attention_backward_tc", launches, flags);
-    // (16-bit types come to the general kernel for their strides or alignment alone)
+    // (16-bit types come to the general kernels for their strides or alignment alone)
     if (p.dtype == SDDMM_F32) return finish(a, launch_attention_backward_general(p, a->parts, h->stream), "attention_backward_general", launches, flags);
     return finish(a, launch_attention_backward_general(p, ONE_PART, h->stream), "attention_backward_general", 2, flags);
 }

@@ -73,30 +73,43 @@ __device__ __forceinline__ bool find_block(const AttentionParams &p, int index, 
 {
     const int lane = threadIdx.x & 31;
     int before = 0;
-    for (int b0 = 0; b0 < p.n_seqs; b0 += 32) {
-        const int b = b0 + lane;
-        Sequence mine = {};
-        if (b < p.n_seqs) mine = sequence_of(p, b);
+    auto among = [&](const Sequence &mine, int b0) {  // the 32 sequences from b0 on, one a lane
         const int blocks = ((keys ? mine.nk : mine.nq) + T - 1) / T;
         int sum = blocks;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += x;
+            const int y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
         }
         const unsigned hit = __ballot_sync(0xffffffffu, index < before + sum);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            number = index - before - __shfl_sync(0xffffffffu, sum - blocks, l);
-            seq = b0 + l;
-            s.q0 = __shfl_sync(0xffffffffu, mine.q0, l);
-            s.nq = __shfl_sync(0xffffffffu, mine.nq, l);
-            s.k0 = __shfl_sync(0xffffffffu, mine.k0, l);
-            s.nk = __shfl_sync(0xffffffffu, mine.nk, l);
-            s.prefix = __shfl_sync(0xffffffffu, mine.prefix, l);
-            return true;
+        if (!hit) {
+            before += __shfl_sync(0xffffffffu, sum, 31);
+            return false;
         }
-        before += __shfl_sync(0xffffffffu, sum, 31);
+        const int l = __ffs(hit) - 1;
+        number = index - before - __shfl_sync(0xffffffffu, sum - blocks, l);
+        seq = b0 + l;
+        s.q0 = __shfl_sync(0xffffffffu, mine.q0, l);
+        s.nq = __shfl_sync(0xffffffffu, mine.nq, l);
+        s.k0 = __shfl_sync(0xffffffffu, mine.k0, l);
+        s.nk = __shfl_sync(0xffffffffu, mine.nk, l);
+        s.prefix = __shfl_sync(0xffffffffu, mine.prefix, l);
+        return true;
+    };
+    if (p.n_seqs <= 32) {
+        Sequence mine = {};
+        if (lane < p.n_seqs) mine = sequence_of(p, lane);
+        return among(mine, 0);
+    }
+    constexpr int AT_ONCE = 4;  // groups whose numbers are asked for together
+    for (int b0 = 0; b0 < p.n_seqs; b0 += 32 * AT_ONCE) {
+        Sequence of[AT_ONCE] = {};
+#pragma unroll
+        for (int x = 0; x < AT_ONCE; ++x)
+            if (b0 + 32 * x + lane < p.n_seqs) of[x] = sequence_of(p, b0 + 32 * x + lane);
+#pragma unroll
+        for (int x = 0; x < AT_ONCE; ++x)
+            if (among(of[x], b0 + 32 * x)) return true;
     }
     return false;
 }

@@ -130,7 +130,8 @@ __global__ void __launch_bounds__(WARPS * 32, resident_blocks(DP)) attention_few
         hi[x] = p.window.right < 0 ? s.nk - 1 : min(s.nk - 1, pos[x] + p.window.right);
         slope[x] = BIAS ? __ldg(p.slopes + head) * LOG2E : 0.f;
     }
-    const float c = CAP ? 2.f * LOG2E * p.scale / p.cap : p.scale * LOG2E, top_of = p.cap * LOG2E;
+    const float c = CAP ? p.scale / p.cap : p.scale * LOG2E, top_of = p.cap * LOG2E;
+    const tc::Tanh tanh_c = tc::tanh_polynomial(c, top_of);
     float o[DP / 8][4];
 #pragma unroll
     for (int d = 0; d < DP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
@@ -154,14 +155,25 @@ __global__ void __launch_bounds__(WARPS * 32, resident_blocks(DP)) attention_few
             }
         }
         const bool open = tile_is_open<KEYS>(p.window, s, ch.reach, j0);
+        if (CAP) {
+            float size = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) size = tc::max3_abs(size, x[0][e], x[1][e]);
+            if (__all_sync(0xffffffffu, size <= tanh_c.range)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) tc::split(tc::tanh2(tc::two(x[0][e], x[1][e]), tanh_c), x[0][e], x[1][e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e / 4][e % 4] = fmaf(-2.f * top_of, tc::rcp(1.f + tc::ex2(x[e / 4][e % 4] * (2.f * LOG2E * c))), top_of);
+            }
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int w = e >> 1, j = j0 + 8 * t + lane % 4 * 2 + (e & 1);
                 float z = x[t][e];
-                if (CAP) z = fmaf(-2.f * top_of, tc::rcp(1.f + tc::ex2(z * c)), top_of);
-                else z *= c;
+                if (!CAP) z *= c;
                 if (BIAS) z = fmaf(-slope[w], fabsf((float)(pos[w] - j)), z);
                 if (!open && !(j < s.prefix || (j >= lo[w] && j <= hi[w]))) z = -INFINITY;
                 x[t][e] = z;
@@ -284,16 +296,18 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.head_dim;
     const int head = blockIdx.x % p.q_heads, i = blockIdx.x / p.q_heads % p.max_q, seq = blockIdx.x / p.q_heads / p.max_q;
     const Sequence s = sequence_of(p, seq);
-    if (i >= s.nq) return;
-    int n;
-    if (TILES) {
+    int n = 0;
+    if (i >= s.nq) {
+    } else if (TILES) {
         const int i0 = i / PROMPT_QUERIES * PROMPT_QUERIES;
         n = (key_tiles<PROMPT_KEYS>(reach_of(p.window, s, i0, min(s.nq, i0 + PROMPT_QUERIES))).n + p.chunk_tiles - 1) / p.chunk_tiles;
     } else {
         n = chunks_of(p, s, (i * p.group + head % p.group) / ROWS).n;
     }
+    // This grid may have been started before the parts were written.  Every block waits, also one that has nothing to add: the grid must not end
+    // before the one that it stands behind.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (n <= 1) return;
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // this grid may have been started before the parts were written
     const int64_t stride = (int64_t)p.q_rows * p.q_heads, at = ((int64_t)s.q0 + i) * p.q_heads + head;
     float y[4] = {}, top = -INFINITY, total = 0.f;
     for (int c0 = warp; c0 < n; c0 += JOIN_WARPS * AT_ONCE) {
@@ -376,7 +390,7 @@ cudaError_t launch(const AttentionParams &p, cudaStream_t s)
     static SmemOptinCache optin;
     cudaError_t e = optin_dynamic_smem(attention_few_kernel<E, DP, CAP, BIAS>, smem, optin);
     if (e != cudaSuccess) return e;
-    const int row_tiles = (p.max_q * p.group + ROWS - 1) / ROWS;
+    const int row_tiles = (int)(((int64_t)p.max_q * p.group + ROWS - 1) / ROWS);
     const unsigned grid = (unsigned)((int64_t)p.n_seqs * p.kv_heads * row_tiles * p.n_splits);
     attention_few_kernel<E, DP, CAP, BIAS><<<grid, WARPS * 32, smem, s>>>(p, row_tiles);
     e = cudaGetLastError();
@@ -398,7 +412,8 @@ ForwardPlan plan_attention_few_tc(const AttentionParams &p, int sm_count)
 {
     ForwardPlan f{0, 1, 0, INFINITY};
     if (p.dtype == 0 || p.max_q == 0 || p.n_seqs == 0) return f;
-    const int64_t row_tiles = (p.max_q * p.group + ROWS - 1) / ROWS, blocks = row_tiles * p.kv_heads * p.n_seqs;
+    if ((int64_t)p.max_q * p.group > INT32_MAX) return f;
+    const int64_t row_tiles = ((int64_t)p.max_q * p.group + ROWS - 1) / ROWS, blocks = row_tiles * p.kv_heads * p.n_seqs;
     const int64_t tiles = (p.max_k + KEYS - 1) / KEYS + 1;  // (+ 1: prefix and window may begin inside tiles)
     auto bytes_of = [&](int64_t n) { return n == 1 ? 0 : n * p.q_rows * p.q_heads * (int64_t)(p.head_dim + 1) * 4; };
     auto n_of = [&](int64_t c) { return tiles <= c ? (int64_t)1 : (tiles + c - 1) / c; };

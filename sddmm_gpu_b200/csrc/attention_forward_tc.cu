@@ -77,9 +77,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
     using Sh = Shape<DP>;
     constexpr int BOXES = Sh::BOXES, Q_BYTES = Sh::Q_BYTES, TILE_BYTES = Sh::TILE_BYTES, Q_BOX = Sh::Q_BOX, BOX = Sh::BOX, STAGES = Sh::STAGES;
     constexpr bool BESIDE = Sh::BESIDE;
-    // Every eighth exponential without the special function unit.  Ragged prompts with a cap, heads of 128: 132 -> 113 us, two of
-    // eight 115; band, heads of 64: 41.9 -> 41.0; long prompt without a cap, heads of 128: 313 -> 317, so not there.
-    constexpr bool POLY = CAP || DP == 64;
+    // Every eighth exponential without the special function unit, where FMAs are to spare: band, heads of 64, 41.9 -> 41.0 us; long prompt,
+    // heads of 128, 313 -> 317; with a cap, whose tanh takes the FMAs, heads of 128, 108 -> 115.
+    constexpr bool POLY = DP == 64 && !CAP;
     constexpr bool BF16 = sizeof(E) == 2 && !std::is_same<E, __half>::value;
     extern __shared__ __align__(1024) unsigned char smem[];  // two tiles of Q, the rings of K and of V
     __shared__ uint64_t q_full, full[2][STAGES], empty[2][STAGES], s_full[2], s_read[2], p_ready[2], o_done[2], o_full, tail;  // [K, V], [tile of Q]
@@ -283,6 +283,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s_read[t]);  // the next scores may come
             }
+            // Without a bias the capped scores keep their order, so the row's maximum is found among the products, and tanh comes with the
+            // exponentials: its FMAs (1,500 clocks a tile) run beside their special function unit (1,000).
+            bool small = true;
             if (CAP) {
                 float size = 0.f;
 #pragma unroll
@@ -291,7 +294,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                     tc::split(x[j], a, b);
                     size = tc::max3_abs(size, a, b);
                 }
-                if (__all_sync(0xffffffffu, size <= tanh_c.range)) {
+                small = __all_sync(0xffffffffu, size <= tanh_c.range);
+            }
+            if (CAP && BIAS) {
+                if (small) {
 #pragma unroll
                     for (int j = 0; j < COLUMNS / 2; ++j) x[j] = tc::tanh2(x[j], tanh_c);
                 } else {
@@ -325,10 +331,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                     }
                 }
             }
-            if (!tile_is_open<COLUMNS>(p.window, s, reach[t], j0)) {
+            const bool open = tile_is_open<COLUMNS>(p.window, s, reach[t], j0);
+            unsigned seen_of[COLUMNS / 32];
+            if (!open) {
 #pragma unroll
                 for (int b = 0; b < COLUMNS / 32; ++b) {
-                    const unsigned seen = seen_bits(lo, hi, s.prefix, j0 + 32 * b);
+                    const unsigned seen = seen_of[b] = seen_bits(lo, hi, s.prefix, j0 + 32 * b);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         float a0, a1;
@@ -355,6 +363,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                 break;
             }
             now = fmaxf(now, row_most[n_s & 1][t][half ^ 1][row]);
+            if (CAP && !BIAS && now > -INFINITY) now = fmaf(-2.f * top_of, tc::rcp(1.f + tc::ex2(now * (2.f * LOG2E * c))), top_of);
             const bool raise = now > most + RAISE;  // (-inf + RAISE = -inf: any row's first)
             if (__any_sync(0xffffffffu, raise)) {
                 const float to = raise ? now : most;
@@ -380,15 +389,42 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
             const float less = most == -INFINITY ? 0.f : -most;
             F2 s2[2] = {0, 0};
             uint32_t w[COLUMNS / 2];
+            auto weigh = [&](auto all_seen, auto is_small) {
 #pragma unroll
-            for (int j = 0; j < COLUMNS / 2; ++j) {
-                const F2 e = CAP || BIAS ? tc::add2(x[j], tc::two(less, less)) : tc::ffma2(x[j], tc::two(c, c), tc::two(less, less));
-                float e0, e1;
-                tc::split(e, e0, e1);
-                if (POLY && j % 8 == 0) tc::split(tc::ex2_poly(e), e0, e1);
-                else e0 = tc::ex2(e0), e1 = tc::ex2(e1);
-                s2[j & 1] = tc::add2(s2[j & 1], tc::two(e0, e1));
-                w[j] = tc::pack<E>(e0, e1);
+                for (int j = 0; j < COLUMNS / 2; ++j) {
+                    F2 e;
+                    float e0, e1;
+                    if (CAP && !BIAS) {
+                        if (decltype(is_small)::value) {
+                            e = tc::ffma2(x[j], tc::tanh_over_x(x[j], tanh_c), tc::two(less, less));
+                        } else {  // cap tanh(y) = cap - 2 cap / (1 + e^2y)
+                            tc::split(x[j], e0, e1);
+                            e0 = fmaf(-2.f * top_of, tc::rcp(1.f + tc::ex2(e0 * (2.f * LOG2E * c))), top_of + less);
+                            e1 = fmaf(-2.f * top_of, tc::rcp(1.f + tc::ex2(e1 * (2.f * LOG2E * c))), top_of + less);
+                            e = tc::two(e0, e1);
+                        }
+                        if (!decltype(all_seen)::value) {
+                            tc::split(e, e0, e1);
+                            e = tc::two(seen_of[j / 16] & 1u << 2 * (j % 16) ? e0 : -INFINITY, seen_of[j / 16] & 2u << 2 * (j % 16) ? e1 : -INFINITY);
+                        }
+                    } else {
+                        e = BIAS ? tc::add2(x[j], tc::two(less, less)) : tc::ffma2(x[j], tc::two(c, c), tc::two(less, less));
+                    }
+                    if (POLY && j % 8 == 0) {
+                        tc::split(tc::ex2_poly(e), e0, e1);
+                    } else {
+                        tc::split(e, e0, e1);
+                        e0 = tc::ex2(e0), e1 = tc::ex2(e1);
+                    }
+                    s2[j & 1] = tc::add2(s2[j & 1], tc::two(e0, e1));
+                    w[j] = tc::pack<E>(e0, e1);
+                }
+            };
+            if (!CAP || BIAS || (open && small)) weigh(std::true_type(), std::true_type());
+            else if (small) weigh(std::false_type(), std::true_type());
+            else {
+                if (open) seen_of[0] = seen_of[1] = ~0u;
+                weigh(std::false_type(), std::false_type());
             }
             if (BESIDE && n_s > 0) ok = ok && tc::warp_wait(&o_done[t], (n_s - 1) & 1);  // the last weights have been used
             tc::tmem_st32(my_weights, w);

@@ -222,7 +222,8 @@ __device__ __forceinline__ F2 ex2_poly(F2 x)
     return mul2(p, two(__uint_as_float((__float_as_uint(a) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(b) << 23) + 0x3f800000u)));
 }
 // tanh(c x) = x (a polynomial in x^2), where |c x| <= 0.6: Chebyshev interpolation of tanh(y) / y in y^2, off by 9e-8, its coefficients
-// times by c^(2i + 1).  A c below 2e-4 would take the last of them under the normal numbers: `range` 0, and no x is in it.
+// times by c^(2i + 1).  `range` is at most 3,000: where c is so small that the last coefficients leave the normal numbers, c x is then so
+// small (0.18 at 6e-5) that their terms do not count.
 struct Tanh {
     F2 a[5];
     float range;  // of |x|
@@ -237,17 +238,18 @@ __device__ __forceinline__ Tanh tanh_polynomial(float c, float by)
         t.a[i] = two(C[i] * power, C[i] * power);
         power *= c * c;
     }
-    t.range = c >= 2e-4f ? 0.6f / c : 0.f;
+    t.range = 0.6f / fmaxf(c, 2e-4f);
     return t;
 }
-__device__ __forceinline__ F2 tanh2(F2 x, const Tanh &t)
+__device__ __forceinline__ F2 tanh_over_x(F2 x, const Tanh &t)
 {
     const F2 u = mul2(x, x);
     F2 p = t.a[4];
 #pragma unroll
     for (int i = 3; i >= 0; --i) p = ffma2(p, u, t.a[i]);
-    return mul2(p, x);
+    return p;
 }
+__device__ __forceinline__ F2 tanh2(F2 x, const Tanh &t) { return mul2(tanh_over_x(x, t), x); }
 // Two values in a word, the first in its lower half.
 template <class T> __device__ __forceinline__ uint32_t pack(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b)

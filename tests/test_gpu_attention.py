@@ -90,6 +90,71 @@ def test_single_tokens_over_slots(engine, dtype, d, hq, hkv, mask):
     _check_forward(engine, p)[0].close()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_gradients_of_slots(engine, dtype, d):
+    # keys in slots that are not full: rows behind their length keep what they hold
+    p = Problem(dtype, d, 4, 2, [30, 1, 200, 0], [50, 300, 260, 7], slot=301, window=(-1, 0), bias=True)
+    _check_backward(engine, p).close()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("cap", [0.05, 0.7, 200.0, 3000.0, 1e5, 1e9])
+@pytest.mark.parametrize("q,k", [([40, 200], [90, 200]), ([1, 1], [700, 33])])
+def test_caps_small_and_large(engine, dtype, cap, q, k):
+    p = Problem(dtype, 64, 4, 2, q, k, window=(-1, 0), cap=cap, gain=3.0)
+    _check_backward(engine, p).close()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_many_sequences(engine, dtype):
+    g = torch.Generator().manual_seed(2)
+    q = [int(x) for x in torch.randint(0, 30, (300,), generator=g)]
+    p = Problem(dtype, 64, 2, 1, q, window=(-1, 0))
+    _check_backward(engine, p).close()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("q,k,heads", [([700], [6000], 1), ([300, 20], [5000, 2100], 2), ([256], [4096], 2)])
+def test_keys_in_parts(engine, dtype, q, k, heads):
+    # too few blocks for the GPU: the keys of each are cut
+    p = Problem(dtype, 128, heads, 1, q, k, window=(3000, 0), prefix=70, gain=2.0)
+    plan, _, _ = _check_forward(engine, p)
+    assert plan.last_kernel_name() in ("attention_tc", "attention_few_tc")
+    plan.close()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("q", [1, 300])
+def test_offsets_past_32_bits(engine, dtype, q):
+    # rows 80,000 elements apart: the last ones lie beyond 2^31 elements and 2^32 bytes
+    rows, stride = 27_000, 80_000
+    p = Problem(dtype, 64, 2, 2, [q], [700], window=(-1, 0))
+    K = torch.empty(rows * stride, dtype=dtype, device="cuda").view(rows, stride)[:, :128].unflatten(1, (2, 64))
+    K[rows - 700:] = p.K
+    plan = engine.attention_plan(dtype, 64, 2, 2, offsets([q]), q, 700, k_offsets=torch.tensor([rows - 700, rows], dtype=torch.int32, device="cuda"),
+                                 window=(-1, 0), k_rows=rows)
+    O = torch.empty_like(p.Q)
+    plan.forward(p.Q, K, K, O)
+    p.V = p.K
+    o, _, tol, _ = p.forward()
+    within(O, o, tol)
+    plan.close()
+
+
+def test_few_and_prompt_kernels_behind_other_work(engine):
+    # what runs next on the stream finds all results, also of calls whose rows all have one part
+    p = Problem(BF16, 128, 8, 8, [1] * 4, [5, 30, 17, 9], slot=8192, window=(-1, 0))
+    plan = engine.attention_plan(BF16, 128, 8, 8, p.q_offsets, 1, 8192, k_offsets=p.k_offsets, k_len=p.k_len, window=(-1, 0), k_rows=p.k_rows)
+    o, _, tol, _ = p.forward()
+    for _ in range(50):
+        O = torch.zeros_like(p.Q)
+        plan.forward(p.Q, p.K, p.V, O, flags=api.FLAG_ASYNC)
+        out = O + 0
+        within(out, o, tol)
+    plan.close()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("q,k", [([1], [9001]), ([3], [5000]), ([17, 2], [4100, 2500]), ([200], [3000])])
 def test_few_queries_many_keys(engine, dtype, q, k):
