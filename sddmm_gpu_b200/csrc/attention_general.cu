@@ -443,24 +443,27 @@ __global__ void __launch_bounds__(THREADS) attention_dkv_general_kernel(const At
         if (turn % (THREADS / 32) == (int)threadIdx.x / 32) strict::dkv_row<T>(p, s, kv, j0 + __ffsll((long long)left) - 1);
 }
 
-// The parts' sums of TILE rows added in order; KV: dK and dV, else dQ.
+// The parts' sums of 16 rows added in order; KV: dK and dV, else dQ.  TILE: rows of the blocks that left them.
+constexpr int SUM_ROWS = 16;
 template <class T, bool KV, int TILE>
 __global__ void __launch_bounds__(THREADS) attention_sum_parts_kernel(const AttentionParams p)
 {
-    __shared__ unsigned long long bad[TILE / 64];
-    if (threadIdx.x < TILE / 64) bad[threadIdx.x] = 0;
-    const int heads = KV ? p.kv_heads : p.q_heads, head = blockIdx.x % heads;
+    __shared__ unsigned bad;
+    if (threadIdx.x == 0) bad = 0;
+    const unsigned slice = blockIdx.x % (TILE / SUM_ROWS), block_of = blockIdx.x / (TILE / SUM_ROWS);
+    const int heads = KV ? p.kv_heads : p.q_heads, head = block_of % heads;
     Sequence s;
     int seq, block;
-    if (!find_block<TILE>(p, blockIdx.x / heads, KV, s, seq, block)) return;
-    const int r0 = block * TILE, rows = min(TILE, (KV ? s.nk : s.nq) - r0);
+    if (!find_block<TILE>(p, block_of / heads, KV, s, seq, block)) return;
+    const int t0 = block * TILE, in_tile = min(TILE, (KV ? s.nk : s.nq) - t0), r0 = t0 + slice * SUM_ROWS, rows = min(SUM_ROWS, t0 + in_tile - r0);
+    if (rows <= 0) return;
     int tiles;
     if (KV) {
         int from, per_head;
-        query_tiles<TILE>(p, s, r0, rows, from, per_head);
+        query_tiles<TILE>(p, s, t0, in_tile, from, per_head);
         tiles = per_head * p.group;
     } else {
-        tiles = key_tiles<TILE>(reach_of(p.window, s, r0, r0 + rows)).n;
+        tiles = key_tiles<TILE>(reach_of(p.window, s, t0, t0 + in_tile)).n;
     }
     const int parts = (tiles + p.chunk_tiles - 1) / p.chunk_tiles;
     if (parts <= 1) return;
@@ -479,20 +482,19 @@ __global__ void __launch_bounds__(THREADS) attention_sum_parts_kernel(const Atte
                 const float4 v = at4(from + k * array * (KV ? 2 : 1));
                 sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
             }
-            collect(&bad[r / 64], not_finite(sum), r % 64);
+            if (not_finite(sum)) atomicOr(&bad, 1u << r);
             store4<T>(KV ? (x ? p.dv : p.dk) : p.dq, row, head, c, p.head_dim, sum);
         }
     }
     __syncthreads();
     int turn = 0;
-    for (int q = 0; q < TILE / 64; ++q)
-        for (unsigned long long left = bad[q]; left; left &= left - 1, ++turn) {
-            const int r = 64 * q + __ffsll((long long)left) - 1;
-            if (turn % (THREADS / 32) != (int)threadIdx.x / 32) continue;
-            const int64_t at = (int64_t)head * p.q_rows + s.q0 + r0 + r;
-            if (KV) strict::dkv_row<T>(p, s, head, r0 + r);
-            else strict::dq_row<T>(p, s, head, r0 + r, __ldg(p.lse + at), p.delta[at]);
-        }
+    for (unsigned left = bad; left; left &= left - 1, ++turn) {
+        const int r = __ffs(left) - 1;
+        if (turn % (THREADS / 32) != (int)threadIdx.x / 32) continue;
+        const int64_t at = (int64_t)head * p.q_rows + s.q0 + r0 + r;
+        if (KV) strict::dkv_row<T>(p, s, head, r0 + r);
+        else strict::dq_row<T>(p, s, head, r0 + r, __ldg(p.lse + at), p.delta[at]);
+    }
 }
 
 template <class Kern>
@@ -576,7 +578,7 @@ Parts plan_attention_parts(const AttentionParams &p, int tile, int per_sm, int s
 
 cudaError_t launch_attention_sum_parts(const AttentionParams &p, bool kv, int tile, cudaStream_t s)
 {
-    const unsigned grid = (unsigned)(kv ? p.kv_heads * most_blocks(p.k_rows, p.n_seqs, p.max_k, tile) : p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, tile));
+    const unsigned grid = (unsigned)(kv ? p.kv_heads * most_blocks(p.k_rows, p.n_seqs, p.max_k, tile) : p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, tile)) * (tile / SUM_ROWS);
     if (grid == 0) return cudaSuccess;
     if (p.dtype == 0) kv ? attention_sum_parts_kernel<float, true, 64><<<grid, THREADS, 0, s>>>(p) : attention_sum_parts_kernel<float, false, 64><<<grid, THREADS, 0, s>>>(p);
     else if (p.dtype == 1) kv ? attention_sum_parts_kernel<__half, true, 128><<<grid, THREADS, 0, s>>>(p) : attention_sum_parts_kernel<__half, false, 128><<<grid, THREADS, 0, s>>>(p);
