@@ -127,6 +127,27 @@ cudaError_t launch_attention_forward_tc(const AttentionParams &p, const ForwardP
 // Adds up the parts of the prompt kernel, whose blocks have 256 queries and go through tiles of 128 keys.
 constexpr int PROMPT_QUERIES = 256, PROMPT_KEYS = 128;
 cudaError_t launch_attention_join(const AttentionParams &p, cudaStream_t s);
+// Launches of one call behind one another: a kernel is set up while the one before it ends.  Every block of such a kernel calls
+// behind_last_kernel() before it touches what that one wrote or reads, and before it ends, so that no grid ends before the one it stands
+// behind; the kernel before it calls next_kernel_may_come().
+__device__ __forceinline__ void behind_last_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void next_kernel_may_come() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <class... Args, class... Given>
+inline cudaError_t launch_behind(void (*kernel)(Args...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, const Given &...args)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 cudaError_t launch_attention_forward_general(const AttentionParams &p, cudaStream_t s);
 // Where the blocks of a backward kernel alone would leave multiprocessors idle, the tiles that a block goes through are cut into parts, a
 // block each, which leave their sums in the workspace (parts x rows x heads x head_dim, dK and dV behind one another) for

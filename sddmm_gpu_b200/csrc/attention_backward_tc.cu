@@ -75,8 +75,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
     const int heads = KV ? p.kv_heads : p.q_heads, head = block_of % heads, kv = KV ? head : head / p.group;
     Sequence s;
     int seq, block;
+    next_kernel_may_come();
     // causal sequences: the last queries see the most keys, the first keys are seen by the most queries
-    if (!find_block<T>(p, KV ? block_of / heads : (blocks - 1 - block_of) / heads, KV, s, seq, block)) return;
+    const bool found = find_block<T>(p, KV ? block_of / heads : (blocks - 1 - block_of) / heads, KV, s, seq, block);
+    if (KV) behind_last_kernel();
+    if (!found) return;
     const int r0 = block * T, n_rows = min(T, (KV ? s.nk : s.nq) - r0);
     // the tiles of the other side
     Reach reach = {};
@@ -522,8 +525,12 @@ cudaError_t launch(const AttentionParams &p0, const Parts &parts, const Maps &ma
     if (e != cudaSuccess) return e;
     p.n_splits = parts.n_kv;
     p.chunk_tiles = parts.tiles_kv;
-    if (grid_kv) attention_backward_tc_kernel<E, DP, CAP, BIAS, true><<<grid_kv * parts.n_kv, THREADS, smem_kv, s>>>(p, maps);
-    e = cudaGetLastError();
+    if (grid_kv && grid_q) {
+        e = launch_behind(attention_backward_tc_kernel<E, DP, CAP, BIAS, true>, grid_kv * parts.n_kv, THREADS, smem_kv, s, p, maps);
+    } else if (grid_kv) {
+        attention_backward_tc_kernel<E, DP, CAP, BIAS, true><<<grid_kv * parts.n_kv, THREADS, smem_kv, s>>>(p, maps);
+        e = cudaGetLastError();
+    }
     if (e == cudaSuccess && parts.n_kv > 1) e = launch_attention_sum_parts(p, true, T, s);
     return e;
 }

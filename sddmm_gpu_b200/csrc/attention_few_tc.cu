@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident_blocks(DP)) attention_few
     if ((int)chunk >= ch.n) return;
     const int first = chunk * p.chunk_tiles, end = min(ch.keys.n, first + p.chunk_tiles);
     const int D = p.head_dim;
-    if (p.n_splits > 1 && threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
+    if (p.n_splits > 1) next_kernel_may_come();
 
     // ---- the ring: this warp's tiles first + warp, + 4, ... ----
     const int mine = max(0, (end - first - warp + WARPS - 1) / WARPS);
@@ -304,9 +304,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
     } else {
         n = chunks_of(p, s, (i * p.group + head % p.group) / ROWS).n;
     }
-    // This grid may have been started before the parts were written.  Every block waits, also one that has nothing to add: the grid must not end
-    // before the one that it stands behind.
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    behind_last_kernel();
     if (n <= 1) return;
     const int64_t stride = (int64_t)p.q_rows * p.q_heads, at = ((int64_t)s.q0 + i) * p.q_heads + head;
     float y[4] = {}, top = -INFINITY, total = 0.f;
@@ -370,16 +368,8 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
 template <class E, bool TILES>
 cudaError_t launch_join(const AttentionParams &p, cudaStream_t s)
 {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)((int64_t)p.n_seqs * p.max_q * p.q_heads));
-    cfg.blockDim = dim3(256);
-    cfg.stream = s;
-    cudaLaunchAttribute early{};  // (24 tokens: 37 us without, 33 with)
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &early;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_join_kernel<E, TILES>, p);
+    // (24 tokens: 37 us as an ordinary launch, 33 so)
+    return launch_behind(attention_join_kernel<E, TILES>, (unsigned)((int64_t)p.n_seqs * p.max_q * p.q_heads), 256, 0, s, p);
 }
 
 template <class E, int DP, bool CAP, bool BIAS>

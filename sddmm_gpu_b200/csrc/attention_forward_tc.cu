@@ -86,6 +86,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
     __shared__ uint32_t tmem_holder, bad[8];
     __shared__ float row_most[2][2][2][T], row_sum[2][2][T], row_lse[2 * T];  // [step parity][tile][half]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (PARTS) next_kernel_may_come();
     const unsigned splits = PARTS ? p.n_splits : 1, blocks = gridDim.x / splits, block_of = blockIdx.x / splits, part = PARTS ? blockIdx.x % splits : 0;
     const int head = block_of % p.q_heads, kv = head / p.group;
     Sequence s;

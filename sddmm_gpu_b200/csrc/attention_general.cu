@@ -266,6 +266,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dq_general_kernel(const 
     const int head = block_of % p.q_heads, kv = head / p.group;
     Sequence s;
     int seq, block;
+    next_kernel_may_come();
     if (!find_block<B>(p, (blocks - 1 - block_of) / p.q_heads, false, s, seq, block)) return;
     const int i0 = block * B, n = min(B, s.nq - i0);
     const Reach reach = reach_of(p.window, s, i0, i0 + n);
@@ -367,7 +368,10 @@ __global__ void __launch_bounds__(THREADS) attention_dkv_general_kernel(const At
     Sequence s;
     int seq, block;
     // the first keys of a causal sequence are seen by the most queries: they go first
-    if (!find_block<B>(p, block_of / p.kv_heads, true, s, seq, block)) return;
+    const bool found = find_block<B>(p, block_of / p.kv_heads, true, s, seq, block);
+    next_kernel_may_come();
+    behind_last_kernel();
+    if (!found) return;
     const int j0 = block * B, m = min(B, s.nk - j0);
     int from, per_head;
     query_tiles<B>(p, s, j0, m, from, per_head);
@@ -454,7 +458,10 @@ __global__ void __launch_bounds__(THREADS) attention_sum_parts_kernel(const Atte
     const int heads = KV ? p.kv_heads : p.q_heads, head = block_of % heads;
     Sequence s;
     int seq, block;
-    if (!find_block<TILE>(p, block_of / heads, KV, s, seq, block)) return;
+    const bool found = find_block<TILE>(p, block_of / heads, KV, s, seq, block);
+    next_kernel_may_come();
+    behind_last_kernel();
+    if (!found) return;
     const int t0 = block * TILE, in_tile = min(TILE, (KV ? s.nk : s.nq) - t0), r0 = t0 + slice * SUM_ROWS, rows = min(SUM_ROWS, t0 + in_tile - r0);
     if (rows <= 0) return;
     int tiles;
@@ -498,11 +505,12 @@ __global__ void __launch_bounds__(THREADS) attention_sum_parts_kernel(const Atte
 }
 
 template <class Kern>
-cudaError_t launch(Kern kern, SmemOptinCache &optin, unsigned grid, size_t smem, const AttentionParams &p, cudaStream_t s)
+cudaError_t launch(Kern kern, SmemOptinCache &optin, unsigned grid, size_t smem, const AttentionParams &p, cudaStream_t s, bool behind = false)
 {
     const cudaError_t e = optin_dynamic_smem(kern, smem, optin);
     if (e != cudaSuccess) return e;
     if (grid == 0) return cudaSuccess;
+    if (behind) return launch_behind(kern, grid, THREADS, smem, s, p);
     kern<<<grid, THREADS, smem, s>>>(p);
     return cudaGetLastError();
 }
@@ -529,7 +537,7 @@ cudaError_t backward_of(const AttentionParams &p0, const Parts &parts, cudaStrea
     if (e != cudaSuccess) return e;
     p.n_splits = parts.n_kv;
     p.chunk_tiles = parts.tiles_kv;
-    e = launch(attention_dkv_general_kernel<T, DP>, optin_kv, grid_kv * parts.n_kv, smem_of(p.head_dim, 4, 2), p, s);
+    e = launch(attention_dkv_general_kernel<T, DP>, optin_kv, grid_kv * parts.n_kv, smem_of(p.head_dim, 4, 2), p, s, grid_q > 0);
     if (e == cudaSuccess && parts.n_kv > 1) e = launch_attention_sum_parts(p, true, B, s);
     return e;
 }
@@ -580,10 +588,10 @@ cudaError_t launch_attention_sum_parts(const AttentionParams &p, bool kv, int ti
 {
     const unsigned grid = (unsigned)(kv ? p.kv_heads * most_blocks(p.k_rows, p.n_seqs, p.max_k, tile) : p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, tile)) * (tile / SUM_ROWS);
     if (grid == 0) return cudaSuccess;
-    if (p.dtype == 0) kv ? attention_sum_parts_kernel<float, true, 64><<<grid, THREADS, 0, s>>>(p) : attention_sum_parts_kernel<float, false, 64><<<grid, THREADS, 0, s>>>(p);
-    else if (p.dtype == 1) kv ? attention_sum_parts_kernel<__half, true, 128><<<grid, THREADS, 0, s>>>(p) : attention_sum_parts_kernel<__half, false, 128><<<grid, THREADS, 0, s>>>(p);
-    else kv ? attention_sum_parts_kernel<__nv_bfloat16, true, 128><<<grid, THREADS, 0, s>>>(p) : attention_sum_parts_kernel<__nv_bfloat16, false, 128><<<grid, THREADS, 0, s>>>(p);
-    return cudaGetLastError();
+    auto run = [&](auto of_kv, auto of_q) { return launch_behind(kv ? of_kv : of_q, grid, THREADS, 0, s, p); };
+    if (p.dtype == 0) return run(attention_sum_parts_kernel<float, true, 64>, attention_sum_parts_kernel<float, false, 64>);
+    if (p.dtype == 1) return run(attention_sum_parts_kernel<__half, true, 128>, attention_sum_parts_kernel<__half, false, 128>);
+    return run(attention_sum_parts_kernel<__nv_bfloat16, true, 128>, attention_sum_parts_kernel<__nv_bfloat16, false, 128>);
 }
 
 cudaError_t launch_attention_forward_general(const AttentionParams &p, cudaStream_t s) { return by_type(nullptr, p, s); }
