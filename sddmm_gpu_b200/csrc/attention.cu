@@ -141,6 +141,15 @@ int sddmm_attention_plan(sddmm_handle_t h, const sddmm_attention_desc *d, sddmm_
         a->prompt = plan_attention_forward_tc(p, h->sm_count);
         a->by_few = a->few.n_splits > 0 && a->few.us < a->prompt.us;
     }
+    if (p.dtype == SDDMM_F32) {
+        a->few = plan_attention_few_f32(p, h->sm_count);
+        // The general kernel's 64 queries take 6.5 us for 64 keys of 64 columns, 10 of 128, on a multiprocessor of their own; every further block
+        // that shares it a quarter more.  (us, general / few: a token of 32 / 8 heads over 8,000 keys 1,243 / 33, 500 queries of 8 heads of 64
+        // on as many keys 57 / 58, 1,000 on 1,000 107 / 152.)
+        const int64_t blocks = p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, 64), waves = (blocks + h->sm_count - 1) / h->sm_count;
+        const double general = 5. + (0.75 + 0.25 * (double)waves) * (double)((p.max_k + 63) / 64) * (p.head_dim <= 64 ? 6.5 : 10.);
+        a->by_few = a->few.n_splits > 0 && a->few.us < general;
+    }
     a->parts = p.dtype == SDDMM_F32 ? plan_attention_parts(p, 64, 4, h->sm_count) : plan_attention_parts(p, 128, 1, h->sm_count);
     *out = a;
     return SDDMM_OK;
@@ -185,6 +194,11 @@ int sddmm_attention_forward(sddmm_attention_t a, const sddmm_head_array *Q, cons
         const ForwardPlan &f = a->by_few ? a->few : a->prompt;
         const cudaError_t e = a->by_few ? launch_attention_few_tc(p, f, workspace, &taken, h->stream) : launch_attention_forward_tc(p, f, workspace, &taken, h->stream);
         if (taken) return finish(a, e, a->by_few ? "attention_few_tc" : "attention_tc", f.n_splits > 1 ? 2 : 1, flags);
+    }
+    if (p.dtype == SDDMM_F32 && a->by_few) {
+        bool taken = false;
+        const cudaError_t e = launch_attention_few_f32(p, a->few, workspace, &taken, h->stream);
+        if (taken) return finish(a, e, "attention_few_f32", a->few.n_splits > 1 ? 2 : 1, flags);
     }
     return finish(a, launch_attention_forward_general(p, h->stream), "attention_general", 1, flags);
 }

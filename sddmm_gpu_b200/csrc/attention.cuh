@@ -124,9 +124,39 @@ ForwardPlan plan_attention_forward_tc(const AttentionParams &p, int sm_count);
 // *taken false, and nothing launched, where the call's type, strides or alignment do not allow the kernel.
 cudaError_t launch_attention_few_tc(const AttentionParams &p, const ForwardPlan &f, void *workspace, bool *taken, cudaStream_t s);
 cudaError_t launch_attention_forward_tc(const AttentionParams &p, const ForwardPlan &f, void *workspace, bool *taken, cudaStream_t s);
-// Adds up the parts of the prompt kernel, whose blocks have 256 queries and go through tiles of 128 keys.
+ForwardPlan plan_attention_few_f32(const AttentionParams &p, int sm_count);
+cudaError_t launch_attention_few_f32(const AttentionParams &p, const ForwardPlan &f, void *workspace, bool *taken, cudaStream_t s);
+// For the kernels of few rows: how the keys are cut for blocks of `rows` rows, tiles of `keys` keys `warps` warps and `least` tiles or more, `resident` blocks to a multiprocessor; us
+// is the number of rows x keys units in all.
+ForwardPlan plan_few(const AttentionParams &p, int rows, int keys, int warps, int least, int resident, int sm_count);
+constexpr int FEW_ROWS = 16, FEW_KEYS = 16, FEW_F32_KEYS = 16;
+// Rows of a block in fp32.
+__host__ __device__ inline int few_rows_f32(const AttentionParams &p)
+{
+    const int64_t rows = (int64_t)p.max_q * p.group;
+    return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
+}
+// The chunks that the keys of row tile `tile` of such a kernel are cut into.
+template <int KEYS> struct Chunks {
+    KeyTiles keys;
+    Reach reach;
+    int n;
+};
+template <int KEYS>
+__device__ __forceinline__ Chunks<KEYS> chunks_of(const AttentionParams &p, const Sequence &s, int tile, int rows)
+{
+    const int r0 = tile * rows, r1 = min(r0 + rows, s.nq * p.group);
+    Chunks<KEYS> c;
+    c.reach = reach_of(p.window, s, r0 / p.group, (r1 - 1) / p.group + 1);
+    c.keys = key_tiles<KEYS>(c.reach);
+    c.n = max(1, (c.keys.n + p.chunk_tiles - 1) / p.chunk_tiles);
+    return c;
+}
+// Adds up parts: of the kernels of few rows, or of the prompt kernel, whose blocks have 256 queries and go through tiles of 128 keys.
 constexpr int PROMPT_QUERIES = 256, PROMPT_KEYS = 128;
-cudaError_t launch_attention_join(const AttentionParams &p, cudaStream_t s);
+enum JoinOf { JOIN_FEW, JOIN_PROMPT, JOIN_FEW_F32 };
+cudaError_t launch_attention_join(const AttentionParams &p, JoinOf of, cudaStream_t s);
+
 // Launches of one call behind one another: a kernel is set up while the one before it ends.  Every block of such a kernel calls
 // behind_last_kernel() before it touches what that one wrote or reads, and before it ends, so that no grid ends before the one it stands
 // behind; the kernel before it calls next_kernel_may_come().

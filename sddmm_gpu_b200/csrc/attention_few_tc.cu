@@ -18,12 +18,9 @@ namespace sddmm {
 
 namespace {
 
-constexpr int KEYS = 16, WARPS = 4, STAGES = 3, ROWS = 16;
+constexpr int KEYS = FEW_KEYS, WARPS = 4, STAGES = 3, ROWS = FEW_ROWS;
 constexpr float RAISE = 8.f;
-#ifndef MOST_TILES
-#define MOST_TILES 64
-#endif
-constexpr int LEAST_TILES = 16;
+constexpr int MOST_TILES = 16;  // of a warp, in one chunk
 constexpr int resident_blocks(int head_dim) { return head_dim <= 64 ? 4 : 2; }  // of a multiprocessor, by registers
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
@@ -50,22 +47,6 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The chunks that the keys of row tile `tile` are cut into.
-struct Chunks {
-    KeyTiles keys;
-    Reach reach;
-    int n;
-};
-__device__ __forceinline__ Chunks chunks_of(const AttentionParams &p, const Sequence &s, int tile)
-{
-    const int r0 = tile * ROWS, r1 = min(r0 + ROWS, s.nq * p.group);
-    Chunks c;
-    c.reach = reach_of(p.window, s, r0 / p.group, (r1 - 1) / p.group + 1);
-    c.keys = key_tiles<KEYS>(c.reach);
-    c.n = max(1, (c.keys.n + p.chunk_tiles - 1) / p.chunk_tiles);
-    return c;
-}
-
 template <class E, int DP, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(WARPS * 32, resident_blocks(DP)) attention_few_kernel(const AttentionParams p, int row_tiles)
 {
@@ -79,7 +60,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident_blocks(DP)) attention_few
     const Sequence s = sequence_of(p, seq);
     const int rows = s.nq * p.group, r0 = tile * ROWS;
     if (r0 >= rows) return;
-    const Chunks ch = chunks_of(p, s, tile);
+    const Chunks<KEYS> ch = chunks_of<KEYS>(p, s, tile, ROWS);
     if ((int)chunk >= ch.n) return;
     const int first = chunk * p.chunk_tiles, end = min(ch.keys.n, first + p.chunk_tiles);
     const int D = p.head_dim;
@@ -287,8 +268,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident_blocks(DP)) attention_few
 
 // The parts of one row added up, a block for a row: warps take chunks in turn, eight at once, so that all of a row's parts are asked for
 // before the first is used.
-// TILES: of the tensor-core prompt kernel (parts of the keys of 256 queries), else of the kernel above (of 16 rows).
-template <class E, bool TILES>
+template <class E, JoinOf OF>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionParams p)
 {
     constexpr int JOIN_WARPS = 8, AT_ONCE = 8;
@@ -298,11 +278,12 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
     const Sequence s = sequence_of(p, seq);
     int n = 0;
     if (i >= s.nq) {
-    } else if (TILES) {
+    } else if (OF == JOIN_PROMPT) {
         const int i0 = i / PROMPT_QUERIES * PROMPT_QUERIES;
         n = (key_tiles<PROMPT_KEYS>(reach_of(p.window, s, i0, min(s.nq, i0 + PROMPT_QUERIES))).n + p.chunk_tiles - 1) / p.chunk_tiles;
     } else {
-        n = chunks_of(p, s, (i * p.group + head % p.group) / ROWS).n;
+        const int rows = OF == JOIN_FEW ? FEW_ROWS : few_rows_f32(p);
+        n = chunks_of<OF == JOIN_FEW ? FEW_KEYS : FEW_F32_KEYS>(p, s, (i * p.group + head % p.group) / rows, rows).n;
     }
     behind_last_kernel();
     if (n <= 1) return;
@@ -365,11 +346,11 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
     }
 }
 
-template <class E, bool TILES>
+template <class E, JoinOf OF>
 cudaError_t launch_join(const AttentionParams &p, cudaStream_t s)
 {
     // (24 tokens: 37 us as an ordinary launch, 33 so)
-    return launch_behind(attention_join_kernel<E, TILES>, (unsigned)((int64_t)p.n_seqs * p.max_q * p.q_heads), 256, 0, s, p);
+    return launch_behind(attention_join_kernel<E, OF>, (unsigned)((int64_t)p.n_seqs * p.max_q * p.q_heads), 256, 0, s, p);
 }
 
 template <class E, int DP, bool CAP, bool BIAS>
@@ -385,7 +366,7 @@ cudaError_t launch(const AttentionParams &p, cudaStream_t s)
     attention_few_kernel<E, DP, CAP, BIAS><<<grid, WARPS * 32, smem, s>>>(p, row_tiles);
     e = cudaGetLastError();
     if (e != cudaSuccess || p.n_splits == 1) return e;
-    return launch_join<E, false>(p, s);
+    return launch_join<E, JOIN_FEW>(p, s);
 }
 template <class E, int DP>
 cudaError_t by_score(const AttentionParams &p, cudaStream_t s)
@@ -398,38 +379,46 @@ bool wide(const HeadArray &a) { return (uintptr_t)a.data % 16 == 0 && a.row % 8 
 
 }  // namespace
 
-ForwardPlan plan_attention_few_tc(const AttentionParams &p, int sm_count)
+ForwardPlan plan_few(const AttentionParams &p, int rows, int keys, int warps, int least, int resident_of_one, int sm_count)
 {
     ForwardPlan f{0, 1, 0, INFINITY};
-    if (p.dtype == 0 || p.max_q == 0 || p.n_seqs == 0) return f;
-    if ((int64_t)p.max_q * p.group > INT32_MAX) return f;
-    const int64_t row_tiles = ((int64_t)p.max_q * p.group + ROWS - 1) / ROWS, blocks = row_tiles * p.kv_heads * p.n_seqs;
-    const int64_t tiles = (p.max_k + KEYS - 1) / KEYS + 1;  // (+ 1: prefix and window may begin inside tiles)
+    if (p.max_q == 0 || p.n_seqs == 0 || (int64_t)p.max_q * p.group > INT32_MAX) return f;
+    const int64_t row_tiles = ((int64_t)p.max_q * p.group + rows - 1) / rows, blocks = row_tiles * p.kv_heads * p.n_seqs;
+    const int64_t tiles = (p.max_k + keys - 1) / keys + 1;  // (+ 1: prefix and window may begin inside tiles)
     auto bytes_of = [&](int64_t n) { return n == 1 ? 0 : n * p.q_rows * p.q_heads * (int64_t)(p.head_dim + 1) * 4; };
     auto n_of = [&](int64_t c) { return tiles <= c ? (int64_t)1 : (tiles + c - 1) / c; };
-    // As many chunks as fill whole waves of resident blocks, of MOST_TILES key tiles at most: longer ones leave
-    // the last block of ragged sequences alone, shorter ones spend their time beginning and ending.
-    const int64_t resident = (int64_t)resident_blocks(p.head_dim) * sm_count, waves = (tiles * blocks + resident * MOST_TILES - 1) / (resident * MOST_TILES);
+    // As many chunks as fill whole waves of resident blocks, of MOST_TILES key tiles a warp at most: longer ones leave the last block of ragged
+    // sequences alone, shorter ones spend their time beginning and ending.
+    const int64_t most = warps * MOST_TILES, resident = (int64_t)resident_of_one * sm_count, waves = (tiles * blocks + resident * most - 1) / (resident * most);
     const int64_t want = resident * waves / blocks > 1 ? resident * waves / blocks : 1;
-    int64_t chunk = ((tiles + want - 1) / want + WARPS - 1) / WARPS * WARPS;
-    if (chunk < LEAST_TILES) chunk = LEAST_TILES;
+    int64_t chunk = ((tiles + want - 1) / want + warps - 1) / warps * warps;
+    if (chunk < least) chunk = least;
     while (n_of(chunk) > 1 && bytes_of(n_of(chunk)) > (1ll << 30)) chunk *= 2;
     const int64_t n = n_of(chunk);
     if (n * blocks > INT32_MAX || (int64_t)p.n_seqs * p.max_q * p.q_heads > INT32_MAX) return f;
     f.chunk_tiles = (int)chunk;
     f.n_splits = (int)n;
     f.bytes = bytes_of(n);
-    // (8 us, and 0.19 for 16 rows x 16 keys on a multiprocessor, however many warps it has; 6 more with a join.  Rows of the sequences, not of
-    // the longest)
-    const int64_t most_rows = (int64_t)p.n_seqs * row_tiles, rows = p.q_rows * p.group / ROWS + p.n_seqs < most_rows ? p.q_rows * p.group / ROWS + p.n_seqs : most_rows;
-    const double units = (double)rows * p.kv_heads * tiles;
-    f.us = 8. + 0.19 * units / sm_count + (n > 1 ? 6. : 0.);
+    // rows of the sequences, not of the longest
+    const int64_t most_rows = p.n_seqs * row_tiles, all_rows = p.q_rows * p.group / rows + p.n_seqs;
+    f.us = (double)(all_rows < most_rows ? all_rows : most_rows) * p.kv_heads * tiles;
     return f;
 }
 
-cudaError_t launch_attention_join(const AttentionParams &p, cudaStream_t s)
+ForwardPlan plan_attention_few_tc(const AttentionParams &p, int sm_count)
 {
-    return p.dtype == 1 ? launch_join<__half, true>(p, s) : launch_join<__nv_bfloat16, true>(p, s);
+    if (p.dtype == 0) return ForwardPlan{0, 1, 0, INFINITY};
+    ForwardPlan f = plan_few(p, ROWS, KEYS, WARPS, 4 * WARPS, resident_blocks(p.head_dim), sm_count);
+    // (8 us, and 0.19 for 16 rows x 16 keys on a multiprocessor, however many warps it has; 6 more with a join)
+    f.us = 8. + 0.19 * f.us / sm_count + (f.n_splits > 1 ? 6. : 0.);
+    return f;
+}
+
+cudaError_t launch_attention_join(const AttentionParams &p, JoinOf of, cudaStream_t s)
+{
+    if (p.dtype == 0) return launch_join<float, JOIN_FEW_F32>(p, s);
+    if (of == JOIN_PROMPT) return p.dtype == 1 ? launch_join<__half, JOIN_PROMPT>(p, s) : launch_join<__nv_bfloat16, JOIN_PROMPT>(p, s);
+    return p.dtype == 1 ? launch_join<__half, JOIN_FEW>(p, s) : launch_join<__nv_bfloat16, JOIN_FEW>(p, s);
 }
 
 cudaError_t launch_attention_few_tc(const AttentionParams &p0, const ForwardPlan &f, void *workspace, bool *taken, cudaStream_t s)

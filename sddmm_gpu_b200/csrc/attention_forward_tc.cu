@@ -563,7 +563,7 @@ cudaError_t launch_attention_forward_tc(const AttentionParams &p0, const Forward
     cudaError_t e;
     if (p.dtype == 1) e = p.head_dim <= 64 ? by_score<__half, 64>(p, maps, s) : by_score<__half, 128>(p, maps, s);
     else e = p.head_dim <= 64 ? by_score<__nv_bfloat16, 64>(p, maps, s) : by_score<__nv_bfloat16, 128>(p, maps, s);
-    return e == cudaSuccess && p.n_splits > 1 ? launch_attention_join(p, s) : e;
+    return e == cudaSuccess && p.n_splits > 1 ? launch_attention_join(p, JOIN_PROMPT, s) : e;
 }
 
 }  // namespace sddmm

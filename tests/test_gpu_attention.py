@@ -162,6 +162,31 @@ def test_few_queries_many_keys(engine, dtype, q, k):
     _check_forward(engine, p)[0].close()
 
 
+@pytest.mark.parametrize("mask", range(len(MASKS)))
+@pytest.mark.parametrize("d,hq,hkv,q,k", [(128, 8, 1, [1], [5000]), (8, 7, 7, [1, 2, 5], [900, 17, 2]), (72, 6, 2, [3, 0, 1], [4000, 90, 2100]),
+                                          (64, 4, 4, [19], [3001])])
+def test_few_queries_in_fp32(engine, d, hq, hkv, q, k, mask):
+    p = Problem(F32, d, hq, hkv, q, k, seed=mask + 1, gain=2.0, **MASKS[mask])
+    plan, _, _ = _check_forward(engine, p)
+    if mask == 0 and k[0] > 3000:
+        assert plan.last_kernel_name() == "attention_few_f32"
+    plan.close()
+
+
+@pytest.mark.parametrize("value", [NAN, math.inf, -math.inf])
+def test_few_queries_in_fp32_masked_places(engine, value):
+    p = Problem(F32, 64, 4, 2, [1, 2], [3000, 2500], window=(700, 0), prefix=5)
+    o, lse, tol_o, tol_l = p.forward()
+    for x in (p.K, p.V):
+        x[5:2298] = value                  # of the first sequence, hidden
+        x[5499] = value                    # seen by the last row alone
+    plan, O, l = _forward(engine, p)
+    within(O[:2], o[:2], tol_o[:2], "O")
+    within(l[:, :2], lse[:, :2], tol_l[:, :2], "lse")
+    assert not bool(O[2].isfinite().all())
+    plan.close()
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_long_band_with_global_tokens(engine, dtype):
     p = Problem(dtype, 64, 2, 2, [2300], window=(256, 256), prefix=80, gain=2.0)
