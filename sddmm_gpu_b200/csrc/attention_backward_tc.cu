@@ -19,6 +19,9 @@
 // dQ: score gradients have a place of their own in tensor memory (two, in turn), so the next tile's scores are computed as soon as the
 // last ones have been read.  dK, dV: tensor memory is full (S, dP, dV, dK); P and dS take the place of S and dP, and the
 // products take turns: dV, S of the next tile, dK, dP of the next tile.
+//
+// What bounds them: the row warps' chain beside the products' issue: dQ 2,170 clocks a tile for 1,600 of issue, dK, dV 3,200 for 2,112.
+// 8,192 causal tokens, 8 heads of 128, bfloat16: 468 us, 735 TFLOP/s of the five products that it cannot do without.
 #include <type_traits>
 
 #include "attention_strict.cuh"
@@ -50,7 +53,7 @@ struct alignas(64) Maps {
 template <int DP, bool KV> struct Shape {
     static constexpr int BOXES = DP / 64, TILE_BYTES = T * DP * 2, BOX_BYTES = T * 128;
     // The streamed tiles: K or Q is used by S and again, an iteration later, by the last product; V or dO is done with earlier in
-    // the dQ kernel.  With one ring of five for both, V waited for the slot of a K (3,270 clocks a tile of dQ instead of 2,600).
+    // the dQ kernel.  With one ring of five for both, V waited for the slot of a K (3,270 clocks a tile of dQ; with two rings 2,600 then, 2,170 now).
     static constexpr int SLOTS0 = DP == 64 ? 4 : 3, SLOTS1 = DP == 64 ? 4 : 2;
     static constexpr int SMEM = (2 + SLOTS0 + SLOTS1) * TILE_BYTES;
 };

@@ -7,6 +7,9 @@
 // its own in shared memory (16-byte asynchronous copies, zeros behind the sequence's end, three stages), keeps maximum, sum and
 // output in registers, and waits for no other warp before the end.  The warps' parts are added in order; where a sequence has several
 // chunks the parts go to the workspace and a second kernel, a block for each row, adds them in order.  Nothing depends on scheduling.
+//
+// What bounds it: memory in the middle, beginning, end and join around it (10 us).  One token on 32,801 keys, 32 / 8 heads of 128, bfloat16: 30.7 us,
+// 4.4 TB/s; 32 tokens on 4,000 each, 8 heads: 95 us, 5.5 TB/s.
 #include <cmath>
 #include <type_traits>
 
