@@ -503,8 +503,16 @@ class Attention:
 
     def _workspace(self, backward, like):
         import torch
-        n = self._bytes[backward]
-        return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None
+        n, h = self._bytes[backward], self.handle
+        if not n:
+            return None
+        if not h._explicit_stream:
+            return torch.empty(n, dtype=torch.uint8, device=like.device)
+        # of the stream that it is used on: given back when the call returns, it may go to that stream's next call alone
+        if not h._stream:
+            raise ValueError("this call needs a workspace, and torch has none for the handle's own stream: set_stream() to a stream or to None")
+        with torch.cuda.stream(torch.cuda.ExternalStream(h._stream, device=like.device)):
+            return torch.empty(n, dtype=torch.uint8, device=like.device)
 
     def forward(self, Q, K, V, O, lse=None, flags=0):
         """O (and lse, heads x rows, natural log) of the whole batch; returns O."""

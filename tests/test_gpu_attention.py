@@ -372,6 +372,36 @@ def test_streams_and_graphs(engine):
     plan.close()
 
 
+def test_workspace_of_a_chosen_stream(engine):
+    # a stream other than torch's current one: what the call gives back must not go to the current stream's next tensor
+    p = Problem(BF16, 64, 8, 2, [1], [9000], window=(-1, 0))
+    plan = p.plan(engine)
+    assert plan._bytes[0] > 0
+    side, seen, get = torch.cuda.Stream(), [], plan._workspace
+
+    def watched(*a):
+        w = get(*a)
+        seen.append(w.data_ptr())
+        return w
+
+    plan._workspace = watched
+    O = torch.empty_like(p.Q)
+    torch.cuda.synchronize()
+    try:
+        engine.set_stream(side.cuda_stream)
+        plan.forward(p.Q, p.K, p.V, O, flags=api.FLAG_ASYNC)
+        assert torch.empty(plan._bytes[0], dtype=torch.uint8, device="cuda").data_ptr() != seen[0]
+        engine.sync()
+        o, _, tol, _ = p.forward()
+        within(O, o, tol)
+        engine.set_stream(0)
+        with pytest.raises(ValueError):
+            plan.forward(p.Q, p.K, p.V, O)
+    finally:
+        engine.set_stream(None)
+    plan.close()
+
+
 def test_backward_in_a_graph(engine):
     p = Problem(BF16, 64, 4, 2, [150, 40], window=(-1, 0))
     plan, O, l = _forward(engine, p)
