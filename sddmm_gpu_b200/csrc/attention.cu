@@ -3,8 +3,10 @@
 
 #include <climits>
 #include <cmath>
+#include <initializer_list>
 #include <new>
 #include <string>
+#include <utility>
 
 #include "attention.cuh"
 #include "device_guard.hpp"
@@ -58,6 +60,17 @@ int check_array(sddmm_handle_s *h, const sddmm_head_array *a, const char *name, 
     return SDDMM_OK;
 }
 
+// Whether an array that is written starts where one of `others` does (arrays without rows are nobody's).
+bool same_start(const HeadArray &w, int64_t rows, std::initializer_list<std::pair<const HeadArray *, int64_t>> others)
+{
+    for (const auto &o : others)
+        if (rows > 0 && o.second > 0 && w.data == o.first->data) return true;
+    return false;
+}
+constexpr const char *OVERLAP = "an array that is written is also read, or written as another";
+// Of offsets, lengths, slopes and lse: 32-bit values in memory of the handle's GPU.
+bool words_on_device(const void *p, int device) { return (uintptr_t)p % 4 == 0 && on_device(p, device); }
+
 // delta of the backward pass, first in its workspace
 int64_t delta_bytes(const AttentionParams &p) { return ((int64_t)sizeof(float) * p.q_heads * p.q_rows + 15) / 16 * 16; }
 
@@ -101,11 +114,11 @@ int sddmm_attention_plan(sddmm_handle_t h, const sddmm_attention_desc *d, sddmm_
     if (!(d->softcap >= 0.f) || !std::isfinite(d->softcap)) return bad(h, "softcap must be 0 (none) or positive and finite");
     if (d->window_left < -1 || d->window_right < -1) return bad(h, "a window's side is -1 (no limit), 0 or positive");
     DeviceGuard guard(h->device);
-    if (d->n_seqs > 0 && !on_device(d->q_offsets, h->device)) return bad(h, "q_offsets must be device memory of the handle's GPU");
+    if (d->n_seqs > 0 && !words_on_device(d->q_offsets, h->device)) return bad(h, "q_offsets must be aligned device memory of the handle's GPU");
     if (d->k_len && !d->k_offsets) return bad(h, "k_len goes with k_offsets");
     const void *more[] = {d->k_offsets, d->k_len, d->prefix, d->slopes};
     for (const void *x : more)
-        if (x && d->n_seqs > 0 && !on_device(x, h->device)) return bad(h, "k_offsets, k_len, prefix and slopes must be device memory of the handle's GPU");
+        if (x && d->n_seqs > 0 && !words_on_device(x, h->device)) return bad(h, "k_offsets, k_len, prefix and slopes must be aligned device memory of the handle's GPU");
     AttentionParams p{};
     p.dtype = d->dtype;
     p.head_dim = d->head_dim;
@@ -181,7 +194,8 @@ int sddmm_attention_forward(sddmm_attention_t a, const sddmm_head_array *Q, cons
     if ((st = check_array(h, K, "K", p.dtype, p.head_dim, p.kv_heads, p.k_rows, false, &p.k))) return st;
     if ((st = check_array(h, V, "V", p.dtype, p.head_dim, p.kv_heads, p.k_rows, false, &p.v))) return st;
     if ((st = check_array(h, O, "O", p.dtype, p.head_dim, p.q_heads, p.q_rows, true, &p.o))) return st;
-    if (lse && p.q_rows > 0 && !on_device(lse, h->device)) return bad(h, "lse must be device memory of the handle's GPU");
+    if (same_start(p.o, p.q_rows, {{&p.q, p.q_rows}, {&p.k, p.k_rows}, {&p.v, p.k_rows}})) return bad(h, OVERLAP);
+    if (lse && p.q_rows > 0 && !words_on_device(lse, h->device)) return bad(h, "lse must be aligned device memory of the handle's GPU");
     p.lse = lse;
     int64_t need = 0;
     sddmm_attention_workspace(a, 0, &need);
@@ -222,7 +236,11 @@ int sddmm_attention_backward(sddmm_attention_t a, const sddmm_head_array *Q, con
     if ((st = check_array(h, dQ, "dQ", p.dtype, p.head_dim, p.q_heads, p.q_rows, true, &p.dq))) return st;
     if ((st = check_array(h, dK, "dK", p.dtype, p.head_dim, p.kv_heads, p.k_rows, true, &p.dk))) return st;
     if ((st = check_array(h, dV, "dV", p.dtype, p.head_dim, p.kv_heads, p.k_rows, true, &p.dv))) return st;
-    if (p.q_rows > 0 && !on_device(lse, h->device)) return bad(h, "lse must be device memory of the handle's GPU");
+    const std::initializer_list<std::pair<const HeadArray *, int64_t>> read = {{&p.q, p.q_rows}, {&p.k, p.k_rows}, {&p.v, p.k_rows}, {&p.o, p.q_rows}, {&p.d_o, p.q_rows}};
+    if (same_start(p.dq, p.q_rows, read) || same_start(p.dk, p.k_rows, read) || same_start(p.dv, p.k_rows, read) ||
+        same_start(p.dq, p.q_rows, {{&p.dk, p.k_rows}, {&p.dv, p.k_rows}}) || same_start(p.dk, p.k_rows, {{&p.dv, p.k_rows}}))
+        return bad(h, OVERLAP);
+    if (p.q_rows > 0 && !words_on_device(lse, h->device)) return bad(h, "lse must be aligned device memory of the handle's GPU");
     p.lse = const_cast<float *>(lse);
     int64_t need = 0;
     sddmm_attention_workspace(a, 1, &need);

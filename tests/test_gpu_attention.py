@@ -512,6 +512,30 @@ def test_refusals(engine):
     plan.close()
 
 
+def test_refused_pointers(engine):
+    p = Problem(F32, 64, 2, 2, [16], window=(-1, 0))
+    plan = p.plan(engine)
+    O, l = torch.empty_like(p.Q), torch.empty((2, 17), device="cuda")
+    forward = api.lib().sddmm_attention_forward
+    q, k, v, o = (_array(t.data_ptr(), t.stride(0), t.stride(1)) for t in (p.Q, p.K, p.V, O))
+    w = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    assert forward(plan._a, q, k, v, o, l.data_ptr() + 2, w.data_ptr(), 1 << 20, 0) == api.INVALID_ARG  # not aligned
+    for x in (q, k, v):
+        assert forward(plan._a, q, k, v, x, None, w.data_ptr(), 1 << 20, 0) == api.INVALID_ARG          # written and read
+    assert forward(plan._a, q, k, k, o, l.data_ptr(), w.data_ptr(), 1 << 20, 0) == api.OK               # K as V is fine
+    grads = [torch.empty_like(p.Q) for _ in range(3)]
+    dq, dk, dv = (_array(t.data_ptr(), t.stride(0), t.stride(1)) for t in grads)
+    do = _array(p.dO.data_ptr(), p.dO.stride(0), p.dO.stride(1))
+    for g in [(do, dk, dv), (dq, q, dv), (dq, dk, o), (dq, dq, dv), (dq, dk, dk), (dv, dk, dv)]:
+        assert api.lib().sddmm_attention_backward(plan._a, q, k, v, o, l.data_ptr(), do, *g, w.data_ptr(), 1 << 20, 0) == api.INVALID_ARG
+    assert api.lib().sddmm_attention_backward(plan._a, q, k, v, o, l.data_ptr(), do, dq, dk, dv, w.data_ptr(), 1 << 20, 0) == api.OK
+    desc = api.AttentionDesc.from_buffer_copy(plan.desc)
+    desc.q_offsets = p.q_offsets.data_ptr() + 1
+    a = C.c_void_p()
+    assert api.lib().sddmm_attention_plan(engine._h, C.byref(desc), C.byref(a)) == api.INVALID_ARG
+    plan.close()
+
+
 def test_nothing_to_do(engine):
     for q, k in [([], []), ([0], [5]), ([0, 0], [0, 0])]:
         p = Problem(BF16, 64, 2, 2, q, k)
