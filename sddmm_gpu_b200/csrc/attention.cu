@@ -147,8 +147,10 @@ int sddmm_attention_plan(sddmm_handle_t h, const sddmm_attention_desc *d, sddmm_
     if (!a) return SDDMM_OUT_OF_MEMORY;
     a->h = h;
     a->p = p;
-    // (a cap beyond a million times the scale: its tanh is left to the general kernels' own)
-    a->tensor_cores = p.dtype != SDDMM_F32 && (p.cap == 0.f || p.scale / p.cap >= 1e-6f);
+    // (a cap that is not within a factor of a million of the scale: its tanh, whose factors might leave fp32's range here, is left to the
+    // general kernels' own; a scale beyond that: likewise)
+    const float of_cap = p.cap == 0.f ? 1.f : p.scale / p.cap;
+    a->tensor_cores = p.dtype != SDDMM_F32 && of_cap >= 1e-6f && of_cap <= 1e6f && p.scale <= 1e6f;
     if (a->tensor_cores) {
         a->few = plan_attention_few_tc(p, h->sm_count);
         a->prompt = plan_attention_forward_tc(p, h->sm_count);

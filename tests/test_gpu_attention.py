@@ -106,6 +106,16 @@ def test_caps_small_and_large(engine, dtype, cap, q, k):
     _check_backward(engine, p).close()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("cap", [1e-4, 1e-9, 1e-38])
+@pytest.mark.parametrize("q,k", [([40, 200], [90, 200]), ([1, 1], [700, 33])])
+def test_caps_next_to_nothing(engine, dtype, cap, q, k):
+    # all scores are +-cap, and 0 where the product is: equal weights
+    p = Problem(dtype, 64, 4, 2, q, k, window=(-1, 0), cap=cap)
+    p.Q[0] = 0
+    _check_forward(engine, p)[0].close()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_many_sequences(engine, dtype):
     g = torch.Generator().manual_seed(2)
