@@ -156,14 +156,10 @@ int sddmm_attention_plan(sddmm_handle_t h, const sddmm_attention_desc *d, sddmm_
         a->prompt = plan_attention_forward_tc(p, h->sm_count);
         a->by_few = a->few.n_splits > 0 && a->few.us < a->prompt.us;
     }
+    if (!a->tensor_cores) a->prompt = plan_attention_forward_general(p, h->sm_count);
     if (p.dtype == SDDMM_F32) {
         a->few = plan_attention_few_f32(p, h->sm_count);
-        // The general kernel's 64 queries take 6.5 us for 64 keys of 64 columns, 10 of 128, on a multiprocessor of their own; every further block
-        // that shares it a quarter more.  (us, general / few: a token of 32 / 8 heads over 8,000 keys 1,243 / 33, 500 queries of 8 heads of 64
-        // on as many keys 57 / 58, 1,000 on 1,000 107 / 152.)
-        const int64_t blocks = p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, 64), waves = (blocks + h->sm_count - 1) / h->sm_count;
-        const double general = 5. + (0.75 + 0.25 * (double)waves) * (double)((p.max_k + 63) / 64) * (p.head_dim <= 64 ? 6.5 : 10.);
-        a->by_few = a->few.n_splits > 0 && a->few.us < general;
+        a->by_few = a->few.n_splits > 0 && a->few.us < a->prompt.us;
     }
     a->parts = p.dtype == SDDMM_F32 ? plan_attention_parts(p, 64, 4, h->sm_count) : plan_attention_parts(p, 128, 1, h->sm_count);
     *out = a;
@@ -216,7 +212,8 @@ int sddmm_attention_forward(sddmm_attention_t a, const sddmm_head_array *Q, cons
         const cudaError_t e = launch_attention_few_f32(p, a->few, workspace, &taken, h->stream);
         if (taken) return finish(a, e, "attention_few_f32", a->few.n_splits > 1 ? 2 : 1, flags);
     }
-    return finish(a, launch_attention_forward_general(p, h->stream), "attention_general", 1, flags);
+    const ForwardPlan one{1, 1 << 30, 0, 0.}, &f = a->tensor_cores || a->by_few ? one : a->prompt;
+    return finish(a, launch_attention_forward_general(p, f, workspace, h->stream), "attention_general", f.n_splits > 1 ? 2 : 1, flags);
 }
 
 int sddmm_attention_backward(sddmm_attention_t a, const sddmm_head_array *Q, const sddmm_head_array *K, const sddmm_head_array *V,

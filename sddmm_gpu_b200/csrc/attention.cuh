@@ -152,9 +152,10 @@ __device__ __forceinline__ Chunks<KEYS> chunks_of(const AttentionParams &p, cons
     c.n = max(1, (c.keys.n + p.chunk_tiles - 1) / p.chunk_tiles);
     return c;
 }
-// Adds up parts: of the kernels of few rows, or of the prompt kernel, whose blocks have 256 queries and go through tiles of 128 keys.
-constexpr int PROMPT_QUERIES = 256, PROMPT_KEYS = 128;
-enum JoinOf { JOIN_FEW, JOIN_PROMPT, JOIN_FEW_F32 };
+// Adds up parts: of the kernels of few rows, of the prompt kernel, whose blocks have 256 queries and go through tiles
+// of 128 keys, or of the general one, with 64 of both.
+constexpr int PROMPT_QUERIES = 256, PROMPT_KEYS = 128, GENERAL_ROWS = 64;
+enum JoinOf { JOIN_FEW, JOIN_PROMPT, JOIN_FEW_F32, JOIN_GENERAL };
 cudaError_t launch_attention_join(const AttentionParams &p, JoinOf of, cudaStream_t s);
 
 // Launches of one call behind one another: a kernel is set up while the one before it ends.  Every block of such a kernel calls
@@ -178,7 +179,8 @@ inline cudaError_t launch_behind(void (*kernel)(Args...), unsigned grid, unsigne
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-cudaError_t launch_attention_forward_general(const AttentionParams &p, cudaStream_t s);
+ForwardPlan plan_attention_forward_general(const AttentionParams &p, int sm_count);
+cudaError_t launch_attention_forward_general(const AttentionParams &p, const ForwardPlan &f, void *workspace, cudaStream_t s);
 // Where the blocks of a backward kernel alone would leave multiprocessors idle, the tiles that a block goes through are cut into parts, a
 // block each, which leave their sums in the workspace (parts x rows x heads x head_dim, dK and dV behind one another) for
 // launch_attention_sum_parts().  Most parts of a block, tiles of a part, bytes of the sums (16-byte aligned, p.part_o).

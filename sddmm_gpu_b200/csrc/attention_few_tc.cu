@@ -293,9 +293,10 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttentionPara
     const Sequence s = sequence_of(p, seq);
     int n = 0;
     if (i >= s.nq) {
-    } else if (OF == JOIN_PROMPT) {
-        const int i0 = i / PROMPT_QUERIES * PROMPT_QUERIES;
-        n = (key_tiles<PROMPT_KEYS>(reach_of(p.window, s, i0, min(s.nq, i0 + PROMPT_QUERIES))).n + p.chunk_tiles - 1) / p.chunk_tiles;
+    } else if (OF == JOIN_PROMPT || OF == JOIN_GENERAL) {
+        constexpr int ROWS_OF = OF == JOIN_PROMPT ? PROMPT_QUERIES : GENERAL_ROWS, KEYS_OF = OF == JOIN_PROMPT ? PROMPT_KEYS : GENERAL_ROWS;
+        const int i0 = i / ROWS_OF * ROWS_OF;
+        n = (key_tiles<KEYS_OF>(reach_of(p.window, s, i0, min(s.nq, i0 + ROWS_OF))).n + p.chunk_tiles - 1) / p.chunk_tiles;
     } else {
         const int rows = OF == JOIN_FEW ? FEW_ROWS : few_rows_f32(p);
         n = chunks_of<OF == JOIN_FEW ? FEW_KEYS : FEW_F32_KEYS>(p, s, (i * p.group + head % p.group) / rows, rows).n;
@@ -431,7 +432,7 @@ ForwardPlan plan_attention_few_tc(const AttentionParams &p, int sm_count)
 
 cudaError_t launch_attention_join(const AttentionParams &p, JoinOf of, cudaStream_t s)
 {
-    if (p.dtype == 0) return launch_join<float, JOIN_FEW_F32>(p, s);
+    if (p.dtype == 0) return of == JOIN_GENERAL ? launch_join<float, JOIN_GENERAL>(p, s) : launch_join<float, JOIN_FEW_F32>(p, s);
     if (of == JOIN_PROMPT) return p.dtype == 1 ? launch_join<__half, JOIN_PROMPT>(p, s) : launch_join<__nv_bfloat16, JOIN_PROMPT>(p, s);
     return p.dtype == 1 ? launch_join<__half, JOIN_FEW>(p, s) : launch_join<__nv_bfloat16, JOIN_FEW>(p, s);
 }

@@ -6,10 +6,15 @@
 // eight neighbouring rows then meet all banks).  The gradients are two kernels, each with the scores anew: dQ (which also leaves
 // delta_i = dO_i.O_i for the other) and dK, dV, which sums over the query heads of its group.  No atomics: results do not
 // depend on scheduling.
+// The forward kernel in fp32 cuts the keys into parts where its blocks leave multiprocessors idle; attention_join_kernel adds them up.
 // A tile's copies are asked for as soon as the last one in its place has been used, and come in under the product in between.
 //
 // What bounds it: the FMA pipe and the shared-memory loads that feed it (two 128-bit loads per 16 FMAs).  fp32, 1,900 + 1,333 tokens that
 // see their past and a prefix of 500, 8 heads of 64: 268 us, 22.5 TFLOP/s; gradient of 701 + 950 tokens, 4 / 2 heads of 80: 201 us, 11.7.
+#include <climits>
+#include <cmath>
+#include <type_traits>
+
 #include "attention_strict.cuh"
 #include "device_utils.cuh"
 
@@ -17,7 +22,7 @@ namespace sddmm {
 
 namespace {
 
-constexpr int B = 64, THREADS = 256, PS = B + 4;
+constexpr int B = GENERAL_ROWS, THREADS = 256, PS = B + 4;
 
 // Rows [row0, row0 + n) of one head into shared memory, zeros behind row n; a row of D columns has `stride` = D + 4 floats.  fp32 rows with
 // 16-byte alignment come by asynchronous copies, which the caller waits for (arrived()); others have been stored when this returns.
@@ -155,7 +160,8 @@ __device__ __forceinline__ void collect(unsigned long long *bits, bool bad, int 
     if (bad) atomicOr(bits, 1ull << row);
 }
 
-template <class T, int DP>
+// PARTS: the keys of a block may be cut (a form of its own: what it has to remember costs the other 4 %).
+template <class T, int DP, bool PARTS>
 __global__ void __launch_bounds__(THREADS, 2) attention_forward_general_kernel(const AttentionParams p)
 {
     extern __shared__ float sm[];
@@ -165,15 +171,19 @@ __global__ void __launch_bounds__(THREADS, 2) attention_forward_general_kernel(c
     const int stride = p.head_dim + 4;
     float *sq = sm, *sk = sq + B * stride, *sv = sk + B * stride, *sp = sv + B * stride;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, head = blockIdx.x % p.q_heads, kv = head / p.group;
+    const unsigned splits = PARTS ? p.n_splits : 1, behind = (gridDim.x - 1 - blockIdx.x) / p.q_heads, part = PARTS ? behind % splits : 0;
+    if (PARTS) next_kernel_may_come();
     Sequence s;
     int seq, block;
     // the last blocks of a causal sequence have the most keys: they go first
-    if (!find_block<B>(p, (gridDim.x - 1 - blockIdx.x) / p.q_heads, false, s, seq, block)) return;
+    if (!find_block<B>(p, behind / splits, false, s, seq, block)) return;
     const int i0 = block * B, n = min(B, s.nq - i0);
-    const float slope = p.slopes ? __ldg(p.slopes + head) : 0.f;
-    load_rows<T>(sq, p.q, (int64_t)s.q0 + i0, n, head, p.head_dim, stride);
     const Reach reach = reach_of(p.window, s, i0, i0 + n);
     const KeyTiles tiles = key_tiles<B>(reach);
+    const Part mine = PARTS ? part_of(p, tiles.n, part) : Part{0, tiles.n, true};
+    if (PARTS && mine.end < 0) return;
+    const float slope = p.slopes ? __ldg(p.slopes + head) : 0.f;
+    load_rows<T>(sq, p.q, (int64_t)s.q0 + i0, n, head, p.head_dim, stride);
     Quad o[4][DP / 64] = {};
     float top[4], sum[4];
 #pragma unroll
@@ -182,8 +192,8 @@ __global__ void __launch_bounds__(THREADS, 2) attention_forward_general_kernel(c
         const int j0 = tiles.tile(t) * B;
         load_rows<T>(to, a, (int64_t)s.k0 + j0, min(B, s.nk - j0), kv, p.head_dim, stride);
     };
-    if (tiles.n > 0) fetch(sk, p.k, 0), fetch(sv, p.v, 0);
-    for (int t = 0; t < tiles.n; ++t) {
+    if (tiles.n > 0) fetch(sk, p.k, mine.first), fetch(sv, p.v, mine.first);
+    for (int t = mine.first; t < mine.end; ++t) {
         const int j0 = tiles.tile(t) * B;
         arrived<1>();  // K, and Q
         __syncthreads();
@@ -221,7 +231,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_forward_general_kernel(c
         }
         arrived<0>();  // V
         __syncthreads();
-        const bool more = t + 1 < tiles.n;
+        const bool more = t + 1 < mine.end;
         if (more) fetch(sk, p.k, t + 1);  // under the product with V
         weights_times_rows<DP>(o, sp, sv, ty, tx, stride);
         __syncthreads();
@@ -233,6 +243,17 @@ __global__ void __launch_bounds__(THREADS, 2) attention_forward_general_kernel(c
         if (i >= n) continue;
         const float inv = sum[r] > 0.f ? 1.f / sum[r] : sum[r] == 0.f ? 0.f : NAN;
         const int64_t row = (int64_t)s.q0 + i0 + i;
+        if (PARTS && !mine.alone) {  // for attention_join_kernel, which also looks after what is not finite
+            const int64_t at = (part * p.q_rows + row) * p.q_heads + head;
+#pragma unroll
+            for (int c = 0; c < DP / 64; ++c) {
+                const float4 v = open(o[r][c]);
+                if (4 * tx + 64 * c < p.head_dim)
+                    *reinterpret_cast<float4 *>(p.part_o + at * p.head_dim + 4 * tx + 64 * c) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+            }
+            if (tx == 0) p.part_lse[at] = sum[r] == 0.f ? -INFINITY : top[r] * LOG2E + log2f(sum[r]);
+            continue;
+        }
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
             const float4 v = open(o[r][c]);
@@ -522,7 +543,11 @@ cudaError_t forward_of(const AttentionParams &p, cudaStream_t s)
 {
     static SmemOptinCache optin;
     const unsigned grid = (unsigned)(p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, B));
-    return launch(attention_forward_general_kernel<T, DP>, optin, grid, smem_of(p.head_dim, 3, 1), p, s);
+    if constexpr (std::is_same<T, float>::value) {
+        static SmemOptinCache optin_parts;
+        if (p.n_splits > 1) return launch(attention_forward_general_kernel<T, DP, true>, optin_parts, grid * p.n_splits, smem_of(p.head_dim, 3, 1), p, s);
+    }
+    return launch(attention_forward_general_kernel<T, DP, false>, optin, grid, smem_of(p.head_dim, 3, 1), p, s);
 }
 template <class T, int DP>
 cudaError_t backward_of(const AttentionParams &p0, const Parts &parts, cudaStream_t s)
@@ -595,7 +620,38 @@ cudaError_t launch_attention_sum_parts(const AttentionParams &p, bool kv, int ti
     return run(attention_sum_parts_kernel<__nv_bfloat16, true, 128>, attention_sum_parts_kernel<__nv_bfloat16, false, 128>);
 }
 
-cudaError_t launch_attention_forward_general(const AttentionParams &p, cudaStream_t s) { return by_type(nullptr, p, s); }
+ForwardPlan plan_attention_forward_general(const AttentionParams &p, int sm_count)
+{
+    // fp32 alone: 16-bit types come here for strides and alignment, which a plan does not know
+    const int64_t tiles = p.max_k > 0 ? (p.max_k + B - 1) / B : 1, blocks = p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, B);
+    const int64_t bytes = p.q_rows * p.q_heads * (int64_t)(p.head_dim + 1) * 4, rows = p.q_rows * p.q_heads;
+    const bool narrow = p.head_dim <= 64;
+    const int resident = narrow ? 2 : 1;  // blocks on a multiprocessor, by shared memory
+    ForwardPlan best{1, 1 << 30, 0, INFINITY};
+    for (int64_t n = 1; n <= 128 && (n == 1 || (n <= tiles / 2 && n * bytes <= 256ll << 20)); ++n) {
+        const int64_t each = (tiles + n - 1) / n;
+        if (n > 1 && (p.dtype != 0 || (tiles + each - 1) / each != n || (int64_t)p.n_seqs * p.max_q * p.q_heads > INT32_MAX)) continue;
+        // A tile of 64 keys takes 6.5 us of a block alone, 7.7 of two together, of 128 columns 10; the join 6 and one for 800 rows.  (us, one part /
+        // parts: 64 queries on 2,000 keys, 8 heads of 64, 209 / 23; 1,000 on 1,000 107 / 78, of 128 165 / 107; where blocks fill the GPU
+        // anyway, 1,900 + 1,333 tokens, 268 / 342.)
+        // Waves: whole ones where all blocks have as much to do, else the short ones fill the last.
+        const double full = (double)(blocks * n) / (resident * sm_count), fill = p.window.right >= 0 && p.max_k < 2ll * p.max_q ? full : ceil(full), us = 5. + (n > 1 ? 6. + rows / 800. : 0.) +
+                            (fill > 1. ? fill : 1.) * each * (!narrow ? 10. : blocks * n > sm_count ? 7.7 : 6.5);
+        if (us < best.us) best = ForwardPlan{(int)n, n == 1 ? 1 << 30 : (int)each, n == 1 ? 0 : n * bytes, us};
+    }
+    return best;
+}
+
+cudaError_t launch_attention_forward_general(const AttentionParams &p0, const ForwardPlan &f, void *workspace, cudaStream_t s)
+{
+    AttentionParams p = p0;
+    p.n_splits = f.n_splits;
+    p.chunk_tiles = f.chunk_tiles;
+    p.part_o = static_cast<float *>(workspace);
+    p.part_lse = p.part_o + (f.n_splits == 1 ? 0 : (int64_t)f.n_splits * p.q_rows * p.q_heads * p.head_dim);
+    const cudaError_t e = by_type(nullptr, p, s);
+    return e == cudaSuccess && p.n_splits > 1 ? launch_attention_join(p, JOIN_GENERAL, s) : e;
+}
 cudaError_t launch_attention_backward_general(const AttentionParams &p, const Parts &parts, cudaStream_t s) { return by_type(&parts, p, s); }
 
 }  // namespace sddmm

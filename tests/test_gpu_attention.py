@@ -183,6 +183,30 @@ def test_few_queries_in_fp32(engine, d, hq, hkv, q, k, mask):
     plan.close()
 
 
+@pytest.mark.parametrize("mask", range(len(MASKS)))
+@pytest.mark.parametrize("d,hq,hkv,q,k", [(64, 4, 2, [200, 64, 0, 129], [1500, 900, 7, 129]), (104, 2, 1, [400], [1100]), (128, 2, 2, [65, 300], [600, 300])])
+def test_keys_in_parts_in_fp32(engine, d, hq, hkv, q, k, mask):
+    p = Problem(F32, d, hq, hkv, q, k, seed=mask + 1, gain=2.0, extra_rows=3, **MASKS[mask])
+    plan, _, _ = _check_forward(engine, p)
+    assert plan.last_kernel_name() == "attention_general" and plan._bytes[0] > 0
+    plan.close()
+
+
+@pytest.mark.parametrize("value", [NAN, math.inf, -math.inf])
+def test_keys_in_parts_in_fp32_masked_places(engine, value):
+    p = Problem(F32, 64, 4, 2, [200], [1500], window=(300, 0), prefix=5)
+    o, lse, tol_o, tol_l = p.forward()
+    for x in (p.K, p.V):
+        x[5:1000] = value                  # hidden from all
+        x[1499] = value                    # seen by the last row alone
+    plan, O, l = _forward(engine, p)
+    assert plan.last_kernel_name() == "attention_general" and plan._bytes[0] > 0
+    within(O[:199], o[:199], tol_o[:199], "O")
+    within(l[:, :199], lse[:, :199], tol_l[:, :199], "lse")
+    assert not bool(O[199].isfinite().all())
+    plan.close()
+
+
 @pytest.mark.parametrize("value", [NAN, math.inf, -math.inf])
 def test_few_queries_in_fp32_masked_places(engine, value):
     p = Problem(F32, 64, 4, 2, [1, 2], [3000, 2500], window=(700, 0), prefix=5)
