@@ -203,7 +203,7 @@ SDDMM_API int sddmm_fused_execute(sddmm_plan_t p, const float *W, const float *H
  *
  * Query head h reads KV head h / (q_heads / kv_heads).  Operands are fp32, fp16 or bfloat16, all of one type; products, softmax and sums
  * are fp32; weights are rounded to the operands' type before the product with V where the kernel is a tensor-core one
- * (fp16, bfloat16).  head_dim: a multiple of 8 up to 128.
+ * (fp16, bfloat16; not those of few queries on many keys).  head_dim: a multiple of 8 up to 128.
  */
 enum { SDDMM_F32 = 0, SDDMM_F16 = 1, SDDMM_BF16 = 2 };
 typedef struct sddmm_attention_s *sddmm_attention_t;

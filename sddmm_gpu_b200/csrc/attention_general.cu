@@ -65,7 +65,7 @@ __device__ __forceinline__ void rows_times_rows(float (&acc)[4][4], const float 
 {
     F2 sum[4][4] = {};
     const int stride = D + 4;
-#pragma unroll 2
+#pragma unroll 4
     for (int d = 0; d < D; d += 4) {
         ulonglong2 a[4], b[4];
 #pragma unroll
@@ -103,7 +103,7 @@ __device__ __forceinline__ void add_times(Quad &acc, float w, ulonglong2 v)
 template <int DP>
 __device__ __forceinline__ void weights_times_rows(Quad (&acc)[4][DP / 64], const float *w, const float *x, int ty, int tx, int stride)
 {
-#pragma unroll 2
+#pragma unroll 4
     for (int j = 0; j < B; j += 4) {
         float4 p[4];
 #pragma unroll
@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_forward_general_kernel(c
         const int j0 = tiles.tile(t) * B;
         arrived<1>();  // K, and Q
         __syncthreads();
+        const bool all = tile_is_open<B>(p.window, s, reach, j0);  // nothing is hidden here
         float x[4][4];
         rows_times_rows(x, sq, sk, ty, tx, p.head_dim);
 #pragma unroll
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_forward_general_kernel(c
             for (int c = 0; c < 4; ++c) {
                 const int j = j0 + tx + 16 * c;
                 const float v = score(p, slope, x[r][c], pos, j, unused);
-                x[r][c] = key_seen(p.window, s, pos, j) ? v : -INFINITY;
+                x[r][c] = all || key_seen(p.window, s, pos, j) ? v : -INFINITY;
                 most = fmaxf(most, x[r][c]);
             }
             const float now = fmaxf(top[r], over16(most, false));
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_forward_general_kernel(c
                 add += e;
                 sp[(ty + 16 * r) * PS + tx + 16 * c] = e;
             }
-            sum[r] = sum[r] * shrink + over16(add, true);
+            sum[r] = sum[r] * shrink + add;  // (of this thread's columns)
             top[r] = now;
 #pragma unroll
             for (int c = 0; c < DP / 64; ++c) {
@@ -237,6 +238,8 @@ __global__ void __launch_bounds__(THREADS, 2) attention_forward_general_kernel(c
         __syncthreads();
         if (more) fetch(sv, p.v, t + 1);  // under the next scores
     }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sum[r] = over16(sum[r], true);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int i = ty + 16 * r;
@@ -325,6 +328,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dq_general_kernel(const 
     if (mine.first < mine.end) fetch(sv, p.v, mine.first), fetch(sk, p.k, mine.first);
     for (int t = mine.first; t < mine.end; ++t) {
         const int j0 = tiles.tile(t) * B;
+        const bool all = tile_is_open<B>(p.window, s, reach, j0);
         float x[4][4], dp[4][4];
         arrived<1>();
         __syncthreads();
@@ -341,7 +345,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dq_general_kernel(const 
                 float dcap;
                 const float v = score(p, slope, x[r][c], pos, j, dcap);
                 float ds = 0.f;
-                if (lse[r] != -INFINITY && key_seen(p.window, s, pos, j)) ds = exp2f((v - lse[r]) * LOG2E) * (dp[r][c] - delta[r]) * dcap * p.scale;
+                if (lse[r] != -INFINITY && (all || key_seen(p.window, s, pos, j))) ds = exp2f((v - lse[r]) * LOG2E) * (dp[r][c] - delta[r]) * dcap * p.scale;
                 sds[(ty + 16 * r) * PS + tx + 16 * c] = ds;
             }
         }
@@ -410,7 +414,15 @@ __global__ void __launch_bounds__(THREADS) attention_dkv_general_kernel(const At
     for (int t = mine.first; t < mine.end; ++t) {
         const int head = kv * p.group + t / per_head, i0 = (from + t % per_head) * B, n = min(B, s.nq - i0);
         const float slope = p.slopes ? __ldg(p.slopes + head) : 0.f;
-        float x[4][4], dp[4][4];
+        float x[4][4], dp[4][4], lse[4], delta[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {  // (on their way under the products)
+            const int i = ty + 16 * r;
+            const int64_t at = (int64_t)head * p.q_rows + s.q0 + i0 + i;
+            lse[r] = i < n ? __ldg(p.lse + at) : -INFINITY;
+            delta[r] = i < n ? p.delta[at] : 0.f;
+        }
+        const bool all = n == B && tile_is_open<B>(p.window, s, reach_of(p.window, s, i0, i0 + n), j0);
         arrived<1>();
         __syncthreads();
         rows_times_rows(dp, sdo, sv, ty, tx, p.head_dim);
@@ -420,17 +432,15 @@ __global__ void __launch_bounds__(THREADS) attention_dkv_general_kernel(const At
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int i = ty + 16 * r, pos = s.nk - s.nq + i0 + i;
-            const int64_t at = (int64_t)head * p.q_rows + s.q0 + i0 + i;
-            const float lse = i < n ? __ldg(p.lse + at) : -INFINITY, delta = i < n ? p.delta[at] : 0.f;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int j = j0 + tx + 16 * c;
                 float dcap;
                 const float v = score(p, slope, x[r][c], pos, j, dcap);
                 float e = 0.f, ds = 0.f;
-                if (lse != -INFINITY && key_seen(p.window, s, pos, j)) {
-                    e = exp2f((v - lse) * LOG2E);
-                    ds = e * (dp[r][c] - delta) * dcap * p.scale;
+                if (lse[r] != -INFINITY && (all || key_seen(p.window, s, pos, j))) {
+                    e = exp2f((v - lse[r]) * LOG2E);
+                    ds = e * (dp[r][c] - delta[r]) * dcap * p.scale;
                 }
                 sp[i * PS + tx + 16 * c] = e;
                 sds[i * PS + tx + 16 * c] = ds;
