@@ -8,7 +8,7 @@
 // up to 8: single tokens with heads of their own would spend eight times the FMAs on one row.
 //
 // What bounds it: memory for a row or two (32 tokens of 8 heads of 128 over 4,000 keys each: 161 us, 6.5 TB/s); FMAs and shared memory for 8
-// (200 queries, 8 heads of 128 on one, 8,000 keys: 419 us, where the general kernel in parts takes 297); beginning, ending and the join for short caches (a token of 32 / 8 heads, 8,000
+// (200 queries, 8 heads of 128 on one, 8,000 keys: 419 us, where the general kernel in parts takes 264); beginning, ending and the join for short caches (a token of 32 / 8 heads, 8,000
 // keys: 27 us, of which 10 are memory).  Twelve warps with one tile each of K and V instead of four with two: 710 -> 161, 1,109 -> 419, 51 -> 33.
 #include <cmath>
 

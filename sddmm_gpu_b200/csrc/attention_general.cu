@@ -10,7 +10,7 @@
 // A tile's copies are asked for as soon as the last one in its place has been used, and come in under the product in between.
 //
 // What bounds it: the FMA pipe and the shared-memory loads that feed it (two 128-bit loads per 16 FMAs).  fp32, 1,900 + 1,333 tokens that
-// see their past and a prefix of 500, 8 heads of 64: 268 us, 22.5 TFLOP/s; gradient of 701 + 950 tokens, 4 / 2 heads of 80: 201 us, 11.7.
+// see their past and a prefix of 500, 8 heads of 64: 244 us, 24.7 TFLOP/s; gradient of 701 + 950 tokens, 4 / 2 heads of 80: 190 us, 12.4.
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -380,8 +380,9 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dq_general_kernel(const 
 }
 
 // dK and dV of 64 keys, over all queries of all heads of the group.
+// (Two blocks on a multiprocessor for heads of 64, which shared memory allows: 1,000 tokens of 8 heads 173 -> 159 us with dQ.)
 template <class T, int DP>
-__global__ void __launch_bounds__(THREADS) attention_dkv_general_kernel(const AttentionParams p)
+__global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1) attention_dkv_general_kernel(const AttentionParams p)
 {
     extern __shared__ float sm[];
     __shared__ unsigned long long bad;
@@ -641,8 +642,8 @@ ForwardPlan plan_attention_forward_general(const AttentionParams &p, int sm_coun
     for (int64_t n = 1; n <= 128 && (n == 1 || (n <= tiles / 2 && n * bytes <= 256ll << 20)); ++n) {
         const int64_t each = (tiles + n - 1) / n;
         if (n > 1 && (p.dtype != 0 || (tiles + each - 1) / each != n || (int64_t)p.n_seqs * p.max_q * p.q_heads > INT32_MAX)) continue;
-        // A tile of 64 keys takes 6.5 us of a block alone, 7.7 of two together, of 128 columns 10; the join 6 and one for 800 rows.  (us, one part /
-        // parts: 64 queries on 2,000 keys, 8 heads of 64, 209 / 23; 1,000 on 1,000 107 / 78, of 128 165 / 107; where blocks fill the GPU
+        // A tile of 64 keys takes 6.5 us of a block alone, 7.7 of two together, of 128 columns 10; the join 6 and one for 800 rows.  (us before tiles without masks
+        // were told apart, one part / parts: 64 queries on 2,000 keys, 8 heads of 64, 209 / 23; 1,000 on 1,000 107 / 78, of 128 165 / 107; where blocks fill the GPU
         // anyway, 1,900 + 1,333 tokens, 268 / 342.)
         // Waves: whole ones where all blocks have as much to do, else the short ones fill the last.
         const double full = (double)(blocks * n) / (resident * sm_count), fill = p.window.right >= 0 && p.max_k < 2ll * p.max_q ? full : ceil(full), us = 5. + (n > 1 ? 6. + rows / 800. : 0.) +
