@@ -382,16 +382,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                     const F2 l2 = KV ? pick(reinterpret_cast<const ulonglong2 *>(my_lse)[u / 2], u & 1) : tc::two(lse2, lse2);
                     F2 z = x[u], dcap = 0;
                     if (CAP) {
-                        F2 th;
-                        if (decltype(is_small)::value) {
-                            th = tc::tanh2(z, tanh_c);
-                        } else {
-                            float a, b;  // tanh(y) = 1 - 2 / (1 + e^2y)
-                            tc::split(z, a, b);
-                            a = fmaf(-2.f, tc::rcp(1.f + tc::ex2(a * (2.f * LOG2E * c))), 1.f);
-                            b = fmaf(-2.f, tc::rcp(1.f + tc::ex2(b * (2.f * LOG2E * c))), 1.f);
-                            th = tc::two(a, b);
-                        }
+                        const F2 th = decltype(is_small)::value ? tc::tanh2(z, tanh_c) : tc::tanh_any(z, tanh_c, c, 1.f, 0.f);
                         dcap = tc::ffma2(tc::mul2(th, th), tc::two(-1.f, -1.f), tc::two(1.f, 1.f));
                         z = BIAS ? tc::mul2(th, tc::two(top_of, top_of)) : tc::ffma2(th, tc::two(top_of, top_of), l2);
                     }

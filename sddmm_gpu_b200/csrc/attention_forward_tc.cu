@@ -303,14 +303,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
 #pragma unroll
                     for (int j = 0; j < COLUMNS / 2; ++j) x[j] = tc::tanh2(x[j], tanh_c);
                 } else {
-                    // cap tanh(y) = cap - 2 cap / (1 + e^2y)
-                    const float c2 = 2.f * LOG2E * c;
 #pragma unroll
-                    for (int j = 0; j < COLUMNS / 2; ++j) {
-                        float a, b;
-                        tc::split(x[j], a, b);
-                        x[j] = tc::two(fmaf(-2.f * top_of, tc::rcp(1.f + tc::ex2(a * c2)), top_of), fmaf(-2.f * top_of, tc::rcp(1.f + tc::ex2(b * c2)), top_of));
-                    }
+                    for (int j = 0; j < COLUMNS / 2; ++j) x[j] = tc::tanh_any(x[j], tanh_c, c, top_of, 0.f);
                 }
             }
             if (BIAS) {
@@ -397,14 +391,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                     F2 e;
                     float e0, e1;
                     if (CAP && !BIAS) {
-                        if (decltype(is_small)::value) {
-                            e = tc::ffma2(x[j], tc::tanh_over_x(x[j], tanh_c), tc::two(less, less));
-                        } else {  // cap tanh(y) = cap - 2 cap / (1 + e^2y)
-                            tc::split(x[j], e0, e1);
-                            e0 = fmaf(-2.f * top_of, tc::rcp(1.f + tc::ex2(e0 * (2.f * LOG2E * c))), top_of + less);
-                            e1 = fmaf(-2.f * top_of, tc::rcp(1.f + tc::ex2(e1 * (2.f * LOG2E * c))), top_of + less);
-                            e = tc::two(e0, e1);
-                        }
+                        if (decltype(is_small)::value) e = tc::ffma2(x[j], tc::tanh_over_x(x[j], tanh_c), tc::two(less, less));
+                        else e = tc::tanh_any(x[j], tanh_c, c, top_of, less);
                         if (!decltype(all_seen)::value) {
                             tc::split(e, e0, e1);
                             e = tc::two(seen_of[j / 16] & 1u << 2 * (j % 16) ? e0 : -INFINITY, seen_of[j / 16] & 2u << 2 * (j % 16) ? e1 : -INFINITY);

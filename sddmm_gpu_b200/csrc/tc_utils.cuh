@@ -250,6 +250,19 @@ __device__ __forceinline__ F2 tanh_over_x(F2 x, const Tanh &t)
     return p;
 }
 __device__ __forceinline__ F2 tanh2(F2 x, const Tanh &t) { return mul2(tanh_over_x(x, t), x); }
+// by tanh(c x) + more of any size, for products a few of which leave the polynomial's range: each by its own size alone, so that what comes out
+// of one does not depend on the others.  Within the range the bits are those of ffma2(x, tanh_over_x(x, t), more), `by` being in t's factors;
+// beyond it by (1 - 2 / (1 + e^2cx)).
+__device__ __forceinline__ F2 tanh_any(F2 x, const Tanh &t, float c, float by, float more)
+{
+    float a, b, u, w;
+    split(x, a, b);
+    split(ffma2(x, tanh_over_x(x, t), two(more, more)), u, w);
+    const float c2 = 2.f * LOG2E * c;
+    u = fabsf(a) <= t.range ? u : fmaf(-2.f * by, rcp(1.f + ex2(a * c2)), by + more);
+    w = fabsf(b) <= t.range ? w : fmaf(-2.f * by, rcp(1.f + ex2(b * c2)), by + more);
+    return two(u, w);
+}
 // Two values in a word, the first in its lower half.
 template <class T> __device__ __forceinline__ uint32_t pack(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b)
