@@ -12,6 +12,7 @@
 #include "device_guard.hpp"
 #include "engine_internal.hpp"
 #include "sddmm_b200.h"
+#include "tc_utils.cuh"
 
 struct sddmm_attention_s {
     sddmm_handle_s *h = nullptr;
@@ -143,13 +144,16 @@ int sddmm_attention_plan(sddmm_handle_t h, const sddmm_attention_desc *d, sddmm_
     p.status = h->d_status;
     if ((most_blocks(p.q_rows, p.n_seqs, p.max_q, 16) + 1) * p.q_heads > INT_MAX || (most_blocks(p.k_rows, p.n_seqs, p.max_k, 64) + 1) * p.q_heads > INT_MAX)
         return bad(h, "too many heads and rows for one launch");
+    // (a cap that is not within a factor of a million of the scale: its tanh, whose factors might leave fp32's range here, is left to the
+    // general kernels' own; a scale beyond that: likewise)
+    const float of_cap = p.cap == 0.f ? 1.f : p.scale / p.cap;
+    const bool reach = of_cap >= tc::TANH_LEAST && of_cap <= tc::TANH_MOST;
+    p.of_cap = reach ? of_cap : 1.f;
+    p.pre = reach ? 1.f : of_cap;
     sddmm_attention_s *a = new (std::nothrow) sddmm_attention_s;
     if (!a) return SDDMM_OUT_OF_MEMORY;
     a->h = h;
     a->p = p;
-    // (a cap that is not within a factor of a million of the scale: its tanh, whose factors might leave fp32's range here, is left to the
-    // general kernels' own; a scale beyond that: likewise)
-    const float of_cap = p.cap == 0.f ? 1.f : p.scale / p.cap;
     a->tensor_cores = p.dtype != SDDMM_F32 && of_cap >= 1e-6f && of_cap <= 1e6f && p.scale <= 1e6f;
     if (a->tensor_cores) {
         a->few = plan_attention_few_tc(p, h->sm_count);

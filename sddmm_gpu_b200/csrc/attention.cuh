@@ -38,6 +38,7 @@ struct AttentionParams {
     float *part_o, *part_lse;  // parts of a split long axis (workspace)
     int n_splits, chunk_tiles;  // chunks of the keys, at most; key tiles of one
     int *status;
+    float of_cap, pre;  // tensor-core kernels: scale / cap, and 1; where it is out of tanh_polynomial()'s reach 1, and that, as a first factor of the products
 };
 
 __device__ __forceinline__ void report_bad_index(int *dev_status)

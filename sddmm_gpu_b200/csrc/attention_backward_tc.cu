@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             asm volatile("bar.sync 1, %0;" ::"n"(ROW_WARPS * 32) : "memory");  // (all row warps come here, and nothing before can keep one)
         }
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const float c = CAP ? p.scale / p.cap : p.scale * LOG2E, top_of = p.cap * LOG2E;
+        const float c = !CAP ? p.scale * LOG2E : p.of_cap, top_of = p.cap * LOG2E;
         const tc::Tanh tanh_c = tc::tanh_polynomial(c, 1.f);
         float slope = BIAS && !KV ? __ldg(p.slopes + head) * LOG2E : 0.f;
         const int off = s.nk - s.nq;
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                     tc::split(x[u], a, b);
                     size = tc::max3_abs(size, a, b);
                 }
-                small = __all_sync(0xffffffffu, size <= tanh_c.range);
+                small = p.pre == 1.f && __all_sync(0xffffffffu, size <= tanh_c.range);
             }
             // weights into w; x leaves as weight, with a cap times 1 - tanh^2
             uint32_t w[MINE / 2];
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                     const F2 l2 = KV ? pick(reinterpret_cast<const ulonglong2 *>(my_lse)[u / 2], u & 1) : tc::two(lse2, lse2);
                     F2 z = x[u], dcap = 0;
                     if (CAP) {
-                        const F2 th = decltype(is_small)::value ? tc::tanh2(z, tanh_c) : tc::tanh_any(z, tanh_c, c, 1.f, 0.f);
+                        const F2 th = decltype(is_small)::value ? tc::tanh2(z, tanh_c) : tc::tanh_any(z, tanh_c, p.pre, c, 1.f, 0.f);
                         dcap = tc::ffma2(tc::mul2(th, th), tc::two(-1.f, -1.f), tc::two(1.f, 1.f));
                         z = BIAS ? tc::mul2(th, tc::two(top_of, top_of)) : tc::ffma2(th, tc::two(top_of, top_of), l2);
                     }

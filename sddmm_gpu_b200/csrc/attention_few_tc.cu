@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident_blocks(DP)) attention_few
         hi[x] = p.window.right < 0 ? s.nk - 1 : min(s.nk - 1, pos[x] + p.window.right);
         slope[x] = BIAS ? __ldg(p.slopes + head) * LOG2E : 0.f;
     }
-    const float c = CAP ? p.scale / p.cap : p.scale * LOG2E, top_of = p.cap * LOG2E;
+    const float c = !CAP ? p.scale * LOG2E : p.of_cap, top_of = p.cap * LOG2E;
     const tc::Tanh tanh_c = tc::tanh_polynomial(c, top_of);
     float o[DP / 8][4];
 #pragma unroll
@@ -148,12 +148,12 @@ __global__ void __launch_bounds__(WARPS * 32, resident_blocks(DP)) attention_few
             float size = 0.f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) size = tc::max3_abs(size, x[0][e], x[1][e]);
-            if (__all_sync(0xffffffffu, size <= tanh_c.range)) {
+            if (p.pre == 1.f && __all_sync(0xffffffffu, size <= tanh_c.range)) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) tc::split(tc::tanh2(tc::two(x[0][e], x[1][e]), tanh_c), x[0][e], x[1][e]);
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) tc::split(tc::tanh_any(tc::two(x[0][e], x[1][e]), tanh_c, c, top_of, 0.f), x[0][e], x[1][e]);
+                for (int e = 0; e < 4; ++e) tc::split(tc::tanh_any(tc::two(x[0][e], x[1][e]), tanh_c, p.pre, c, top_of, 0.f), x[0][e], x[1][e]);
             }
         }
 #pragma unroll

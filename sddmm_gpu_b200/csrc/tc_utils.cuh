@@ -222,8 +222,9 @@ __device__ __forceinline__ F2 ex2_poly(F2 x)
     return mul2(p, two(__uint_as_float((__float_as_uint(a) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(b) << 23) + 0x3f800000u)));
 }
 // tanh(c x) = x (a polynomial in x^2), where |c x| <= 0.6: Chebyshev interpolation of tanh(y) / y in y^2, off by 9e-8, its coefficients
-// times by c^(2i + 1).  `range` is at most 3,000: where c is so small that the last coefficients leave the normal numbers, c x is then so
-// small (0.18 at 6e-5) that their terms do not count.
+// times by c^(2i + 1).  c^9 has to stay among the normal numbers, with room for `by`: c from TANH_LEAST to TANH_MOST.  Where scale / cap is
+// not in there c is 1, and products go by tanh_any(), which multiplies them by it (AttentionParams::pre) first.
+constexpr float TANH_LEAST = 2e-4f, TANH_MOST = 1e4f;
 struct Tanh {
     F2 a[5];
     float range;  // of |x|
@@ -238,7 +239,7 @@ __device__ __forceinline__ Tanh tanh_polynomial(float c, float by)
         t.a[i] = two(C[i] * power, C[i] * power);
         power *= c * c;
     }
-    t.range = 0.6f / fmaxf(c, 2e-4f);
+    t.range = 0.6f / c;
     return t;
 }
 __device__ __forceinline__ F2 tanh_over_x(F2 x, const Tanh &t)
@@ -250,12 +251,13 @@ __device__ __forceinline__ F2 tanh_over_x(F2 x, const Tanh &t)
     return p;
 }
 __device__ __forceinline__ F2 tanh2(F2 x, const Tanh &t) { return mul2(tanh_over_x(x, t), x); }
-// by tanh(c x) + more of any size, for products a few of which leave the polynomial's range: each by its own size alone, so that what comes out
-// of one does not depend on the others.  Within the range the bits are those of ffma2(x, tanh_over_x(x, t), more), `by` being in t's factors;
-// beyond it by (1 - 2 / (1 + e^2cx)).
-__device__ __forceinline__ F2 tanh_any(F2 x, const Tanh &t, float c, float by, float more)
+// by tanh(c pre x) + more of any size, for products a few of which leave the polynomial's range: each by its own size alone, so that what comes
+// out of one does not depend on the others.  Within the range, and with pre = 1, the bits are those of ffma2(x, tanh_over_x(x, t), more), `by`
+// being in t's factors; beyond it by (1 - 2 / (1 + e^2cx)).
+__device__ __forceinline__ F2 tanh_any(F2 x, const Tanh &t, float pre, float c, float by, float more)
 {
     float a, b, u, w;
+    x = mul2(x, two(pre, pre));
     split(x, a, b);
     split(ffma2(x, tanh_over_x(x, t), two(more, more)), u, w);
     const float c2 = 2.f * LOG2E * c;

@@ -55,6 +55,42 @@ def _check(engine, p, backward=True):
     return name
 
 
+SHAPES = [([40, 200], [90, 200]), ([1, 1], [700, 33])]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("cap", [0.05, 0.7, 30.0, 3000.0, 1e5, 1e9])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("q,k", SHAPES)
+def test_caps_small_and_large(engine, dtype, cap, bias, q, k):
+    _check(engine, Capped(dtype, 64, 4, 2, q, k, window=(-1, 0), cap=cap, bias=bias, gain=3.0))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("cap", [5e-5, 5e-6, 1.5e-6, 1e-6, 5e-7, 2e-7, 1.3e-7])
+@pytest.mark.parametrize("zero", ["Q", "K", "both"])
+@pytest.mark.parametrize("q,k", SHAPES)
+def test_products_of_zero_under_tiny_caps(engine, dtype, cap, zero, q, k):
+    # equal weights, whatever the cap; the cap's slope is one
+    p = Capped(dtype, 64, 4, 2, q, k, window=(-1, 0), cap=cap)
+    if zero != "K":
+        p.Q.zero_()
+    if zero != "Q":
+        p.K.zero_()
+    _check(engine, p)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("scale,cap", [(1e-2, 1e4), (1e-3, 1e3), (2e-2, 1e3)])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("q,k", SHAPES)
+def test_large_products_far_below_their_cap(engine, dtype, scale, cap, bias, q, k):
+    # products of up to 40,000; scores of up to 400, far below the cap: as exact as without one
+    p = Capped(dtype, 8, 4, 2, q, k, window=(-1, 0), cap=cap, scale=scale, bias=bias, gain=3000.0)
+    name = _check(engine, p)
+    assert dtype == F32 or name in ("attention_tc", "attention_few_tc")
+
+
 # Products of a warp that all lie within the range of tanh's polynomial go the short way; one that does not must change nothing for the others.
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("d,hq,hkv", [(64, 4, 2), (128, 4, 4)])
