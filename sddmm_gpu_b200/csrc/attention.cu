@@ -72,8 +72,9 @@ constexpr const char *OVERLAP = "an array that is written is also read, or writt
 // Of offsets, lengths, slopes and lse: 32-bit values in memory of the handle's GPU.
 bool words_on_device(const void *p, int device) { return (uintptr_t)p % 4 == 0 && on_device(p, device); }
 
-// delta of the backward pass, first in its workspace
+// delta of the backward pass, first in its workspace, and in fp16 what its tiles of dO hold at most
 int64_t delta_bytes(const AttentionParams &p) { return ((int64_t)sizeof(float) * p.q_heads * p.q_rows + 15) / 16 * 16; }
+int64_t most_bytes(const AttentionParams &p) { return p.dtype == SDDMM_F16 ? ((int64_t)sizeof(float) * p.q_heads * most_tiles(p) + 15) / 16 * 16 : 0; }
 
 bool capturing(cudaStream_t s)
 {
@@ -179,7 +180,7 @@ int sddmm_attention_destroy(sddmm_attention_t a)
 int sddmm_attention_workspace(sddmm_attention_t a, int backward, int64_t *bytes)
 {
     if (!a || !bytes) return SDDMM_INVALID_ARG;
-    *bytes = backward ? delta_bytes(a->p) + a->parts.bytes : a->by_few ? a->few.bytes : a->prompt.bytes;
+    *bytes = backward ? delta_bytes(a->p) + most_bytes(a->p) + a->parts.bytes : a->by_few ? a->few.bytes : a->prompt.bytes;
     return SDDMM_OK;
 }
 
@@ -250,7 +251,8 @@ int sddmm_attention_backward(sddmm_attention_t a, const sddmm_head_array *Q, con
     if (need > 0 && (workspace_bytes < need || !on_device(workspace, h->device) || (uintptr_t)workspace % 16))
         return bad(h, "workspace: sddmm_attention_workspace() bytes of device memory, 16-byte aligned");
     p.delta = static_cast<float *>(workspace);
-    p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + delta_bytes(p));
+    p.d_o_most = reinterpret_cast<float *>(static_cast<char *>(workspace) + delta_bytes(p));
+    p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + delta_bytes(p) + most_bytes(p));
     if (!(flags & SDDMM_FLAG_ASYNC) && capturing(h->stream)) return bad(h, "a captured call must be asynchronous");
     if (p.n_seqs == 0 || (p.max_q == 0 && p.max_k == 0)) return SDDMM_OK;
     bool taken = false;

@@ -35,6 +35,7 @@ struct AttentionParams {
     HeadArray q, k, v, o, d_o, dq, dk, dv;
     float *lse;    // q_heads x q_rows
     float *delta;  // q_heads x q_rows, workspace of the backward pass
+    float *d_o_most;  // the same, fp16: the largest |dO| of every tile of queries of a head (tile_index())
     float *part_o, *part_lse;  // parts of a split long axis (workspace)
     int n_splits, chunk_tiles;  // chunks of the keys, at most; key tiles of one
     int *status;
@@ -210,6 +211,14 @@ __device__ __forceinline__ void query_tiles(const AttentionParams &p, const Sequ
     queries_of(p.window, s, j0, j0 + m, from, to);
     from /= T;
     per_head = to > from * T ? (to + T - 1) / T - from : 0;
+}
+// A place for every tile of 128 queries: q_rows / 128 + n_seqs a head.  (A sequence's last tile is at most as far as the next one's first row, whose own
+// tiles lie one further for their sequence's number.)
+constexpr int DO_TILE = 128;
+__host__ __device__ inline int64_t most_tiles(const AttentionParams &p) { return p.q_rows / DO_TILE + p.n_seqs; }
+__device__ __forceinline__ int64_t tile_index(const AttentionParams &p, const Sequence &s, int seq, int head, int tile)
+{
+    return head * most_tiles(p) + s.q0 / DO_TILE + seq + tile;
 }
 cudaError_t launch_attention_backward_general(const AttentionParams &p, const Parts &parts, cudaStream_t s);
 cudaError_t launch_attention_backward_tc(const AttentionParams &p, const Parts &parts, bool *taken, cudaStream_t s);

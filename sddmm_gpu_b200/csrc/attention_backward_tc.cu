@@ -7,8 +7,10 @@
 //
 // with P = exp(S - lse) and delta_i = dO_i.O_i, which the first kernel leaves for the second.  Scores are computed in both (7 products
 // where one kernel would do with 5): a single kernel would have to add up dQ over blocks, by atomics in no fixed order, in a
-// fp32 array of its own.  P and dS are rounded to the operands' type, as every operand of the tensor cores is; fp16 thus
-// limits |P (dP - delta)| to 65,504.
+// fp32 array of its own.  P and dS are rounded to the operands' type, as every operand of the tensor cores is.  fp16 has five bits of exponent,
+// so there P (dP - delta) is multiplied by a power of two first that brings the largest |dO| to 4 .. 8, and the sums are divided by it again: a power for
+// every row in the dQ kernel, one for all rows that a block goes through in the other, from what the first kernel leaves for each tile.  (It costs
+// nothing: dP comes in by an FMA, and delta is multiplied once.)  Beyond 65,504 rows are computed anew (attention_strict.cuh).
 //
 //   warps 0-15  a row of the block in every thread, a quarter of the tile's columns in each group of four warps: scores from tensor
 //               memory, weights and score gradients back to it;
@@ -37,6 +39,7 @@ using tc::mbar_init;
 using tc::F2;
 
 constexpr int T = 128;
+static_assert(T == DO_TILE, "the workspace has a place for every tile");
 constexpr int ROW_WARPS = 16, MMA_WARP = 16, LOAD_WARP = 17, STATS_WARP = 18, THREADS = 640;
 constexpr int MINE = 32;  // columns of a thread
 constexpr uint32_t TMEM_COLUMNS = 512, S_AT = 0, DP_AT = 128;
@@ -58,6 +61,20 @@ template <int DP, bool KV> struct Shape {
     static constexpr int SMEM = (2 + SLOTS0 + SLOTS1) * TILE_BYTES;
 };
 
+// Power of two that brings `most` to 4 .. 8 (1 for zero), and its inverse; fp16 values and their maxima, not infinite.
+__device__ __forceinline__ float power_for(float most) { return most > 0.f ? __uint_as_float((256u - (__float_as_uint(most) >> 23)) << 23) : 1.f; }
+__device__ __forceinline__ float inverse_power(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
+// The largest finite magnitude of eight fp16 values, as fp16 bits
+__device__ __forceinline__ unsigned most_finite(const uint4 &v)
+{
+    unsigned m = 0;
+    for (unsigned w : {v.x, v.y, v.z, v.w}) {
+        w &= 0x7fff7fffu;
+        m = __vmaxu2(m, w & __vcmpltu2(w, 0x7c007c00u));
+    }
+    return max(m & 0xffffu, m >> 16);
+}
+
 __device__ __forceinline__ F2 pick(const ulonglong2 &v, int second) { return second ? v.y : v.x; }
 
 template <class E, int DP, bool CAP, bool BIAS, bool KV>
@@ -66,13 +83,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
     using Sh = Shape<DP, KV>;
     constexpr int BOXES = Sh::BOXES, TILE_BYTES = Sh::TILE_BYTES, BOX_BYTES = Sh::BOX_BYTES, SLOTS0 = Sh::SLOTS0, SLOTS1 = Sh::SLOTS1;
     constexpr bool BF16 = !std::is_same<E, __half>::value;
+    constexpr bool POWER = !BF16;
     extern __shared__ __align__(1024) unsigned char smem[];  // the block's two tiles, the two rings
     // dQ: s_full = scores and dP there, p_ready = they have been read.  ds_ready, of even and odd tiles: in the dQ kernel a warp may be done with
     // the next tile before another is done with this one, and its arrival must not count for this one.
     __shared__ uint64_t own_full, full[SLOTS0 + SLOTS1], empty[SLOTS0 + SLOTS1], s_full, dp_full, p_ready, ds_ready[2], acc_full, tail, stats_full[2];
     __shared__ uint32_t tmem_holder, bad[4];
-    __shared__ __align__(16) float stats[KV ? 4 : 2][T];  // dQ: lse and delta of the rows; else of the columns, of two tiles
-    float *const row_lse = stats[0], *const row_delta = stats[1];
+    __shared__ __align__(16) float stats[KV ? 4 : 3][T];  // dQ: lse, delta and the largest |dO| of the rows; else lse and delta of the columns, of two tiles
+    __shared__ unsigned warp_most[THREADS / 32];
+    float *const row_lse = stats[0], *const row_delta = stats[1], *const row_most = stats[KV ? 0 : 2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const unsigned blocks = gridDim.x / p.n_splits, block_of = blockIdx.x / p.n_splits, part = blockIdx.x % p.n_splits;
     const int heads = KV ? p.kv_heads : p.q_heads, head = block_of % heads, kv = KV ? head : head / p.group;
@@ -120,6 +139,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
         mbar_fence_init();
     }
     if (threadIdx.x < 4) bad[threadIdx.x] = 0;
+    if (POWER && KV) {
+        unsigned most = 0;  // (as bits: none is negative)
+        for (int j = threadIdx.x; j < count; j += THREADS) most = max(most, __float_as_uint(p.d_o_most[tile_index(p, s, seq, head_at(j), tile_at(j) / T)]));
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) warp_most[warp] = most;
+    }
     if (warp == MMA_WARP) tc::tmem_alloc(&tmem_holder, TMEM_COLUMNS);
     const int group = warp >> 2, row = (warp & 3) * 32 + lane;  // of warps 0-15: columns MINE * group .. of that row
     tc::fence_before();
@@ -127,6 +152,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
     tc::fence_after();
     const uint32_t tmem = tmem_holder, base = tc::smem_u32(smem), ring = base + 2 * TILE_BYTES;
     bool ok = true;
+    float power = 1.f;  // fp16: of the row (dQ) or of the block
+    if (POWER && KV) {
+        unsigned most = 0;
+        for (int w = 0; w < THREADS / 32; ++w) most = max(most, warp_most[w]);
+        power = power_for(__uint_as_float(most));
+    }
 
     if (warp >= ROW_WARPS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 " OTHER_REGISTERS ";");
@@ -177,7 +208,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                     const int i = tile + 32 * x + lane;
                     const float l = i < s.nq ? __ldg(p.lse + at + i) : -INFINITY, d = i < s.nq ? __ldg(p.delta + at + i) : 0.f;
                     stats[(2 * j & 2)][32 * x + lane] = l == -INFINITY ? -INFINITY : -l * LOG2E;  // nothing seen: weights of zero
-                    stats[(2 * j & 2) + 1][32 * x + lane] = -d;
+                    stats[(2 * j & 2) + 1][32 * x + lane] = POWER ? -d * power : -d;
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&stats_full[j & 1]);
@@ -305,6 +336,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                 for (int e = 0; e < 8; ++e) d = fmaf(to_f(a[e]), to_f(b[e]), d);
 #pragma unroll
                 for (int x = LANES / 2; x >= 1; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
+                if (POWER) {
+                    unsigned most = most_finite(d_o[k]);
+#pragma unroll
+                    for (int x = LANES / 2; x >= 1; x >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, x));
+                    if (lane % LANES == 0) row_most[r] = __half2float(__ushort_as_half((unsigned short)most));
+                }
                 if (lane % LANES == 0) {
                     const int64_t at = (int64_t)head * p.q_rows + s.q0 + r0 + r;
                     row_delta[r] = d;
@@ -313,6 +350,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                 }
             }
             asm volatile("bar.sync 1, %0;" ::"n"(ROW_WARPS * 32) : "memory");  // (all row warps come here, and nothing before can keep one)
+            if (POWER && warp == 0 && part == 0) {
+                unsigned most = 0;
+                for (int r = lane; r < T; r += 32) most = max(most, __float_as_uint(row_most[r]));
+                most = __reduce_max_sync(0xffffffffu, most);
+                if (lane == 0) p.d_o_most[tile_index(p, s, seq, head, block)] = __uint_as_float(most);
+            }
         }
         const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const float c = !CAP ? p.scale * LOG2E : p.of_cap, top_of = p.cap * LOG2E;
@@ -333,7 +376,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             pre = s.prefix;
             lo = p.window.left < 0 ? 0 : max(0, pos - p.window.left);
             hi = p.window.right < 0 ? s.nk - 1 : min(s.nk - 1, pos + p.window.right);
-            delta = -row_delta[row];
+            if (POWER) power = power_for(row_most[row]);
+            delta = POWER ? -row_delta[row] * power : -row_delta[row];
             lse2 = row_lse[row] == -INFINITY ? -INFINITY : -row_lse[row] * LOG2E;  // a row that has seen nothing: weights of zero
         }
         int next_tile = KV && count > 0 ? tile_at(0) : 0, next_head = KV && count > 0 ? head_at(0) : 0;  // dK, dV
@@ -429,7 +473,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             for (int u = 0; u < MINE / 2; ++u) {
                 const F2 d = KV ? pick(reinterpret_cast<const ulonglong2 *>(my_delta)[u / 2], u & 1) : tc::two(delta, delta);
                 float g0, g1;
-                tc::split(tc::mul2(x[u], tc::add2(y[u], d)), g0, g1);
+                tc::split(tc::mul2(x[u], POWER ? tc::ffma2(y[u], tc::two(power, power), d) : tc::add2(y[u], d)), g0, g1);
                 w[u] = tc::pack<E>(g0, g1);
             }
             if (!open) {
@@ -451,7 +495,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             const HeadArray &to = KV ? (group < 2 ? p.dv : p.dk) : p.dq;
             const int first = COLUMNS * (KV ? group & 1 : group);
             const uint32_t from_column = (KV ? (group < 2 ? DV_AT : DK_AT) : DQ_AT) + first;
-            const float by = KV && group < 2 ? 1.f : p.scale;
+            const float by = KV && group < 2 ? 1.f : POWER ? p.scale * inverse_power(power) : p.scale;
             float zero = 0.f;  // NaN as soon as a result is not finite
             if (first < DP) {
                 unsigned char *const stage = smem + warp * 32 * COLUMNS * 2;  // the block's own tiles are done with
