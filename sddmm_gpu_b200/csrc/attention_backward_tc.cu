@@ -84,6 +84,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
     constexpr int BOXES = Sh::BOXES, TILE_BYTES = Sh::TILE_BYTES, BOX_BYTES = Sh::BOX_BYTES, SLOTS0 = Sh::SLOTS0, SLOTS1 = Sh::SLOTS1;
     constexpr bool BF16 = !std::is_same<E, __half>::value;
     constexpr bool POWER = !BF16;
+    // dK, dV in fp16: P times 2^8 as an operand, since the weights of a long sequence are subnormal (one of 60,000 equal ones was off by 2^-9.5 of itself)
+    constexpr float RAISED = POWER && KV ? 8.f : 0.f, RAISE_BY = POWER && KV ? 256.f : 1.f;
     extern __shared__ __align__(1024) unsigned char smem[];  // the block's two tiles, the two rings
     // dQ: s_full = scores and dP there, p_ready = they have been read.  ds_ready, of even and odd tiles: in the dQ kernel a warp may be done with
     // the next tile before another is done with this one, and its arrival must not count for this one.
@@ -156,7 +158,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
     if (POWER && KV) {
         unsigned most = 0;
         for (int w = 0; w < THREADS / 32; ++w) most = max(most, warp_most[w]);
-        power = power_for(__uint_as_float(most));
+        power = power_for(__uint_as_float(most)) * (1.f / RAISE_BY);  // (for a product with raised weights)
     }
 
     if (warp >= ROW_WARPS) {
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                 for (int x = 0; x < T / 32; ++x) {
                     const int i = tile + 32 * x + lane;
                     const float l = i < s.nq ? __ldg(p.lse + at + i) : -INFINITY, d = i < s.nq ? __ldg(p.delta + at + i) : 0.f;
-                    stats[(2 * j & 2)][32 * x + lane] = l == -INFINITY ? -INFINITY : -l * LOG2E;  // nothing seen: weights of zero
+                    stats[(2 * j & 2)][32 * x + lane] = l == -INFINITY ? -INFINITY : fmaf(-l, LOG2E, RAISED);  // nothing seen: weights of zero
                     stats[(2 * j & 2) + 1][32 * x + lane] = POWER ? -d * power : -d;
                 }
                 __syncwarp();
@@ -495,7 +497,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             const HeadArray &to = KV ? (group < 2 ? p.dv : p.dk) : p.dq;
             const int first = COLUMNS * (KV ? group & 1 : group);
             const uint32_t from_column = (KV ? (group < 2 ? DV_AT : DK_AT) : DQ_AT) + first;
-            const float by = KV && group < 2 ? 1.f : POWER ? p.scale * inverse_power(power) : p.scale;
+            const float by = (KV && group < 2 ? 1.f : POWER ? p.scale * inverse_power(power) : p.scale) * (1.f / RAISE_BY);
             float zero = 0.f;  // NaN as soon as a result is not finite
             if (first < DP) {
                 unsigned char *const stage = smem + warp * 32 * COLUMNS * 2;  // the block's own tiles are done with

@@ -105,3 +105,22 @@ def test_no_gradient_at_all(engine):
     for g in _gradients(plan, p, O, l, torch.zeros_like(p.dO)):
         assert bool((g == 0).all())
     plan.close()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [60000, 200000])
+def test_weights_of_many_keys(engine, d, n):
+    # equal weights of 1 / n, below the least normal value of fp16
+    nq = 70
+    p = Problem(F16, d, 1, 1, [nq], [n])
+    p.Q.zero_()
+    p.dO.fill_(128.0)
+    plan = p.plan(engine)
+    O, l = torch.empty_like(p.Q), torch.empty((1, nq), device="cuda")
+    plan.forward(p.Q, p.K, p.V, O, l)
+    _, dK, dV = _gradients(plan, p, O, l, p.dO)
+    assert plan.last_kernel_name() == "attention_backward_tc"
+    # a weight: half a step, and exp (2^-19: its argument is of 2^5); dV: half a step, and where it is subnormal 2^-25
+    within(dV, torch.full_like(dV, nq * 128.0 / n, dtype=torch.float64), nq * 128.0 / n * (2.0 ** -10 + 2.0 ** -18) + 2.0 ** -25, "dV")
+    assert bool((dK == 0).all())
+    plan.close()
