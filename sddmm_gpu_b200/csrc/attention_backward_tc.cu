@@ -204,11 +204,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
             for (int j = 0; j < count && ok; ++j) {
                 if (j >= 2) ok = tc::warp_wait(&ds_ready[j & 1], (j - 2) >> 1 & 1);  // of tile j - 2: the rows are done with its values
                 if (!ok) break;
-                const int64_t at = (int64_t)of * p.q_rows + s.q0;
+                const int64_t at = (int64_t)of * p.q_rows + s.q0;  // (delta: an ordinary load, the kernel before wrote it while this one may have been there)
 #pragma unroll
                 for (int x = 0; x < T / 32; ++x) {
                     const int i = tile + 32 * x + lane;
-                    const float l = i < s.nq ? __ldg(p.lse + at + i) : -INFINITY, d = i < s.nq ? __ldg(p.delta + at + i) : 0.f;
+                    const float l = i < s.nq ? __ldg(p.lse + at + i) : -INFINITY, d = i < s.nq ? p.delta[at + i] : 0.f;
                     stats[(2 * j & 2)][32 * x + lane] = l == -INFINITY ? -INFINITY : fmaf(-l, LOG2E, RAISED);  // nothing seen: weights of zero
                     stats[(2 * j & 2) + 1][32 * x + lane] = POWER ? -d * power : -d;
                 }
