@@ -44,7 +44,7 @@ struct AttentionParams {
 
 __device__ __forceinline__ void report_bad_index(int *dev_status)
 {
-    *reinterpret_cast<volatile int *>(dev_status) = (int)DEV_BAD_INDEX;
+    reinterpret_cast<volatile int *>(dev_status)[BAD_INDEX_WORD] = (int)DEV_BAD_INDEX;
     __threadfence_system();
 }
 

@@ -78,8 +78,10 @@ inline cudaError_t optin_dynamic_smem(Kern kern, size_t bytes, SmemOptinCache &c
     return e;
 }
 
-// Device status word: written by kernels whose bounded waits give up, or that met an index outside its array and left it out.
-enum DeviceStatus : int { DEV_OK = 0, DEV_MBARRIER_TIMEOUT = 1, DEV_BAD_INDEX = 2 };
+// Device status words, one for each thing that kernels report, so that neither is written over: bounded waits that gave up, and an index outside
+// its array that was left out (that many words further).
+enum DeviceStatus : int { DEV_OK = 0, DEV_MBARRIER_TIMEOUT = 1, DEV_BAD_INDEX = 1 };
+constexpr int BAD_INDEX_WORD = 1;
 
 struct PanelConfig {
     int panel_rows;      // rows of W per staged panel

@@ -222,16 +222,19 @@ struct CallTimer {
     }
 };
 
-// After a synchronising point: turn the device status word into a status code.
+// After a synchronising point: turn the device status words into a status code.  Of two reports the wait comes first, the index at the next such point.
 int check_device_status(sddmm_handle_s *h)
 {
     volatile int *status = h->h_status;
-    const int found = *status;
-    if (found != DEV_OK) {
+    if (*status != DEV_OK) {
         *status = DEV_OK;
-        h->last_error = found == DEV_BAD_INDEX ? "an offset, length or row index on the device leaves its array or the plan's limits; what it names was left out"
-                                               : "a bounded device-side wait (mbarrier) gave up";
-        return found == DEV_BAD_INDEX ? SDDMM_INDEX_OUT_OF_RANGE : SDDMM_DEVICE_TIMEOUT;
+        h->last_error = "a bounded device-side wait (mbarrier) gave up";
+        return SDDMM_DEVICE_TIMEOUT;
+    }
+    if (status[BAD_INDEX_WORD] != DEV_OK) {
+        status[BAD_INDEX_WORD] = DEV_OK;
+        h->last_error = "an offset, length or row index on the device leaves its array or the plan's limits; what it names was left out";
+        return SDDMM_INDEX_OUT_OF_RANGE;
     }
     return SDDMM_OK;
 }
@@ -485,7 +488,7 @@ int sddmm_create(sddmm_handle_t *out, int device)
     if (e == cudaSuccess) e = cudaMalloc((void **)&h->d_clocks, 2 * sizeof(unsigned long long) * N_KERNEL_CLOCKS);
     if (e == cudaSuccess) e = cudaMemset(h->d_clocks, 0, 2 * sizeof(unsigned long long) * N_KERNEL_CLOCKS);
     if (e == cudaSuccess) e = cudaMalloc((void **)&h->d_work_counters, sizeof(unsigned long long) * SDDMM_WORK_COUNTERS);
-    // mapped host memory: the status word, and at 64 bytes the words that plan-time kernels answer in
+    // mapped host memory: the status words, and at 64 bytes the words that plan-time kernels answer in
     if (e == cudaSuccess) e = cudaHostAlloc((void **)&h->h_status, 64 + sizeof(unsigned long long) * PICK_MAX, cudaHostAllocMapped);
     if (e == cudaSuccess) e = cudaHostGetDevicePointer((void **)&h->d_status, h->h_status, 0);
     if (e == cudaSuccess) e = cudaMalloc((void **)&h->d_plan_words, sizeof(unsigned long long) * PLAN_WORDS);
@@ -496,7 +499,7 @@ int sddmm_create(sddmm_handle_t *out, int device)
         sddmm_destroy(h);
         return SDDMM_CUDA_ERROR;
     }
-    *h->h_status = DEV_OK;
+    h->h_status[0] = h->h_status[BAD_INDEX_WORD] = DEV_OK;
     h->h_words = reinterpret_cast<volatile unsigned long long *>(h->h_status + 16);
     h->d_words = reinterpret_cast<unsigned long long *>(h->d_status + 16);
     h->free_clocks.reserve(N_KERNEL_CLOCKS);

@@ -34,7 +34,7 @@ struct sddmm_handle_s {
     cudaEvent_t ev_begin[SDDMM_EVENT_PAIRS] = {}, ev_end[SDDMM_EVENT_PAIRS] = {};
     sddmm_plan_s *ev_owner[SDDMM_EVENT_PAIRS] = {};
     int next_pair = 0;
-    int *h_status = nullptr;  // status word of bounded waits, in mapped host memory
+    int *h_status = nullptr;  // status words of bounded waits and of bad indexes, in mapped host memory
     int *d_status = nullptr;  // its device address
     // dynamic work distribution of the ring kernel: a counter for each launch, taken in turn, since launches on other streams may overlap
     unsigned long long *d_work_counters = nullptr;
