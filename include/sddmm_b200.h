@@ -248,7 +248,9 @@ SDDMM_API const char *sddmm_attention_last_kernel(sddmm_attention_t a);
  *
  * One launch turns up to four arrays of the same rows (Q and K; V with rotate = 0 is only copied), each to dst, which may be src itself
  * with the same strides, or to listed rows of dst (a cache): row i goes to row dst_rows[i]; negative: it is not stored; n_dst_rows or more: it is
- * left out and reported as SDDMM_INDEX_OUT_OF_RANGE, as above.  Listed rows must differ from one another.
+ * left out and reported as SDDMM_INDEX_OUT_OF_RANGE, as above.  Listed rows must differ from one another.  Otherwise what is written must not
+ * overlap what any part reads or another writes; parts that begin at the same address are refused, but for two that store to one dst by lists of
+ * their own (whose rows must differ, too).
  */
 enum { SDDMM_ROTARY_HALF = 0, SDDMM_ROTARY_INTERLEAVED = 1 };
 typedef struct {

@@ -257,6 +257,16 @@ int sddmm_rotary(sddmm_handle_t h, const sddmm_rotary_desc *d, const sddmm_rotar
         any = true;
     }
     if (!any) return SDDMM_OK;
+    // What is written is read by no other thread and written by no other: in place, thread by thread; or rows of a cache by different lists
+    for (int i = 0; i < n_parts; ++i) {
+        if (p.part[i].turn + p.part[i].copy == 0) continue;
+        for (int j = 0; j < n_parts; ++j) {
+            const bool in_place = i == j && parts[i].src_row_stride == parts[i].dst_row_stride && parts[i].src_head_stride == parts[i].dst_head_stride && !parts[i].dst_rows;
+            const bool lists = parts[i].dst_rows && parts[j].dst_rows && parts[i].dst_rows != parts[j].dst_rows;
+            if ((parts[i].dst == parts[j].src && !in_place) || (i != j && parts[i].dst == parts[j].dst && !lists))
+                return bad(h, "part " + std::to_string(i) + " writes what part " + std::to_string(j) + " reads or writes");
+        }
+    }
     // Heads a thread takes: its sines serve all of them; fewer where that leaves the GPU without enough threads
     int64_t threads = 0;
     for (int i = 0; i < n_parts; ++i) threads += (int64_t)(p.part[i].turn + p.part[i].copy) / V * p.part[i].heads * d->n_rows;
