@@ -243,8 +243,9 @@ SDDMM_API const char *sddmm_attention_last_kernel(sddmm_attention_t a);
 /*
  * Rotary positions (no counterpart in the reference): the first rot_dim elements of every head are rot_dim / 2 pairs, (i, i + rot_dim / 2)
  * or interleaved (2i, 2i + 1); pair i of a row at position t is turned by the angle t * frequencies[i] (radians) and multiplied by magnitude;
- * the rest of the head is copied.  inverse: turned back, and multiplied by the same magnitude: the gradient of the rotation.  Angles are
- * exact to 2^-25 of half a turn for every 64-bit position.
+ * the rest of the head is copied.  inverse: turned back, and multiplied by the same magnitude: the gradient of the rotation.  Frequencies are
+ * below 2^64 in magnitude.  An angle is off by at most |t| 2^-64 turns (a frequency is held as turns a position, to 64 bits behind the point) and
+ * 2^-25 of half a turn: by next to nothing more than the latter up to positions of 2^38.
  *
  * One launch turns up to four arrays of the same rows (Q and K; V with rotate = 0 is only copied), each to dst, which may be src itself
  * with the same strides, or to listed rows of dst (a cache): row i goes to row dst_rows[i]; negative: it is not stored; n_dst_rows or more: it is

@@ -3,9 +3,10 @@
 //   (a, b) -> m (a cos - b sin, b cos + a sin),
 //
 // for up to four arrays of the same rows in one launch (Q, K and, only copied, V), each to an array of its own, in place, or to listed rows
-// (of a cache).  A frequency comes as turns a position in 64 bits behind the point, so that position * frequency modulo one turn is an
-// integer product that wraps: exact for every 64-bit position, near or far; its upper 32 bits become the argument of
-// sincospi (off by 2^-25 of half a turn).  The inverse turns the other way: also the gradient of the rotation.
+// (of a cache).  A frequency comes as turns a position, whole turns left out, cut to 64 bits behind the point, so that position * frequency modulo
+// one turn is an integer product that wraps, near or far; its upper 32 bits become the argument of sincospi.  The angle is thus off by
+// |position| 2^-64 turns, from the cut, and 2^-25 of half a turn, from the argument: the first is the lesser up to positions of 2^38.  The inverse
+// turns the other way: also the gradient of the rotation.
 //
 // What bounds it: DRAM, and next to it the sines (56 % of the issue slots at 25 % occupancy).  A thread keeps the sines of V pairs (16 bytes
 // of each half) of one row and takes up to HEADS heads, whose loads are all asked for before the first is used.  32,768 rows of
@@ -159,6 +160,30 @@ cudaError_t by_vector(int V, const RotaryParams &p, int n_parts, cudaStream_t s)
     }
 }
 
+constexpr double MOST_FREQUENCY = 18446744073709551616.0;  // 2^64 radians a position
+// f radians (|f| < 2^64) as turns, whole ones left out, cut to 64 bits behind the point: f = m 2^e times 1 / (2 pi), in whole numbers.
+uint64_t turns_of(double f)
+{
+    // 256 bits of 1 / (2 pi), the last ones first (by Machin's formula for pi): off by 2^-192 turns for the largest f
+    static constexpr uint64_t PER_RADIAN[4] = {0x7f9458eaf7aef158u, 0x36d8a5664f10e410u, 0x7f09d5f47d4d3770u, 0x28be60db9391054au};
+    if (f == 0) return 0;
+    int e;
+    const uint64_t m = (uint64_t)std::ldexp(std::frexp(std::fabs(f), &e), 53);
+    uint64_t product[5], carry = 0;
+    for (int i = 0; i < 4; ++i) {
+        const unsigned __int128 x = (unsigned __int128)m * PER_RADIAN[i] + carry;
+        product[i] = (uint64_t)x;
+        carry = (uint64_t)(x >> 64);
+    }
+    product[4] = carry;
+    // |f| = m 2^(e - 53); product 2^(e - 53 - 256) turns, of which the bits from 2^-64 to 2^-1 are wanted
+    const int shift = 192 + 53 - e, word = shift / 64, bit = shift % 64;
+    uint64_t t = 0;
+    if (word < 5) t = product[word] >> bit;
+    if (bit && word + 1 < 5) t |= product[word + 1] << (64 - bit);
+    return f < 0 ? 0 - t : t;
+}
+
 int bad(sddmm_handle_s *h, const std::string &why)
 {
     h->last_error = why;
@@ -216,12 +241,8 @@ int sddmm_rotary(sddmm_handle_t h, const sddmm_rotary_desc *d, const sddmm_rotar
     p.interleaved = d->layout == SDDMM_ROTARY_INTERLEAVED;
     p.status = h->d_status;
     for (int i = 0; i < p.half; ++i) {
-        if (!std::isfinite(d->frequencies[i])) return bad(h, "a frequency is not finite");
-        // radians to turns; whole turns fall away; 64 bits behind the point
-        long double t = (long double)d->frequencies[i] / 6.283185307179586476925286766559005768L;
-        if (d->inverse) t = -t;
-        if (t < 0 || t >= 1) t -= floorl(t);
-        p.turns[i] = t >= 1.0L ? 0 : (uint64_t)(t * 18446744073709551616.0L);
+        if (!(std::fabs(d->frequencies[i]) < MOST_FREQUENCY)) return bad(h, "a frequency is not finite, or of 2^64 radians or more");
+        p.turns[i] = turns_of(d->inverse ? -d->frequencies[i] : d->frequencies[i]);
     }
     // Elements of an access: 16 bytes, or as many as all pieces, addresses and strides are multiples of
     int V = (int)(16 / size);
