@@ -118,7 +118,7 @@ __device__ __forceinline__ void output_row(const AttentionParams &p, const Seque
 template <class T>
 __device__ __forceinline__ void dq_row(const AttentionParams &p, const Sequence &s, int head, int i, float lse, float delta)
 {
-    if (isnan(lse) || isnan(delta)) return;
+    if (isnan(lse) || (isnan(delta) && lse != -INFINITY)) return;  // (a row that sees nothing has no gradient, whatever dO holds)
     const int kv = head / p.group, pos = s.nk - s.nq + i;
     const float slope = p.slopes ? __ldg(p.slopes + head) : 0.f;
     float q[PER_LANE], d_o[PER_LANE], k[PER_LANE], v[PER_LANE], dq[PER_LANE] = {}, dcap;
