@@ -205,8 +205,9 @@ int sddmm_attention_forward(sddmm_attention_t a, const sddmm_head_array *Q, cons
     if (need > 0 && (workspace_bytes < need || !on_device(workspace, h->device) || (uintptr_t)workspace % 16))
         return bad(h, "workspace: sddmm_attention_workspace() bytes of device memory, 16-byte aligned");
     if (!(flags & SDDMM_FLAG_ASYNC) && capturing(h->stream)) return bad(h, "a captured call must be asynchronous");
-    if (p.n_seqs == 0 || p.max_q == 0) return SDDMM_OK;
-    if (a->tensor_cores) {
+    if (p.n_seqs == 0) return SDDMM_OK;
+    // (no queries: the general kernel has one block, which looks whether the sequences agree)
+    if (a->tensor_cores && p.max_q > 0) {
         bool taken = false;
         const ForwardPlan &f = a->by_few ? a->few : a->prompt;
         const cudaError_t e = a->by_few ? launch_attention_few_tc(p, f, workspace, &taken, h->stream) : launch_attention_forward_tc(p, f, workspace, &taken, h->stream);
@@ -254,10 +255,11 @@ int sddmm_attention_backward(sddmm_attention_t a, const sddmm_head_array *Q, con
     p.d_o_most = reinterpret_cast<float *>(static_cast<char *>(workspace) + delta_bytes(p));
     p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + delta_bytes(p) + most_bytes(p));
     if (!(flags & SDDMM_FLAG_ASYNC) && capturing(h->stream)) return bad(h, "a captured call must be asynchronous");
-    if (p.n_seqs == 0 || (p.max_q == 0 && p.max_k == 0)) return SDDMM_OK;
+    if (p.n_seqs == 0) return SDDMM_OK;
+    const bool nothing = p.max_q == 0 && p.max_k == 0;  // (as in the forward call)
     bool taken = false;
     const int launches = 2 + (a->parts.n_q > 1) + (a->parts.n_kv > 1);
-    const cudaError_t e = a->tensor_cores ? launch_attention_backward_tc(p, a->parts, &taken, h->stream) : cudaSuccess;
+    const cudaError_t e = a->tensor_cores && !nothing ? launch_attention_backward_tc(p, a->parts, &taken, h->stream) : cudaSuccess;
     if (taken) return finish(a, e, "attention_backward_tc", launches, flags);
     // (16-bit types come to the general kernels for their strides or alignment alone)
     if (p.dtype == SDDMM_F32) return finish(a, launch_attention_backward_general(p, a->parts, h->stream), "attention_backward_general", launches, flags);

@@ -553,7 +553,7 @@ template <class T, int DP>
 cudaError_t forward_of(const AttentionParams &p, cudaStream_t s)
 {
     static SmemOptinCache optin;
-    const unsigned grid = (unsigned)(p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, B));
+    const unsigned grid = (unsigned)(p.max_q > 0 ? p.q_heads * most_blocks(p.q_rows, p.n_seqs, p.max_q, B) : 1);
     if constexpr (std::is_same<T, float>::value) {
         static SmemOptinCache optin_parts;
         if (p.n_splits > 1) return launch(attention_forward_general_kernel<T, DP, true>, optin_parts, grid * p.n_splits, smem_of(p.head_dim, 3, 1), p, s);
@@ -564,7 +564,7 @@ template <class T, int DP>
 cudaError_t backward_of(const AttentionParams &p0, const Parts &parts, cudaStream_t s)
 {
     static SmemOptinCache optin_q, optin_kv;
-    const unsigned grid_q = (unsigned)(p0.q_heads * most_blocks(p0.q_rows, p0.n_seqs, p0.max_q, B));
+    const unsigned grid_q = (unsigned)(p0.max_q > 0 || p0.max_k > 0 ? p0.q_heads * most_blocks(p0.q_rows, p0.n_seqs, p0.max_q, B) : 1);
     const unsigned grid_kv = (unsigned)(p0.kv_heads * most_blocks(p0.k_rows, p0.n_seqs, p0.max_k, B));
     AttentionParams p = p0;
     p.n_splits = parts.n_q;
