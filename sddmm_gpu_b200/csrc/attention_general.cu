@@ -238,6 +238,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_forward_general_kernel(c
         __syncthreads();
         if (more) fetch(sv, p.v, t + 1);  // under the next scores
     }
+    arrived<0>();  // (a block without tiles: its rows' copies)
 #pragma unroll
     for (int r = 0; r < 4; ++r) sum[r] = over16(sum[r], true);
 #pragma unroll
@@ -356,6 +357,7 @@ __global__ void __launch_bounds__(THREADS, 2) attention_dq_general_kernel(const 
         __syncthreads();
         if (more) fetch(sk, p.k, t + 1);  // under the next dP
     }
+    arrived<0>();  // (a block without tiles: its rows' copies)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int i = ty + 16 * r;
@@ -456,6 +458,7 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1) attention_dkv_gener
         __syncthreads();
         if (more) fetch(sq, p.q, t + 1);  // under the next dP
     }
+    arrived<0>();  // (a block without tiles: its rows' copies)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         if (4 * ty + r >= m) continue;
