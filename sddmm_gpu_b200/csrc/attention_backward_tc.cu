@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_backward_tc_kernel(const
                     const F2 l2 = KV ? pick(reinterpret_cast<const ulonglong2 *>(my_lse)[u / 2], u & 1) : tc::two(lse2, lse2);
                     F2 z = x[u], dcap = 0;
                     if (CAP) {
-                        const F2 th = decltype(is_small)::value ? tc::tanh2(z, tanh_c) : tc::tanh_any(z, tanh_c, p.pre, c, 1.f, 0.f);
+                        const F2 th = decltype(is_small)::value ? tc::tanh2(z, tanh_c) : tc::tanh_any(tc::mul2(z, tc::two(p.pre, p.pre)), tanh_c, c, 1.f, 0.f);
                         dcap = tc::ffma2(tc::mul2(th, th), tc::two(-1.f, -1.f), tc::two(1.f, 1.f));
                         z = BIAS ? tc::mul2(th, tc::two(top_of, top_of)) : tc::ffma2(th, tc::two(top_of, top_of), l2);
                     }

@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident_blocks(DP)) attention_few
                 for (int e = 0; e < 4; ++e) tc::split(tc::tanh2(tc::two(x[0][e], x[1][e]), tanh_c), x[0][e], x[1][e]);
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) tc::split(tc::tanh_any(tc::two(x[0][e], x[1][e]), tanh_c, p.pre, c, top_of, 0.f), x[0][e], x[1][e]);
+                for (int e = 0; e < 4; ++e) tc::split(tc::tanh_any(tc::two(x[0][e] * p.pre, x[1][e] * p.pre), tanh_c, c, top_of, 0.f), x[0][e], x[1][e]);
             }
         }
 #pragma unroll

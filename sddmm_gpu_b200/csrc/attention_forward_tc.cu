@@ -297,6 +297,10 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                     size = tc::max3_abs(size, a, b);
                 }
                 small = p.pre == 1.f && __all_sync(0xffffffffu, size <= tanh_c.range);
+                if (!small && p.pre != 1.f) {
+#pragma unroll
+                    for (int j = 0; j < COLUMNS / 2; ++j) x[j] = tc::mul2(x[j], tc::two(p.pre, p.pre));
+                }
             }
             if (CAP && BIAS) {
                 if (small) {
@@ -304,7 +308,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                     for (int j = 0; j < COLUMNS / 2; ++j) x[j] = tc::tanh2(x[j], tanh_c);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < COLUMNS / 2; ++j) x[j] = tc::tanh_any(x[j], tanh_c, p.pre, c, top_of, 0.f);
+                    for (int j = 0; j < COLUMNS / 2; ++j) x[j] = tc::tanh_any(x[j], tanh_c, c, top_of, 0.f);
                 }
             }
             if (BIAS) {
@@ -359,7 +363,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                 break;
             }
             now = fmaxf(now, row_most[n_s & 1][t][half ^ 1][row]);
-            if (CAP && !BIAS && now > -INFINITY) now = fmaf(-2.f * top_of, tc::rcp(1.f + tc::ex2(now * p.pre * (2.f * LOG2E * c))), top_of);
+            if (CAP && !BIAS && now > -INFINITY) now = fmaf(-2.f * top_of, tc::rcp(1.f + tc::ex2(now * (2.f * LOG2E * c))), top_of);
             const bool raise = now > most + RAISE;  // (-inf + RAISE = -inf: any row's first)
             if (__any_sync(0xffffffffu, raise)) {
                 const float to = raise ? now : most;
@@ -392,7 +396,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_forward_tc_kernel(const 
                     float e0, e1;
                     if (CAP && !BIAS) {
                         if (decltype(is_small)::value) e = tc::ffma2(x[j], tc::tanh_over_x(x[j], tanh_c), tc::two(less, less));
-                        else e = tc::tanh_any(x[j], tanh_c, p.pre, c, top_of, less);
+                        else e = tc::tanh_any(x[j], tanh_c, c, top_of, less);
                         if (!decltype(all_seen)::value) {
                             tc::split(e, e0, e1);
                             e = tc::two(seen_of[j / 16] & 1u << 2 * (j % 16) ? e0 : -INFINITY, seen_of[j / 16] & 2u << 2 * (j % 16) ? e1 : -INFINITY);

@@ -223,7 +223,7 @@ __device__ __forceinline__ F2 ex2_poly(F2 x)
 }
 // tanh(c x) = x (a polynomial in x^2), where |c x| <= 0.6: Chebyshev interpolation of tanh(y) / y in y^2, off by 9e-8, its coefficients
 // times by c^(2i + 1).  c^9 has to stay among the normal numbers, with room for `by`: c from TANH_LEAST to TANH_MOST.  Where scale / cap is
-// not in there c is 1, and products go by tanh_any(), which multiplies them by it (AttentionParams::pre) first.
+// not in there c is 1, and products are multiplied by it (AttentionParams::pre) first and go by tanh_any().
 constexpr float TANH_LEAST = 2e-4f, TANH_MOST = 1e4f;
 struct Tanh {
     F2 a[5];
@@ -251,19 +251,27 @@ __device__ __forceinline__ F2 tanh_over_x(F2 x, const Tanh &t)
     return p;
 }
 __device__ __forceinline__ F2 tanh2(F2 x, const Tanh &t) { return mul2(tanh_over_x(x, t), x); }
-// by tanh(c pre x) + more of any size, for products a few of which leave the polynomial's range: each by its own size alone, so that what comes
-// out of one does not depend on the others.  Within the range, and with pre = 1, the bits are those of ffma2(x, tanh_over_x(x, t), more), `by`
-// being in t's factors; beyond it by (1 - 2 / (1 + e^2cx)).
-__device__ __forceinline__ F2 tanh_any(F2 x, const Tanh &t, float pre, float c, float by, float more)
+// Both values, each from `near` where |x| <= range, else from `far`; as instructions, so that no lane branches.  (With conditional expressions, and
+// the other way by single values: 4,096 causal tokens, 8 heads of 128, most scores near their cap, 255 us; so 158.)
+__device__ __forceinline__ F2 by_size(F2 x, float range, F2 near, F2 far)
 {
-    float a, b, u, w;
-    x = mul2(x, two(pre, pre));
-    split(x, a, b);
-    split(ffma2(x, tanh_over_x(x, t), two(more, more)), u, w);
+    float a, b, n0, n1, f0, f1;
+    split(x, a, b), split(near, n0, n1), split(far, f0, f1);
+    asm("{\n\t.reg .pred p;\n\tsetp.le.f32 p, %1, %2;\n\tselp.f32 %0, %0, %3, p;\n\t}" : "+f"(n0) : "f"(fabsf(a)), "f"(range), "f"(f0));
+    asm("{\n\t.reg .pred p;\n\tsetp.le.f32 p, %1, %2;\n\tselp.f32 %0, %0, %3, p;\n\t}" : "+f"(n1) : "f"(fabsf(b)), "f"(range), "f"(f1));
+    return two(n0, n1);
+}
+// by tanh(c x) + more of any size, for products a few of which leave the polynomial's range: each by its own size alone, so that what comes out
+// of one does not depend on the others.  Within the range the bits are those of ffma2(x, tanh_over_x(x, t), more), `by` being in t's factors;
+// beyond it by (1 - 2 / (1 + e^2cx)).
+__device__ __forceinline__ F2 tanh_any(F2 x, const Tanh &t, float c, float by, float more)
+{
+    float a, b;
     const float c2 = 2.f * LOG2E * c;
-    u = fabsf(a) <= t.range ? u : fmaf(-2.f * by, rcp(1.f + ex2(a * c2)), by + more);
-    w = fabsf(b) <= t.range ? w : fmaf(-2.f * by, rcp(1.f + ex2(b * c2)), by + more);
-    return two(u, w);
+    split(mul2(x, two(c2, c2)), a, b);
+    split(add2(two(ex2(a), ex2(b)), two(1.f, 1.f)), a, b);
+    const F2 far = ffma2(two(rcp(a), rcp(b)), two(-2.f * by, -2.f * by), two(by + more, by + more));
+    return by_size(x, t.range, ffma2(x, tanh_over_x(x, t), two(more, more)), far);
 }
 // Two values in a word, the first in its lower half.
 template <class T> __device__ __forceinline__ uint32_t pack(float a, float b);
