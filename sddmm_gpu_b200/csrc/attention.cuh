@@ -128,8 +128,8 @@ cudaError_t launch_attention_few_tc(const AttentionParams &p, const ForwardPlan 
 cudaError_t launch_attention_forward_tc(const AttentionParams &p, const ForwardPlan &f, void *workspace, bool *taken, cudaStream_t s);
 ForwardPlan plan_attention_few_f32(const AttentionParams &p, int sm_count);
 cudaError_t launch_attention_few_f32(const AttentionParams &p, const ForwardPlan &f, void *workspace, bool *taken, cudaStream_t s);
-// For the kernels of few rows: how the keys are cut for blocks of `rows` rows, tiles of `keys` keys `warps` warps and `least` tiles or more, `resident` blocks to a multiprocessor; us
-// is the number of rows x keys units in all.
+// For the kernels of few rows: how the keys are cut for blocks of `rows` rows and `warps` warps, in tiles of `keys` keys, `least` of them or more, with
+// `resident` blocks on a multiprocessor.  (us here: the units of rows x keys in all.)
 ForwardPlan plan_few(const AttentionParams &p, int rows, int keys, int warps, int least, int resident, int sm_count);
 constexpr int FEW_ROWS = 16, FEW_KEYS = 16, FEW_F32_KEYS = 16;
 // Rows of a block in fp32.

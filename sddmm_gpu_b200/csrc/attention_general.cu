@@ -645,12 +645,13 @@ ForwardPlan plan_attention_forward_general(const AttentionParams &p, int sm_coun
     for (int64_t n = 1; n <= 128 && (n == 1 || (n <= tiles / 2 && n * bytes <= 256ll << 20)); ++n) {
         const int64_t each = (tiles + n - 1) / n;
         if (n > 1 && (p.dtype != 0 || (tiles + each - 1) / each != n || (int64_t)p.n_seqs * p.max_q * p.q_heads > INT32_MAX)) continue;
-        // A tile of 64 keys takes 6.5 us of a block alone, 7.7 of two together, of 128 columns 10; the join 6 and one for 800 rows.  (us before tiles without masks
-        // were told apart, one part / parts: 64 queries on 2,000 keys, 8 heads of 64, 209 / 23; 1,000 on 1,000 107 / 78, of 128 165 / 107; where blocks fill the GPU
-        // anyway, 1,900 + 1,333 tokens, 268 / 342.)
-        // Waves: whole ones where all blocks have as much to do, else the short ones fill the last.
-        const double full = (double)(blocks * n) / (resident * sm_count), fill = p.window.right >= 0 && p.max_k < 2ll * p.max_q ? full : ceil(full), us = 5. + (n > 1 ? 6. + rows / 800. : 0.) +
-                            (fill > 1. ? fill : 1.) * each * (!narrow ? 10. : blocks * n > sm_count ? 7.7 : 6.5);
+        // A tile of 64 keys takes 6.5 us of a block alone and 7.7 of two together, of 128 columns 10; the join takes 6 and 1 for 800 rows.  One part / parts:
+        // 64 queries on 2,000 keys, 8 heads of 64, 209 / 23 us; 1,000 on 1,000 107 / 78, of 128 165 / 107; where blocks fill the GPU anyway, 1,900 + 1,333
+        // tokens, 268 / 342 (measured before tiles without masks were told apart).
+        // Waves: whole ones where all blocks have as much to do; else the short ones fill the last.
+        const double full = (double)(blocks * n) / (resident * sm_count), fill = p.window.right >= 0 && p.max_k < 2ll * p.max_q ? full : ceil(full);
+        const double tile = !narrow ? 10. : blocks * n > sm_count ? 7.7 : 6.5;
+        const double us = 5. + (n > 1 ? 6. + rows / 800. : 0.) + (fill > 1. ? fill : 1.) * (double)each * tile;
         if (us < best.us) best = ForwardPlan{(int)n, n == 1 ? 1 << 30 : (int)each, n == 1 ? 0 : n * bytes, us};
     }
     return best;

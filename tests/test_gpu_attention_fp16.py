@@ -124,3 +124,19 @@ def test_weights_of_many_keys(engine, d, n):
     within(dV, torch.full_like(dV, nq * 128.0 / n, dtype=torch.float64), nq * 128.0 / n * (2.0 ** -10 + 2.0 ** -18) + 2.0 ** -25, "dV")
     assert bool((dK == 0).all())
     plan.close()
+
+
+def test_many_short_sequences(engine):
+    # every tile of every sequence has a place of its own for its largest |dO|
+    g = torch.Generator().manual_seed(5)
+    q = [int(x) for x in torch.randint(0, 200, (150,), generator=g)]
+    p, plan, O, l = _problem(engine, 64, 4, 2, q, window=(-1, 0))
+    first = _gradients(plan, p, O, l, p.dO)
+    # sequences of different sizes: each is exact by itself
+    by = torch.cat([torch.full((n,), 2.0 ** -(b % 11), dtype=torch.float64) for b, n in enumerate(q)]).cuda()[:, None, None]
+    second = _gradients(plan, p, O, l, (p.dO.double() * by).to(F16))
+    for a, b, what in zip(first, second, ("dQ", "dK", "dV")):
+        a = a.double() * by
+        tol = torch.where((b.double().abs() >= 2.0 ** -13) & (a.abs() >= 2.0 ** -13 * by), 0.0, a.abs() * 2.0 ** -11 + 2.0 ** -25 * (1 + by))
+        within(b, a, tol, what)
+    plan.close()
