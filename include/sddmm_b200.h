@@ -301,8 +301,10 @@ SDDMM_API int sddmm_kernel_launches(sddmm_handle_t h, int64_t *n);
 
 /*
  * Wait for everything enqueued on the handle's stream and report the device
- * status word: SDDMM_DEVICE_TIMEOUT if a bounded device-side wait of any earlier
- * call gave up -- the way to learn the outcome of SDDMM_FLAG_ASYNC calls.  The
+ * status words: SDDMM_DEVICE_TIMEOUT if a bounded device-side wait of any earlier
+ * call gave up, SDDMM_INDEX_OUT_OF_RANGE if one met an index on the device that leaves
+ * its array (of two reports the wait comes first, the index at the next synchronising
+ * call) -- the way to learn the outcome of SDDMM_FLAG_ASYNC calls.  The
  * reference's equivalent is cudaEventSynchronize(stop) (HiPC18/src/sddmm.cu:110).
  */
 SDDMM_API int sddmm_sync(sddmm_handle_t h);
