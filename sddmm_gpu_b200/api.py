@@ -305,7 +305,7 @@ class Handle:
 
     def sync(self):
         """Wait for the handle's stream; raises SddmmError(DEVICE_TIMEOUT) if a bounded device-side wait of
-        an earlier (possibly FLAG_ASYNC) call gave up."""
+        an earlier (possibly FLAG_ASYNC) call gave up, or INDEX_OUT_OF_RANGE if one left out what an index on the device named."""
         self._check(lib().sddmm_sync(self._h))
 
     def upload_rows(self, host, dev, d_row_ids, n_rows, K, cuda_stream=None):
